@@ -3,7 +3,7 @@
  *
  * Every entry point takes plain device pointers and sizes, enqueues its work on the CUDA
  * stream it is given, never synchronises the device and never allocates device memory
- * (the moa_peer_alloc / moa_peer_free pair is the one exception, and says so).
+ * (the moa_peer_alloc / moa_peer_free pair and moa_paged_status are the exceptions, and say so).
  * The return value is a moa_status (0 = MOA_OK); moa_strerror() names it and
  * moa_last_error_detail() gives the CUDA error text of the calling thread's last failure.
  *
@@ -239,6 +239,93 @@ int moa_prefill_fwd(const void* q, const void* k, const void* v, void* out,
 int moa_rope_qk(void* q, void* k, int64_t sb, int64_t sh, int64_t sn, const void* cos, const void* sin,
                 int64_t cos_batch_stride, int64_t cos_token_stride, int B, int H, int64_t N, int D, int dtype,
                 moa_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Paged key/value cache: sequences of different lengths in one batch, query heads that share key/value
+ * heads.  No counterpart in the reference, whose only cache is the ring (one token count for the whole batch,
+ * one ring per head); the span of a head means the same as there (sink_size first tokens, local_size last
+ * tokens: what a ring of that size holds once it has wrapped, MoA/attention/cache_utils.py:1020-1058).
+ *
+ * A pool of num_pages pages holds page_size tokens (a power of two, 1..65536) of KV heads each; token p of
+ * sequence b is in slot p % page_size of page page_table[b, p / page_size].
+ *   k_pages, v_pages  element (page, head, slot, d) at page*xp_page + head*xp_head + slot*xp_slot + d: both
+ *                     (pages, heads, slots, D) and (pages, slots, heads, D) memory orders, and pools that
+ *                     interleave keys and values, are strides.  16-byte aligned, strides multiples of 8
+ *   page_table        int32, row b at page_table + b*table_stride, max_pages entries.  Entries that hold no
+ *                     token are never read through (they may be anything, -1 for instance)
+ *   lengths           (B) int32, tokens in the pages before the call.  Advanced by the call when `advance` is
+ *                     set, else left as they are
+ *   rope_cos/sin      NULL, or tables of D-wide rows: with rope_rows == 0 the row of token i of sequence b is at
+ *                     b*rope_sb + i*rope_sn, with rope_rows > 0 the row of position p is at p*rope_sn.
+ *                     In the tensors' dtype, or float32 with rope_f32 set.  16-byte aligned rows
+ * The library trusts no index: a token whose page (or, by position, rope row) does not exist is not stored
+ * and not attended, nothing is read or written for it, and the first such token since the last look is
+ * reported by moa_paged_status:
+ *   {31, sequence, position, 0} an appended token, {32, sequence, position, head} an attended one without a page,
+ *   {33, sequence, position, 0} a position behind the last rope row, {34, sequence, length, 0} a length beyond
+ *   the page table's width (the tokens behind it are left out).
+ * Pages may be shared between sequences for reading.  Two tokens of one call that land in the same place are
+ * the caller's mistake: one of them is stored.
+ *
+ * moa_paged_append: keys and values of new tokens into the pages, the rotary embedding applied to the keys on
+ *   the way when tables are given.  k, v (B, KV, N, D) through the element strides (sb, sh, sn); of sequence b the
+ *   first min(counts[b], N) tokens are stored (counts NULL: all N) at positions lengths[b], lengths[b] + 1, ...;
+ *   lengths[b] < 0 marks a row without a sequence, which is left alone.  With q (B, H, N, D) and q_out, k_out
+ *   (contiguous (B, H, N, D) and (B, KV, N, D)) given (tables are then required) the rotated query and key are
+ *   written there too; rows that are not stored because they lie behind a count are zero there.
+ *
+ * moa_paged_decode: attention of one query token per sequence over its pages.
+ *   q (B, H, D) through (q_sb, q_sh), H a multiple of KV, query head h reads key head h / (H / KV);
+ *   out[b*o_sb + h*o_sh + d], the dtype of q or float32 (out_f32).
+ *   sink_size, local_size (KV) int64, both or none: key head g of a sequence of n tokens attends positions
+ *   < sink_size[g] and >= n - local_size[g]; none: all n.  A head that attends nothing gets zeros.
+ *   k_new, v_new NULL: n = lengths[b].  Given, (B, KV, D) through their strides: the new token is stored at
+ *   position lengths[b] and attended, n = lengths[b] + 1 (lengths[b] < 0: no sequence, nothing is stored and the
+ *   output row is zero); with tables q and k_new are rotated, and the key is attended as it is stored.
+ *   workspace: moa_paged_decode_workspace_bytes() bytes on the current device, the first
+ *   MOA_PAGED_COUNTER_BYTES of them zeroed once; the kernel leaves them zero.  Calls that can overlap in time
+ *   need one each.
+ * Both take their arguments as a struct of 8-byte fields and read it before they return.
+ *
+ * moa_paged_status: copies the status words above to host memory and clears them.  Waits for the device: for
+ *   checks, not for the hot path.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct moa_paged_append_args {
+  const void *k, *v, *q;
+  void *k_pages, *v_pages;
+  const int32_t* page_table;
+  int32_t* lengths;
+  const int32_t* counts;
+  const void *rope_cos, *rope_sin;
+  void *q_out, *k_out;
+  int64_t k_sb, k_sh, k_sn, v_sb, v_sh, v_sn, q_sb, q_sh, q_sn;
+  int64_t kp_page, kp_head, kp_slot, vp_page, vp_head, vp_slot;
+  int64_t table_stride, max_pages, num_pages, page_size;
+  int64_t rope_sb, rope_sn, rope_rows, rope_f32;
+  int64_t B, H, KV, N, D, dtype, advance;
+} moa_paged_append_args;
+
+typedef struct moa_paged_decode_args {
+  const void *q, *k_new, *v_new;
+  void *k_pages, *v_pages, *out;
+  const int32_t* page_table;
+  int32_t* lengths;
+  const int64_t *sink_size, *local_size;
+  const void *rope_cos, *rope_sin;
+  void* workspace;
+  int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh, o_sb, o_sh;
+  int64_t kp_page, kp_head, kp_slot, vp_page, vp_head, vp_slot;
+  int64_t table_stride, max_pages, num_pages, page_size;
+  int64_t rope_sb, rope_sn, rope_rows, rope_f32;
+  int64_t B, H, KV, D, dtype, out_f32, advance, workspace_bytes;
+  double sm_scale;
+} moa_paged_decode_args;
+
+#define MOA_PAGED_COUNTER_BYTES 8192
+int moa_paged_append(const moa_paged_append_args* args, moa_stream_t stream);
+int64_t moa_paged_decode_workspace_bytes(void);
+int moa_paged_decode(const moa_paged_decode_args* args, moa_stream_t stream);
+int moa_paged_status(int32_t status[4]);
 
 /* ------------------------------------------------------------------------------------------
  * Buffers that the GPUs of one node write into directly (what moa_decode_gather_fwd's out_peers point at),

@@ -25,6 +25,7 @@ SYMBOLS = (
     "moa_decode_fwd_static", "moa_decode_rope_fwd", "moa_decode_gather_fwd", "moa_selftest_bounded_wait",
     "moa_rope_qk", "moa_peer_alloc", "moa_peer_free", "moa_peer_export", "moa_peer_open", "moa_peer_close",
     "moa_peer_barrier",
+    "moa_paged_append", "moa_paged_decode", "moa_paged_decode_workspace_bytes", "moa_paged_status",
 )
 
 
@@ -68,10 +69,17 @@ def _load() -> ctypes.CDLL:
     lib.moa_cache_scan_mask.argtypes = [P, I64, P, P, I, I64, P]
     lib.moa_cache_fill.argtypes = [P, P, I64, I64, I64, P, P, P, P, P, P, P, P, P, I64, I, I, I64, I, I64, I64, I, P]
     lib.moa_prefill_fwd.argtypes = [P, P, P, P] + [I64] * 12 + [P, P, I, I, I64, I, c_float, I, I, P, P]
+    # the argument structs of these two (8-byte fields) are packed into bytes by moa_b200/paged.py
+    lib.moa_paged_append.argtypes = [c_char_p, P]
+    lib.moa_paged_decode.argtypes = [c_char_p, P]
+    lib.moa_paged_decode_workspace_bytes.restype = c_int64
+    lib.moa_paged_decode_workspace_bytes.argtypes = []
+    lib.moa_paged_status.argtypes = [P]
     for name in ("moa_decode_workspace_init", "moa_decode_fwd", "moa_decode_rope_fwd", "moa_decode_gather_fwd",
                  "moa_decode_fwd_static", "moa_rope_qk", "moa_selftest_bounded_wait", "moa_cache_append",
                  "moa_cache_scan_mask", "moa_cache_fill", "moa_prefill_fwd", "moa_peer_alloc", "moa_peer_free",
-                 "moa_peer_export", "moa_peer_open", "moa_peer_close", "moa_peer_barrier"):
+                 "moa_peer_export", "moa_peer_open", "moa_peer_close", "moa_peer_barrier",
+                 "moa_paged_append", "moa_paged_decode", "moa_paged_status"):
         getattr(lib, name).restype = c_int
     if lib.moa_abi_version() != ABI_VERSION:
         raise ImportError(f"{LIB_PATH}: ABI version {lib.moa_abi_version()} != {ABI_VERSION}; rebuild it "
@@ -137,6 +145,7 @@ def current_stream(device) -> int:
 
 
 _NVTX = os.environ.get("MOA_B200_NVTX") == "1"
+NO_RANGE = contextlib.nullcontext()
 
 
 def nvtx_range(name: str):
@@ -146,4 +155,4 @@ def nvtx_range(name: str):
         import torch
 
         return torch.cuda.nvtx.range(name)
-    return contextlib.nullcontext()
+    return NO_RANGE

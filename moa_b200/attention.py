@@ -43,8 +43,8 @@ def _status_words(device) -> Tensor:
 
 def check_device_status(device=None) -> None:
     """Synchronise and raise if a kernel on ``device`` reported that one of its bounded waits ran
-    out (its output is then invalid).  Cheap enough for tests and once-per-request checks; the
-    hot path never synchronises."""
+    out (its output is then invalid), or that a paged call left a token out for want of a page.  Cheap
+    enough for tests and once-per-request checks; the hot path never synchronises."""
     want = torch.device(device) if device is not None else None
     if want is not None and want.index is None and want.type == "cuda":
         want = torch.device("cuda", torch.cuda.current_device())
@@ -58,6 +58,9 @@ def check_device_status(device=None) -> None:
             what = _WAIT_NAMES.get(words[0], "?")
             raise _lib.MoaError("moa_prefill_fwd", 5, lib.moa_strerror(5).decode(),
                                 f"wait code {words[0]} ({what}) in block {words[1]} thread {words[3]}")
+    from . import paged
+
+    paged.check_status(want)
 
 
 def _decode_workspace(device, B: int, H: int, D: int, S: int) -> Tensor:

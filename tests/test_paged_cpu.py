@@ -1,0 +1,188 @@
+"""Paged cache without a GPU: what the entry points refuse, and the layout of the argument structs."""
+import ctypes
+import os
+import re
+
+import pytest
+import torch
+
+import moa_b200
+from moa_b200 import _lib, paged
+
+HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "moa_b200.h")
+
+
+def _fields(name):
+    """Field names of a struct of the header, in order."""
+    text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, flags=re.S).group(1)
+    got = []
+    for line in body.split(";"):
+        line = re.sub(r"\b(const|void|int32_t|int64_t|double)\b", " ", line).replace("*", " ")
+        got += [f.strip() for f in line.split(",") if f.strip()]
+    return got
+
+
+def test_packed_arguments_have_the_header_structs_size():
+    assert paged._APPEND.size == 8 * len(_fields("moa_paged_append_args"))
+    assert paged._DECODE.size == 8 * len(_fields("moa_paged_decode_args"))
+    text = open(HEADER).read()
+    assert int(re.search(r"MOA_PAGED_COUNTER_BYTES (\d+)", text).group(1)) == paged._COUNTER_BYTES
+
+
+def _inputs(B=2, H=4, KV=2, N=1, D=64, page=16, dtype=torch.float16):
+    return dict(query=torch.zeros(B, H, N, D, dtype=dtype), key=torch.zeros(B, KV, N, D, dtype=dtype),
+                value=torch.zeros(B, KV, N, D, dtype=dtype), key_pages=torch.zeros(6, KV, page, D, dtype=dtype),
+                value_pages=torch.zeros(6, KV, page, D, dtype=dtype), page_table=torch.zeros(B, 3, dtype=torch.int32),
+                lengths=torch.zeros(B, dtype=torch.int32))
+
+
+def _append(**changes):
+    t = _inputs()
+    t.update(changes)
+    t.pop("query") if "query" not in changes else None
+    return moa_b200.paged_append(**t)
+
+
+def _decode(step=False, **changes):
+    t = _inputs()
+    if not step:
+        t.pop("key"), t.pop("value")
+    t.update(changes)
+    return moa_b200.paged_decode(**t, sm_scale=0.1)
+
+
+def test_cpu_tensors_are_rejected_not_silently_computed():
+    for call in (_append, _decode, lambda: _decode(step=True)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+
+
+TABLE2 = torch.zeros(48, 64, dtype=torch.float16)
+APPEND_BAD = {
+    "key and value differ": dict(value=torch.zeros(2, 2, 2, 64).half()),
+    "fp32": dict(key=torch.zeros(2, 2, 1, 64), value=torch.zeros(2, 2, 1, 64)),
+    "value of another type": dict(value=torch.zeros(2, 2, 1, 64).bfloat16()),
+    "pages of another type": dict(key_pages=torch.zeros(6, 2, 16, 64).bfloat16()),
+    "other heads": dict(key_pages=torch.zeros(6, 3, 16, 64).half(), value_pages=torch.zeros(6, 3, 16, 64).half()),
+    "pages differ": dict(value_pages=torch.zeros(7, 2, 16, 64).half()),
+    "pages with rows that are not contiguous": dict(key_pages=torch.zeros(6, 2, 64, 16).half().transpose(2, 3)),
+    "int64 page table": dict(page_table=torch.zeros(2, 3, dtype=torch.int64)),
+    "page table of another batch": dict(page_table=torch.zeros(3, 3, dtype=torch.int32)),
+    "page table by columns": dict(page_table=torch.zeros(3, 2, dtype=torch.int32).t()),
+    "int64 lengths": dict(lengths=torch.zeros(2, dtype=torch.int64)),
+    "lengths of another batch": dict(lengths=torch.zeros(3, dtype=torch.int32)),
+    "lengths apart": dict(lengths=torch.zeros(4, dtype=torch.int32)[::2]),
+    "int64 counts": dict(counts=torch.zeros(2, dtype=torch.int64)),
+    "counts of another batch": dict(counts=torch.zeros(1, dtype=torch.int32)),
+    "query without tables": dict(query=torch.zeros(2, 4, 1, 64).half()),
+    "query of another length": dict(query=torch.zeros(2, 4, 2, 64).half(), rope=(TABLE2, TABLE2)),
+    "tables of another width": dict(rope=(TABLE2[:, :32], TABLE2[:, :32])),
+    "tables of another type": dict(rope=(TABLE2.bfloat16(), TABLE2.bfloat16())),
+    "tables of two shapes": dict(rope=(TABLE2, TABLE2[:5])),
+    "tables of another batch": dict(rope=(torch.zeros(3, 1, 64).half(), torch.zeros(3, 1, 64).half())),
+    "tables of another length": dict(rope=(torch.zeros(2, 2, 64).half(), torch.zeros(2, 2, 64).half())),
+    "an empty table": dict(rope=(TABLE2[:0], TABLE2[:0])),
+}
+DECODE_BAD = {
+    "two query tokens": dict(query=torch.zeros(2, 4, 2, 64).half()),
+    "heads that do not divide": dict(query=torch.zeros(2, 5, 1, 64).half()),
+    "another head size": dict(query=torch.zeros(2, 4, 1, 128).half()),
+    "key without value": dict(key=torch.zeros(2, 2, 1, 64).half()),
+    "tables without a new token": dict(rope=(TABLE2, TABLE2)),
+    "advance without a new token": dict(advance=True),
+    "sink without local": dict(sink_size=torch.zeros(2, dtype=torch.int64)),
+    "int32 spans": dict(sink_size=torch.zeros(2, dtype=torch.int32), local_size=torch.zeros(2, dtype=torch.int32)),
+    "spans by query head": dict(sink_size=torch.zeros(4, dtype=torch.int64), local_size=torch.zeros(4, dtype=torch.int64)),
+    "int64 page table": dict(page_table=torch.zeros(2, 3, dtype=torch.int64)),
+    "int64 lengths": dict(lengths=torch.zeros(2, dtype=torch.int64)),
+    "pages of another type": dict(value_pages=torch.zeros(6, 2, 16, 64).bfloat16()),
+}
+STEP_BAD = {
+    "key of another batch": dict(key=torch.zeros(1, 2, 1, 64).half(), value=torch.zeros(1, 2, 1, 64).half()),
+    "two new tokens": dict(key=torch.zeros(2, 2, 2, 64).half(), value=torch.zeros(2, 2, 2, 64).half()),
+    "key by query head": dict(key=torch.zeros(2, 4, 1, 64).half(), value=torch.zeros(2, 4, 1, 64).half()),
+    "value of another type": dict(value=torch.zeros(2, 2, 1, 64).bfloat16()),
+    "tables of another length": dict(rope=(torch.zeros(2, 2, 64).half(), torch.zeros(2, 2, 64).half())),
+}
+
+
+@pytest.mark.parametrize("what", APPEND_BAD)
+def test_append_refuses(what):
+    with pytest.raises(AssertionError):
+        _append(**APPEND_BAD[what])
+
+
+@pytest.mark.parametrize("what", DECODE_BAD)
+def test_decode_refuses(what):
+    with pytest.raises(AssertionError):
+        _decode(**DECODE_BAD[what])
+
+
+@pytest.mark.parametrize("what", STEP_BAD)
+def test_step_refuses(what):
+    with pytest.raises(AssertionError):
+        _decode(step=True, **STEP_BAD[what])
+
+
+def test_gradients_are_refused():
+    key = torch.zeros(2, 2, 1, 64).half().requires_grad_()
+    with pytest.raises(NotImplementedError, match="inference"):
+        _append(key=key)
+    with pytest.raises(NotImplementedError, match="inference"):
+        _decode(query=torch.zeros(2, 4, 1, 64).half().requires_grad_())
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):     # and nothing else is wrong with the call
+        _append(key=key)
+
+
+# The C entry points check what they are given before anything is launched, so that the checks can be
+# exercised with made-up (aligned, never read) addresses.
+A = 4096
+APPEND_OK = dict(k=A, v=A, k_pages=A, v_pages=A, page_table=A, lengths=A, k_sb=128, k_sh=64, k_sn=64, v_sb=128, v_sh=64,
+                 v_sn=64, kp_page=2048, kp_head=1024, kp_slot=64, vp_page=2048, vp_head=1024, vp_slot=64, table_stride=3,
+                 max_pages=3, num_pages=6, page_size=16, B=2, H=4, KV=2, N=1, D=64)
+DECODE_OK = dict(q=A, k_pages=A, v_pages=A, out=A, page_table=A, lengths=A, workspace=A, q_sb=256, q_sh=64, o_sb=256,
+                 o_sh=64, kp_page=2048, kp_head=1024, kp_slot=64, vp_page=2048, vp_head=1024, vp_slot=64, table_stride=3,
+                 max_pages=3, num_pages=6, page_size=16, B=2, H=4, KV=2, D=64, workspace_bytes=1 << 40, sm_scale=0.1)
+
+
+def _call_c(entry, packer, good, **changes):
+    values = dict(good)
+    values.update(changes)
+    names = _fields("moa_%s_args" % entry)
+    assert set(values) <= set(names)
+    packed = packer.pack(*[values.get(n, 0) for n in names])
+    return getattr(_lib.lib, "moa_" + entry)(packed, 0)
+
+
+@pytest.mark.parametrize("changes,status,text", [
+    (dict(k=0), 1, b"null"), (dict(k_pages=0), 1, b"null"), (dict(lengths=0), 1, b"null"), (dict(B=0), 1, b"shape"),
+    (dict(B=65536), 1, b"shape"), (dict(N=0), 1, b"number of tokens"), (dict(num_pages=0), 1, b"page table"),
+    (dict(max_pages=0), 1, b"page table"), (dict(page_size=24), 1, b"power of two"), (dict(page_size=1 << 17), 1, b"power of two"),
+    (dict(k_pages=A + 8), 1, b"aligned"), (dict(kp_slot=68), 1, b"aligned"), (dict(v=A + 2), 1, b"aligned"),
+    (dict(k_sn=-64), 1, b"aligned"), (dict(rope_cos=A), 1, b"go together"), (dict(rope_cos=A, rope_sin=A, rope_sn=60), 1, b"rope"),
+    (dict(q=A), 1, b"go together"), (dict(q=A, q_out=A, k_out=A), 1, b"tables"), (dict(D=96), 2, b"head_dim"),
+    (dict(dtype=7), 2, b"dtype"),
+])
+def test_append_entry_checks_its_arguments(changes, status, text):
+    assert _call_c("paged_append", paged._APPEND, APPEND_OK, **changes) == status
+    assert text in _lib.lib.moa_last_error_detail()
+
+
+@pytest.mark.parametrize("changes,status,text", [
+    (dict(q=0), 1, b"null"), (dict(out=0), 1, b"null"), (dict(page_table=0), 1, b"null"), (dict(KV=0), 1, b"shape"),
+    (dict(H=5), 1, b"multiple"), (dict(k_new=A), 1, b"go together"), (dict(sink_size=A), 1, b"go together"),
+    (dict(advance=1), 1, b"new token"), (dict(rope_cos=A, rope_sin=A), 1, b"new token"), (dict(q=A + 2), 1, b"aligned"),
+    (dict(page_size=0), 1, b"power of two"), (dict(workspace=0), 4, b"workspace"), (dict(workspace_bytes=100), 4, b"workspace"),
+    (dict(D=80), 2, b"head_dim"), (dict(dtype=2), 2, b"dtype"),
+])
+def test_decode_entry_checks_its_arguments(changes, status, text):
+    assert _call_c("paged_decode", paged._DECODE, DECODE_OK, **changes) == status
+    assert text in _lib.lib.moa_last_error_detail()
+
+
+def test_null_arguments_are_an_error_not_a_crash():
+    assert _lib.lib.moa_paged_append(None, 0) == 1
+    assert _lib.lib.moa_paged_decode(None, 0) == 1
+    assert _lib.lib.moa_paged_status(0) == 1
+    assert ctypes.sizeof(ctypes.c_void_p) == 8
