@@ -144,15 +144,14 @@ def current_stream(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-_NVTX = os.environ.get("MOA_B200_NVTX") == "1"
-NO_RANGE = contextlib.nullcontext()
+NVTX = os.environ.get("MOA_B200_NVTX") == "1"
 
 
 def nvtx_range(name: str):
     """NVTX range around a launch when ``MOA_B200_NVTX=1`` (the reference's efficiency script marks its
     prefill and decode steps the same way, scripts/evaluate/effieicency_test.py:81-83); a no-op otherwise."""
-    if _NVTX:
+    if NVTX:
         import torch
 
         return torch.cuda.nvtx.range(name)
-    return NO_RANGE
+    return contextlib.nullcontext()

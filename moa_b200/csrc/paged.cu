@@ -4,7 +4,9 @@
 // Token p of sequence b lives in slot p % page_size of page table[b, p / page_size]; every index that
 // comes from device memory (lengths, counts, table entries) is checked against its array before it
 // is used, and a token whose place does not exist is left out and reported in g_paged_status.
+#include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -176,6 +178,37 @@ __global__ void paged_advance_kernel(int32_t* lengths, const int32_t* counts, in
 }
 
 // ---- attention of one token ----------------------------------------------------------------------
+//
+//   o = sum_p w_p v_p / sum_p w_p,   w_p = exp(scale q.k_p - max),   p over the head's span
+//
+// Every key and value row is read once and used for all query heads that share it, G flops a byte: the kernel
+// is bound by memory, and is built to keep loads in flight.
+//
+// Work.  An item is (sequence, key head, tile of up to 8*MT query heads).  Its rows are counted in units of 16;
+// all items' units, and kItemCost more per item for its epilogue, are laid out on one line that is cut into
+// equal parts, one per block (one block per SM).  A block therefore moves the same number of bytes however
+// ragged the lengths are, and the cut is computed on the device from `lengths` alone: nothing is planned on the
+// host, and a captured launch stays right when the lengths change.  An item that is cut leaves one partial
+// result (maximum, sum, sum of values) per block; the block that finishes last joins them, in the blocks'
+// order, so results do not depend on timing.  No block waits for another.
+//
+// Loads.  The 8 warps of a block take the units of a segment in turn.  Each warp runs its own ring of kStages
+// units in shared memory, filled with cp.async by a cursor that runs ahead of the arithmetic, over the ends of
+// items too, so the epilogue of one item overlaps with the loads of the next: 192 KB in flight per SM.
+//
+// Arithmetic.  m16n8k16 tensor instructions with the 8 query heads of a tile in rows 0-7 and, where an operand
+// does not fit 16 bits, its remainder in rows 8-15: the weights w are held to 16 + 16 bits that way (hi + lo),
+// and so is the rotated query of the fused step.  Rows 8-15 would idle otherwise (G is small), so the result has
+// fp32 weights at no cost.  MT = 2 serves 9..16 heads with one pass over the keys.
+constexpr int kWarps = 8, kDecodeThreads = kWarps * 32;
+constexpr int kUnit = 16;                   // rows of a unit (k of the second product)
+constexpr int kItemCost = 2;                // an item's epilogue, in units
+constexpr int kMinUnits = 8;                // least share of a block: fewer blocks work when there is less
+constexpr int kJoin = 16;                   // partial results joined at once
+constexpr int kMaxBlocks = 256;           // kJoin * kJoin: two levels of joining reach it
+constexpr int kRecHeads = 16;
+constexpr int64_t kRecFloats = kRecHeads * (128 + 2);
+
 struct DecodeParams {
   Pool pool;
   const void *q, *k_new, *v_new;
@@ -183,142 +216,612 @@ struct DecodeParams {
   int32_t* lengths;
   const int64_t *sink, *local;
   int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh, o_sb, o_sh;
-  int B, H, KV;
+  int B, H, KV, G, tiles;                   // tiles of query heads per key head
+  int capacity;                             // positions that a row of the page table reaches
   float scale_log2;
-  int out_f32;
+  int out_f32, advance;
+  int* counters;                            // 3 per block, zero between launches, and one behind them
+  float* records;                           // 2 per block
 };
 
-// One block per (query head, sequence): 4 warps walk the rows of the head's span, D/8 lanes a row, with a
-// running maximum and sum each; the block joins them.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_decode_kernel(const __grid_constant__ DecodeParams p) {
-  constexpr int LPR = D / 8, RPI = 32 / LPR, GROUPS = 4 * RPI;
-  __shared__ __align__(16) T sm_q[D], sm_k[D], sm_v[D];
-  __shared__ float sm_m[GROUPS], sm_l[GROUPS];
-  __shared__ float sm_acc[GROUPS][D];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, li = lane % LPR, g = warp * RPI + lane / LPR;
-  const int h = blockIdx.x, G = p.H / p.KV, kh = h / G;
-  const int64_t b = blockIdx.y;
-  const int32_t* table_row = p.pool.table + b * p.pool.table_stride;
-  const int64_t slot_mask = (1ll << p.pool.shift) - 1, capacity = p.pool.max_pages << p.pool.shift;
-  const int64_t len = p.lengths[b];
-  const bool fused = p.k_new != nullptr;
-  int64_t n = fused ? (len < 0 ? 0 : len + 1) : max(len, (int64_t)0);
-  const int64_t pos_new = fused && n > 0 ? len : -1;
-  if (n > capacity) {
-    if (tid == 0 && h == 0) report(kStatusLength, b, n, 0);
-    n = capacity;
+// The rows of one (sequence, key head): positions [0, sink) and [n - (rows - sink), n).
+struct Span {
+  int n, sink, rows;
+};
+
+__device__ __forceinline__ int tokens_of(const DecodeParams& p, int b) {
+  const int len = p.lengths[b];
+  if (len < 0) return 0;
+  const int64_t n = (int64_t)len + (p.k_new ? 1 : 0);
+  return (int)min(n, (int64_t)p.capacity);
+}
+
+__device__ __forceinline__ Span span_of(const DecodeParams& p, int n, int kh) {
+  Span s;
+  s.n = n;
+  s.sink = n;
+  s.rows = n;
+  if (p.sink) {
+    s.sink = (int)min(max(p.sink[kh], (int64_t)0), (int64_t)n);
+    s.rows = (int)min((int64_t)n, s.sink + min(max(p.local[kh], (int64_t)0), (int64_t)n));
   }
-  bool have_new = pos_new >= 0 && pos_new < n;
-  const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_sb + h * p.q_sh;
-  float qf[8];
-  if (have_new) {
-    const int64_t row = p.pool.cos ? rope_row(p.pool, b, 0, pos_new) : 0;
-    const int32_t page = page_of(p.pool, table_row, pos_new);
-    if (row < 0 || page < 0) {
-      if (tid == 0 && h == 0) report(row < 0 ? kStatusRope : kStatusAppend, b, pos_new, 0);
-      have_new = false;
-    }
-    if (tid < D / 16 && row >= 0) {
-      const T* ks = reinterpret_cast<const T*>(p.k_new) + b * p.k_sb + kh * p.k_sh + tid * 8;
-      const T* vs = reinterpret_cast<const T*>(p.v_new) + b * p.v_sb + kh * p.v_sh + tid * 8;
-      uint4 klo = *reinterpret_cast<const uint4*>(ks), khi = *reinterpret_cast<const uint4*>(ks + D / 2);
-      const uint4 vlo = *reinterpret_cast<const uint4*>(vs), vhi = *reinterpret_cast<const uint4*>(vs + D / 2);
-      if (p.pool.cos) rotate_pair<T, D>(p.pool, row, tid, klo, khi);
-      *reinterpret_cast<uint4*>(sm_k + tid * 8) = klo;
-      *reinterpret_cast<uint4*>(sm_k + D / 2 + tid * 8) = khi;
-      *reinterpret_cast<uint4*>(sm_v + tid * 8) = vlo;
-      *reinterpret_cast<uint4*>(sm_v + D / 2 + tid * 8) = vhi;
-      if (have_new && h % G == 0) {
-        T* kd = reinterpret_cast<T*>(p.pool.k) + page * p.pool.k_page + kh * p.pool.k_head + (pos_new & slot_mask) * p.pool.k_slot + tid * 8;
-        T* vd = reinterpret_cast<T*>(p.pool.v) + page * p.pool.v_page + kh * p.pool.v_head + (pos_new & slot_mask) * p.pool.v_slot + tid * 8;
-        *reinterpret_cast<uint4*>(kd) = klo;
-        *reinterpret_cast<uint4*>(kd + D / 2) = khi;
-        *reinterpret_cast<uint4*>(vd) = vlo;
-        *reinterpret_cast<uint4*>(vd + D / 2) = vhi;
+  return s;
+}
+__device__ __forceinline__ int units_of(int rows) { return (rows + kUnit - 1) / kUnit; }
+
+// A walk over the items of a block's part [lo, hi) of the line.
+struct Cursor {
+  int b, kh, tile;
+  int n;                                    // tokens of sequence b
+  Span span;
+  int64_t at;                               // where the item begins on the line
+  int units;
+  int u0, u1;                               // the units of the item that are in the part
+  __device__ __forceinline__ void enter(const DecodeParams& p, int64_t lo, int64_t hi) {
+    span = span_of(p, n, kh);
+    units = units_of(span.rows);
+    u0 = (int)min(max(lo - at, (int64_t)0), (int64_t)units);
+    u1 = (int)min(hi - at, (int64_t)units);
+  }
+  // To the next item; false when it is not in the part.
+  __device__ __forceinline__ bool next(const DecodeParams& p, int64_t lo, int64_t hi) {
+    at += units + kItemCost;
+    if (at >= hi) return false;
+    if (++tile == p.tiles) {
+      tile = 0;
+      if (++kh == p.KV) {
+        kh = 0;
+        ++b;
+        n = tokens_of(p, b);
       }
+    }
+    enter(p, lo, hi);
+    return true;
+  }
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// x = hi + lo with both in T, for two values; hi of an fp16 that does not fit is its largest, lo takes the rest.
+template <typename T>
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  if (std::is_same<T, __half>::value) {
+    hi = Cvt<T>::pack(fminf(fmaxf(x0, -65504.f), 65504.f), fminf(fmaxf(x1, -65504.f), 65504.f));
+  } else {
+    hi = Cvt<T>::pack(x0, x1);
+  }
+  const float2 h = Cvt<T>::unpack(hi);
+  lo = Cvt<T>::pack(x0 - h.x, x1 - h.y);
+}
+// hi + lo of a sum that was split; an infinity of hi is the result (its lo is inf - inf or 0 * inf).
+__device__ __forceinline__ float joined(float hi, float lo) { return isinf(hi) ? hi : hi + lo; }
+
+template <typename T>
+__device__ __forceinline__ float2 load_table2(const Pool& p, const void* t, int64_t off) {
+  if (p.rope_f32) return *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(t) + off);
+  return Cvt<T>::unpack(*reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(t) + off));
+}
+
+template <int D>
+struct Layout {
+  static constexpr int kRowBytes = D * 2, kTileBytes = kUnit * kRowBytes, kStageBytes = 2 * kTileBytes;
+  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kPitch = D + 8;                                 // floats per head in the join buffer
+  static constexpr int kJoinBytes = kWarps * 8 * kPitch * 4;
+  static constexpr int kBytes = kRing + kJoinBytes + kWarps * kStages * 4 + 2 * kWarps * 8 * 4 + 128;
+};
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const __grid_constant__ DecodeParams p) {
+  using L = Layout<D>;
+  constexpr int kStages = L::kStages, RB = L::kRowBytes;
+  constexpr int LPR = D / 8, RPI = 32 / LPR;      // lanes per row, rows per load instruction
+  constexpr int KS = D / 16;                      // k steps of the first product, pairs of n tiles of the second
+  extern __shared__ __align__(128) unsigned char smem[];
+  float* sm_o = reinterpret_cast<float*>(smem + L::kRing);
+  uint32_t* sm_mask = reinterpret_cast<uint32_t*>(smem + L::kRing + L::kJoinBytes);
+  float* sm_m = reinterpret_cast<float*>(sm_mask + kWarps * kStages);
+  float* sm_l = sm_m + kWarps * 8;
+  int64_t* sm_scan = reinterpret_cast<int64_t*>(sm_l + kWarps * 8);   // 8 warp sums, then {b, item of b, at} of the part
+  int* sm_flag = reinterpret_cast<int*>(sm_scan + 12);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int items_per_seq = p.KV * p.tiles;
+  const int64_t slot_mask = (1ll << p.pool.shift) - 1;
+
+  // ---- the line: total length, and where this block's part begins
+  const int per = (p.B + kDecodeThreads - 1) / kDecodeThreads;
+  const int b_lo = min(tid * per, p.B), b_hi = min(b_lo + per, p.B);
+  auto cost_of = [&](int b) {
+    const int n = tokens_of(p, b);
+    if (!p.sink) return (int64_t)items_per_seq * (units_of(n) + kItemCost);
+    int64_t sum = 0;
+    for (int kh = 0; kh < p.KV; ++kh) sum += units_of(span_of(p, n, kh).rows) + kItemCost;
+    return sum * p.tiles;
+  };
+  int64_t mine = 0;
+  for (int b = b_lo; b < b_hi; ++b) mine += cost_of(b);
+  int64_t before = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t other = __shfl_up_sync(0xffffffffu, before, off);
+    if (lane >= off) before += other;
+  }
+  if (lane == 31) sm_scan[warp] = before;
+  before -= mine;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sm_scan[w];
+    total += sm_scan[w];
+  }
+  const int64_t blocks = min(max(total / kMinUnits, (int64_t)1), (int64_t)gridDim.x);
+  const int64_t block = blockIdx.x;
+  const int64_t lo = block * total / blocks, hi = (block + 1) * total / blocks;
+  const bool busy = block < blocks && lo < hi;
+
+  if (busy) {
+    if (before <= lo && lo < before + mine) {     // one thread: the part begins among its sequences
+      int64_t at = before;
+      int b = b_lo;
+      for (int64_t c; lo >= at + (c = cost_of(b)); ++b) at += c;
+      const int n = tokens_of(p, b);
+      int item = 0;
+      for (;; ++item) {
+        const int64_t c = units_of(span_of(p, n, item / p.tiles).rows) + kItemCost;
+        if (lo < at + c) break;
+        at += c;
+      }
+      sm_scan[8] = b;
+      sm_scan[9] = item;
+      sm_scan[10] = at;
     }
     __syncthreads();
-    unpack8<T>(*reinterpret_cast<const uint4*>(q + li * 8), qf);
-    if (p.pool.cos && row >= 0) {       // the query is rotated in fp32 and not rounded
-      float other[8], cf[8], sf[8];
-      const bool upper = li >= LPR / 2;
-      unpack8<T>(*reinterpret_cast<const uint4*>(q + (upper ? li * 8 - D / 2 : li * 8 + D / 2)), other);
-      load_table8<T>(p.pool, p.pool.cos, row + li * 8, cf);
-      load_table8<T>(p.pool, p.pool.sin, row + li * 8, sf);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) qf[j] = fmaf(qf[j], cf[j], (upper ? other[j] : -other[j]) * sf[j]);
-    }
-  } else {
-    unpack8<T>(*reinterpret_cast<const uint4*>(q + li * 8), qf);
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) qf[j] *= p.scale_log2;
+    Cursor cur;
+    cur.b = (int)sm_scan[8];
+    cur.kh = (int)sm_scan[9] / p.tiles;
+    cur.tile = (int)sm_scan[9] % p.tiles;
+    cur.at = sm_scan[10];
+    cur.n = tokens_of(p, cur.b);
+    cur.enter(p, lo, hi);
 
-  int64_t sink = n, rows = n;           // the span: positions [0, sink) and [n - (rows - sink), n)
-  if (p.sink) {
-    sink = min(max(p.sink[kh], (int64_t)0), n);
-    rows = min(n, sink + min(max(p.local[kh], (int64_t)0), n));
-  }
-  const int64_t gap = n - rows;
-  float m = -INFINITY, l = 0.f, acc[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-  for (int64_t r0 = 0; r0 < rows; r0 += GROUPS) {
-    const int64_t r = r0 + g;
-    const int64_t pos = r < sink ? r : r + gap;
-    uint4 ku = make_uint4(0, 0, 0, 0), vu = ku;
-    bool ok = r < rows;
-    if (ok && pos == pos_new) {
-      ok = have_new;
-      ku = *reinterpret_cast<const uint4*>(sm_k + li * 8);
-      vu = *reinterpret_cast<const uint4*>(sm_v + li * 8);
-    } else if (ok) {
-      const int32_t page = page_of(p.pool, table_row, pos);
-      ok = page >= 0;
-      if (ok) {
-        ku = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.pool.k) + page * p.pool.k_page + kh * p.pool.k_head + (pos & slot_mask) * p.pool.k_slot + li * 8);
-        vu = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.pool.v) + page * p.pool.v_page + kh * p.pool.v_head + (pos & slot_mask) * p.pool.v_slot + li * 8);
-      } else if (li == 0) {
-        report(kStatusAttend, b, pos, h);
+    // ---- loads: a cursor of this warp's own
+    Cursor ld = cur;
+    bool ld_more = true;
+    int ld_u = ld.u0 + warp;
+    int32_t ld_page = -1;                          // of row `lane % 16` of the unit that is loaded next
+    int ld_pos = -1;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * kStages * L::kStageBytes;
+    uint32_t* my_mask = sm_mask + warp * kStages;
+
+    auto ld_seek = [&]() {                         // to the next unit of this warp, and look up its rows' pages
+      while (ld_u >= ld.u1) {
+        if (!ld.next(p, lo, hi)) {
+          ld_more = false;
+          return;
+        }
+        ld_u = ld.u0 + warp;
       }
+      const int r = ld_u * kUnit + (lane & 15);
+      ld_pos = -1;
+      ld_page = -1;
+      if (r < ld.span.rows) {
+        ld_pos = r < ld.span.sink ? r : r + (ld.span.n - ld.span.rows);
+        ld_page = p.pool.table[(int64_t)ld.b * p.pool.table_stride + (ld_pos >> p.pool.shift)];
+      }
+    };
+
+    // The new token's row of (b, kh): rotated and rounded, into shared memory (stage address and row, row < 0:
+    // not there) and, `store`, into its page.  Called by a whole warp.  False when it has no place.
+    auto new_row = [&](int b, int kh, int n, uint32_t stage_addr, int row, bool store) {
+      const int64_t pos = n - 1;
+      const int64_t rope = p.pool.cos ? rope_row(p.pool, b, 0, pos) : 0;
+      const int32_t page = page_of(p.pool, p.pool.table + (int64_t)b * p.pool.table_stride, pos);
+      const bool placed = rope >= 0 && page >= 0;
+      if (!placed && lane == 0) report(rope < 0 ? kStatusRope : kStatusAppend, b, pos, kh);
+      if (lane < D / 16) {
+        uint4 x[4];                                // key and value, lower and upper half; zeros without a place
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = make_uint4(0, 0, 0, 0);
+        if (placed) {
+          const T* ks = reinterpret_cast<const T*>(p.k_new) + b * p.k_sb + kh * p.k_sh + lane * 8;
+          const T* vs = reinterpret_cast<const T*>(p.v_new) + b * p.v_sb + kh * p.v_sh + lane * 8;
+          x[0] = *reinterpret_cast<const uint4*>(ks);
+          x[1] = *reinterpret_cast<const uint4*>(ks + D / 2);
+          x[2] = *reinterpret_cast<const uint4*>(vs);
+          x[3] = *reinterpret_cast<const uint4*>(vs + D / 2);
+          if (p.pool.cos) rotate_pair<T, D>(p.pool, rope, lane, x[0], x[1]);
+        }
+        if (placed && store) {
+          const int64_t slot = pos & slot_mask;
+          T* kd = reinterpret_cast<T*>(p.pool.k) + page * p.pool.k_page + kh * p.pool.k_head + slot * p.pool.k_slot + lane * 8;
+          T* vd = reinterpret_cast<T*>(p.pool.v) + page * p.pool.v_page + kh * p.pool.v_head + slot * p.pool.v_slot + lane * 8;
+          *reinterpret_cast<uint4*>(kd) = x[0];
+          *reinterpret_cast<uint4*>(kd + D / 2) = x[1];
+          *reinterpret_cast<uint4*>(vd) = x[2];
+          *reinterpret_cast<uint4*>(vd + D / 2) = x[3];
+        }
+        if (row >= 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int chunk = lane + (i & 1) * (D / 16);
+            const uint32_t a = stage_addr + (i >> 1) * L::kTileBytes + row * RB + ((chunk ^ (row & 7)) << 4);
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x[i].x), "r"(x[i].y), "r"(x[i].z), "r"(x[i].w) : "memory");
+          }
+        }
+      }
+      return placed;
+    };
+
+    auto ld_issue = [&](int stage) {
+      if (ld_more) {
+        const uint32_t dst = ring + stage * L::kStageBytes;
+        bool ok = (uint32_t)ld_page < (uint32_t)p.pool.num_pages && ld_pos >= 0;
+        const bool is_new = p.k_new && ld_pos >= 0 && ld_pos == ld.n - 1 && ld.n == (int64_t)p.lengths[ld.b] + 1;
+        if (ld_pos >= 0 && !ok && !is_new && lane < 16) report(kStatusAttend, ld.b, ld_pos, ld.kh);
+        const bool take = ok && !is_new;
+        const T* kp = reinterpret_cast<const T*>(p.pool.k);
+        const T* vp = reinterpret_cast<const T*>(p.pool.v);
+        if (take) {
+          kp += ld_page * p.pool.k_page + ld.kh * p.pool.k_head + (ld_pos & slot_mask) * p.pool.k_slot;
+          vp += ld_page * p.pool.v_page + ld.kh * p.pool.v_head + (ld_pos & slot_mask) * p.pool.v_slot;
+        }
+        const uint32_t taken = __ballot_sync(0xffffffffu, take) & 0xffffu;
+        const uint32_t fresh = __ballot_sync(0xffffffffu, is_new) & 0xffffu;     // written below, not copied
+#pragma unroll
+        for (int i = 0; i < kUnit / RPI; ++i) {
+          const int row = i * RPI + lane / LPR, chunk = lane % LPR;
+          const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(kp), row));
+          if (!((fresh >> row) & 1)) cp_async16(dst + row * RB + ((chunk ^ (row & 7)) << 4), src + chunk * 8, (taken >> row) & 1);
+        }
+#pragma unroll
+        for (int i = 0; i < kUnit / RPI; ++i) {
+          const int row = i * RPI + lane / LPR, chunk = lane % LPR;
+          const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(vp), row));
+          if (!((fresh >> row) & 1)) cp_async16(dst + L::kTileBytes + row * RB + ((chunk ^ (row & 7)) << 4), src + chunk * 8, (taken >> row) & 1);
+        }
+        uint32_t present = taken;
+        if (fresh && new_row(ld.b, ld.kh, ld.n, dst, __ffs(fresh) - 1, ld.tile == 0)) present |= fresh;
+        if (lane == 0) my_mask[stage] = present;
+        ld_u += kWarps;
+        ld_seek();
+      }
+      cp_async_commit();
+    };
+
+    ld_seek();
+#pragma unroll 1
+    for (int s = 0; s < kStages; ++s) ld_issue(s);
+
+    // ---- items
+    const int g = lane >> 2, t = lane & 3;         // row (query head of a tile) and column pair of a fragment
+    int stage = 0;
+    do {
+      const int heads0 = cur.tile * 8 * MT;        // first query head of the tile within its key head's group
+      const int heads = min(p.G - heads0, 8 * MT);
+      const bool owner = cur.at >= lo;             // the item begins in this part
+      const bool with_new = p.k_new && cur.n > 0 && cur.n == (int64_t)p.lengths[cur.b] + 1;
+      if (owner && warp == 0) {
+        if (with_new && cur.tile == 0 && !(cur.span.rows > cur.span.sink || cur.span.rows == cur.n))
+          new_row(cur.b, cur.kh, cur.n, 0, -1, true);     // stored although the span does not reach it
+        if (lane == 0 && cur.kh == 0 && cur.tile == 0 && p.lengths[cur.b] >= 0 &&
+            (int64_t)p.lengths[cur.b] + (p.k_new ? 1 : 0) > p.capacity)
+          report(kStatusLength, cur.b, (int64_t)p.lengths[cur.b] + (p.k_new ? 1 : 0), 0);
+      }
+      auto store_out = [&](int head, int d, float o) {
+        const int64_t off = (int64_t)cur.b * p.o_sb + (int64_t)(cur.kh * p.G + heads0 + head) * p.o_sh + d;
+        if (p.out_f32) reinterpret_cast<float*>(p.out)[off] = o;
+        else reinterpret_cast<T*>(p.out)[off] = static_cast<T>(o);
+      };
+      if (cur.units == 0) {                        // nothing to attend (only its owner gets here)
+        for (int i = tid; i < heads * D; i += kDecodeThreads) store_out(i / D, i % D, 0.f);
+        continue;
+      }
+      if (cur.u0 >= cur.u1) continue;              // only the item's cost lies in this part
+
+      float m[MT], l[MT], acc[MT][D / 8][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        m[mt] = -INFINITY;
+        l[mt] = 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[mt][j][e] = 0.f;
+      }
+      if (cur.u0 + warp < cur.u1) {
+        // query fragments: rows 0-7 the heads, rows 8-15 what a rotated query has beyond 16 bits
+        uint32_t qa[MT][KS][4];
+        const int64_t rope = with_new && p.pool.cos ? rope_row(p.pool, cur.b, 0, cur.n - 1) : -1;
+        const bool split = rope >= 0;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const int head = mt * 8 + g;
+          const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)cur.b * p.q_sb + (int64_t)(cur.kh * p.G + heads0 + head) * p.q_sh + 2 * t;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            qa[mt][ks][0] = head < heads ? *reinterpret_cast<const uint32_t*>(q + ks * 16) : 0u;
+            qa[mt][ks][2] = head < heads ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8) : 0u;
+            qa[mt][ks][1] = qa[mt][ks][3] = 0u;
+          }
+          if (split) {
+#pragma unroll
+            for (int ks = 0; ks < KS / 2; ++ks)
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                const int d = ks * 16 + e * 4 + 2 * t;
+                const float2 cl = load_table2<T>(p.pool, p.pool.cos, rope + d), ch = load_table2<T>(p.pool, p.pool.cos, rope + d + D / 2);
+                const float2 sl = load_table2<T>(p.pool, p.pool.sin, rope + d), sh = load_table2<T>(p.pool, p.pool.sin, rope + d + D / 2);
+                const float2 a = Cvt<T>::unpack(qa[mt][ks][e]), b = Cvt<T>::unpack(qa[mt][ks + KS / 2][e]);
+                split2<T>(fmaf(a.x, cl.x, -b.x * sl.x), fmaf(a.y, cl.y, -b.y * sl.y), qa[mt][ks][e], qa[mt][ks][e + 1]);
+                split2<T>(fmaf(b.x, ch.x, a.x * sh.x), fmaf(b.y, ch.y, a.y * sh.y), qa[mt][ks + KS / 2][e], qa[mt][ks + KS / 2][e + 1]);
+              }
+          }
+        }
+        const int mi = lane >> 3, r8 = lane & 7;
+#pragma unroll 1
+        for (int u = cur.u0 + warp; u < cur.u1; u += kWarps) {
+          cp_async_wait<kStages - 1>();
+          __syncwarp();
+          const uint32_t ka = ring + stage * L::kStageBytes, va = ka + L::kTileBytes;
+          const uint32_t present = my_mask[stage] >> (2 * t);
+          float sc[MT][2][4];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[mt][0][e] = sc[mt][1][e] = 0.f;
+          {
+            const uint32_t base = ka + ((mi >> 1) * 8 + r8) * RB;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+              uint32_t kb[4];
+              ldmatrix4(kb, base + (((2 * ks + (mi & 1)) ^ r8) << 4));
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                mma16816<T>(sc[mt][0], qa[mt][ks], kb[0], kb[1]);
+                mma16816<T>(sc[mt][1], qa[mt][ks], kb[2], kb[3]);
+              }
+            }
+          }
+          uint32_t pa[MT][4];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            float s[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float hi_part = sc[mt][e >> 1][e & 1], lo_part = sc[mt][e >> 1][(e & 1) + 2];
+              const float v = (split ? joined(hi_part, lo_part) : hi_part) * p.scale_log2;
+              s[e] = (present >> ((e >> 1) * 8 + (e & 1))) & 1 ? v : -INFINITY;
+            }
+            float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float m_new = fmaxf(m[mt], top), base = m_new == -INFINITY ? 0.f : m_new;
+            const float corr = exp2f(m[mt] - base);
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = exp2f(s[e] - base);
+            l[mt] = l[mt] * corr + ((w[0] + w[1]) + (w[2] + w[3]));
+            split2<T>(w[0], w[1], pa[mt][0], pa[mt][1]);
+            split2<T>(w[2], w[3], pa[mt][2], pa[mt][3]);
+            if (__any_sync(0xffffffffu, m_new != m[mt])) {
+#pragma unroll
+              for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[mt][j][e] *= corr;
+            }
+            m[mt] = m_new;
+          }
+          {
+            const uint32_t base = va + ((mi & 1) * 8 + r8) * RB;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+              uint32_t vb[4];
+              ldmatrix4_trans(vb, base + (((2 * j + (mi >> 1)) ^ r8) << 4));
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                mma16816<T>(acc[mt][2 * j], pa[mt], vb[0], vb[1]);
+                mma16816<T>(acc[mt][2 * j + 1], pa[mt], vb[2], vb[3]);
+              }
+            }
+          }
+          __syncwarp();
+          ld_issue(stage);
+          stage = stage + 1 == kStages ? 0 : stage + 1;
+        }
+      }
+
+      // ---- the warps' results joined
+      const bool whole = cur.u0 == 0 && cur.u1 == cur.units;
+      const int nw = min(kWarps, cur.u1 - cur.u0);
+      float* rec = p.records + (2 * block + (owner ? 1 : 0)) * kRecFloats;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const int here = min(heads - mt * 8, 8);
+        if (MT > 1 && here <= 0) break;
+        if (warp < nw) {
+          float sum = l[mt];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          if (t == 0) {
+            sm_m[warp * 8 + g] = m[mt];
+            sm_l[warp * 8 + g] = sum;
+          }
+          if (g < here) {
+            float* o = sm_o + (warp * 8 + g) * L::kPitch + 2 * t;
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j)
+              *reinterpret_cast<float2*>(o + j * 8) = make_float2(joined(acc[mt][j][0], acc[mt][j][2]), joined(acc[mt][j][1], acc[mt][j][3]));
+          }
+        }
+        __syncthreads();
+        for (int i = tid; i < here * D; i += kDecodeThreads) {
+          const int head = i / D, d = i % D;
+          float M = -INFINITY, Ls = 0.f, O = 0.f;
+          for (int w = 0; w < nw; ++w) M = fmaxf(M, sm_m[w * 8 + head]);
+          const float base = M == -INFINITY ? 0.f : M;
+          for (int w = 0; w < nw; ++w) {
+            const float f = exp2f(sm_m[w * 8 + head] - base);
+            Ls += f * sm_l[w * 8 + head];
+            O += f * sm_o[(w * 8 + head) * L::kPitch + d];
+          }
+          if (whole) {
+            store_out(mt * 8 + head, d, Ls == 0.f ? 0.f : O / Ls);
+          } else {
+            rec[(mt * 8 + head) * D + d] = O;
+            if (d == 0) *reinterpret_cast<float2*>(rec + kRecHeads * 128 + (mt * 8 + head) * 2) = make_float2(M, Ls);
+          }
+        }
+        __syncthreads();
+      }
+      if (whole) continue;
+
+      // ---- the blocks' results joined: kJoin neighbours by the last of them, then their results by the last of those
+      auto block_of = [&](int64_t x) { return ((x + 1) * blocks - 1) / total; };
+      const int64_t c0 = block_of(cur.at);
+      const int parts = (int)(block_of(cur.at + cur.units - 1) - c0) + 1;
+      const int group = (int)(block - c0) / kJoin, groups = (parts + kJoin - 1) / kJoin;
+      auto record_of = [&](int i) { return p.records + (i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * kRecFloats; };
+      bool final = false;
+      for (int level = 0; level < 2; ++level) {
+        const int first = level == 0 ? group * kJoin : 0, step = level == 0 ? 1 : kJoin;
+        const int count = level == 0 ? min(parts - first, kJoin) : groups;
+        int* counter = p.counters + (level == 0 ? 3 * (c0 + first) + (group == 0 ? 0 : 1) : 3 * c0 + 2);
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+          *sm_flag = atomicAdd(counter, 1) == count - 1;
+          if (*sm_flag) *counter = 0;
+        }
+        __syncthreads();
+        if (!*sm_flag) break;
+        __threadfence();
+        final = level == 1 || groups == 1;
+        float* wm = sm_o;                          // (record, head): maximum, then weight; and sum
+        float* wl = sm_o + kJoin * kRecHeads;
+        {
+          const int i = tid / kRecHeads, head = tid % kRecHeads;
+          if (i < count && head < heads) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(record_of(first + i * step) + kRecHeads * 128 + head * 2));
+            wm[tid] = ml.x;
+            wl[tid] = ml.y;
+          }
+        }
+        __syncthreads();
+        float* to = record_of(first);
+        for (int i4 = tid; i4 < heads * D / 4; i4 += kDecodeThreads) {
+          const int head = i4 * 4 / D, d = i4 * 4 % D;
+          float4 x[kJoin];
+#pragma unroll
+          for (int i = 0; i < kJoin; ++i)
+            if (i < count) x[i] = __ldcg(reinterpret_cast<const float4*>(record_of(first + i * step) + i4 * 4));
+          float M = -INFINITY, Ls = 0.f;
+          for (int i = 0; i < count; ++i) M = fmaxf(M, wm[i * kRecHeads + head]);
+          const float base = M == -INFINITY ? 0.f : M;
+          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i < kJoin; ++i)
+            if (i < count) {
+              const float f = exp2f(wm[i * kRecHeads + head] - base);
+              Ls += f * wl[i * kRecHeads + head];
+              O.x += f * x[i].x; O.y += f * x[i].y; O.z += f * x[i].z; O.w += f * x[i].w;
+            }
+          if (final) {
+            const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
+            store_out(head, d, Ls == 0.f ? 0.f : O.x * inv);
+            store_out(head, d + 1, Ls == 0.f ? 0.f : O.y * inv);
+            store_out(head, d + 2, Ls == 0.f ? 0.f : O.z * inv);
+            store_out(head, d + 3, Ls == 0.f ? 0.f : O.w * inv);
+          } else {
+            // (each element of the group's first record is read by the thread that writes it)
+            *reinterpret_cast<float4*>(to + i4 * 4) = O;
+            if (d == 0) *reinterpret_cast<float2*>(to + kRecHeads * 128 + head * 2) = make_float2(M, Ls);
+          }
+        }
+        if (final) break;
+      }
+      __syncthreads();                             // sm_o is free again
+    } while (cur.next(p, lo, hi));
+    cp_async_wait<0>();
+  }
+
+  if (p.advance) {                                 // the last block to get here: every block has read the lengths
+    __syncthreads();
+    if (tid == 0) {
+      int* done = p.counters + 3 * kMaxBlocks;
+      *sm_flag = atomicAdd(done, 1) == (int)gridDim.x - 1;
+      if (*sm_flag) *done = 0;
     }
-    float kf[8], vf[8], s = 0.f;
-    unpack8<T>(ku, kf);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s = fmaf(qf[j], kf[j], s);
-#pragma unroll
-    for (int off = LPR / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    if (ok) {
-      unpack8<T>(vu, vf);
-      const float m_new = fmaxf(m, s), base = m_new == -INFINITY ? 0.f : m_new;
-      const float corr = exp2f(m - base), pr = exp2f(s - base);
-      l = l * corr + pr;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = fmaf(pr, vf[j], acc[j] * corr);
-      m = m_new;
-    }
+    __syncthreads();
+    if (*sm_flag)
+      for (int b = tid; b < p.B; b += kDecodeThreads) {
+        const int len = p.lengths[b];
+        if (len >= 0 && len < 2147483647) p.lengths[b] = len + 1;
+      }
   }
-  if (li == 0) {
-    sm_m[g] = m;
-    sm_l[g] = l;
+}
+
+constexpr int kMaxDevices = 64;
+// SMs of the current device (kept per device ordinal); 148 where no device can be asked.
+int sm_count() {
+  static int cached[kMaxDevices];                  // benign race: every writer stores the same value
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices ||
+      (cached[dev] == 0 && cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)) {
+    (void)cudaGetLastError();
+    return 148;
   }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) sm_acc[g][li * 8 + j] = acc[j];
-  __syncthreads();
-  if (tid >= D) return;
-  float M = -INFINITY, L = 0.f, O = 0.f;
-  for (int i = 0; i < GROUPS; ++i) M = fmaxf(M, sm_m[i]);
-  if (M == -INFINITY) M = 0.f;
-  for (int i = 0; i < GROUPS; ++i) {
-    const float w = exp2f(sm_m[i] - M);
-    L += sm_l[i] * w;
-    O += sm_acc[i][tid] * w;
+  if (cached[dev] == 0) cached[dev] = sms < kMaxBlocks ? sms : kMaxBlocks;
+  return cached[dev];
+}
+
+template <typename T, int D, int MT>
+int launch_decode(const DecodeParams& p, int grid, cudaStream_t stream) {
+  static bool ready[kMaxDevices];
+  int dev = 0;
+  MOA_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= kMaxDevices || !ready[dev]) {
+    MOA_CUDA_CHECK(cudaFuncSetAttribute(paged_decode_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kBytes));
+    if (dev >= 0 && dev < kMaxDevices) ready[dev] = true;
   }
-  const float o = L == 0.f ? 0.f : O / L;
-  const int64_t off = b * p.o_sb + h * p.o_sh + tid;
-  if (p.out_f32) reinterpret_cast<float*>(p.out)[off] = o;
-  else reinterpret_cast<T*>(p.out)[off] = static_cast<T>(o);
+  paged_decode_kernel<T, D, MT><<<grid, kDecodeThreads, Layout<D>::kBytes, stream>>>(p);
+  MOA_CUDA_CHECK(cudaGetLastError());
+  return MOA_OK;
+}
+template <typename T>
+int launch_decode(const DecodeParams& p, int D, int grid, cudaStream_t stream) {
+  if (D == 128) return p.G > 8 ? launch_decode<T, 128, 2>(p, grid, stream) : launch_decode<T, 128, 1>(p, grid, stream);
+  return p.G > 8 ? launch_decode<T, 64, 2>(p, grid, stream) : launch_decode<T, 64, 1>(p, grid, stream);
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -410,7 +913,10 @@ int moa_paged_append(const moa_paged_append_args* args, moa_stream_t stream) {
   return MOA_OK;
 }
 
-int64_t moa_paged_decode_workspace_bytes(void) { return MOA_PAGED_COUNTER_BYTES; }
+int64_t moa_paged_decode_workspace_bytes(void) {
+  static_assert((3 * moa::kMaxBlocks + 1) * 4 <= MOA_PAGED_COUNTER_BYTES, "counters");
+  return MOA_PAGED_COUNTER_BYTES + (int64_t)moa::sm_count() * 2 * moa::kRecFloats * 4;
+}
 
 int moa_paged_decode(const moa_paged_decode_args* args, moa_stream_t stream) {
   using namespace moa;
@@ -436,24 +942,19 @@ int moa_paged_decode(const moa_paged_decode_args* args, moa_stream_t stream) {
   p.sink = a.sink_size; p.local = a.local_size;
   p.q_sb = a.q_sb; p.q_sh = a.q_sh; p.k_sb = a.k_sb; p.k_sh = a.k_sh; p.v_sb = a.v_sb; p.v_sh = a.v_sh;
   p.o_sb = a.o_sb; p.o_sh = a.o_sh;
-  p.B = (int)a.B; p.H = (int)a.H; p.KV = (int)a.KV;
+  p.B = (int)a.B; p.H = (int)a.H; p.KV = (int)a.KV; p.G = p.H / p.KV;
+  p.tiles = (p.G + (p.G > 8 ? 15 : 7)) / (p.G > 8 ? 16 : 8);
+  p.capacity = (int)std::min(a.max_pages * a.page_size, (int64_t)2147483647 - 64);
   p.scale_log2 = (float)(a.sm_scale * 1.4426950408889634);
-  p.out_f32 = a.out_f32 != 0;
-  dim3 grid((unsigned)a.H, (unsigned)a.B);
+  p.out_f32 = a.out_f32 != 0; p.advance = a.advance != 0;
+  p.counters = reinterpret_cast<int*>(a.workspace);
+  p.records = reinterpret_cast<float*>(reinterpret_cast<char*>(a.workspace) + MOA_PAGED_COUNTER_BYTES);
+  // one block per SM, or as many as the longest sequences that the table allows could employ
+  const int64_t most = a.B * a.KV * p.tiles * (std::min(ceil_div64(p.capacity, kUnit), (int64_t)4096) + kItemCost);
+  const int grid = (int)std::max((int64_t)1, std::min((int64_t)sm_count(), most / kMinUnits));
   cudaStream_t st = (cudaStream_t)stream;
-  if (a.dtype == MOA_F16) {
-    if (a.D == 128) paged_decode_kernel<__half, 128><<<grid, 128, 0, st>>>(p);
-    else paged_decode_kernel<__half, 64><<<grid, 128, 0, st>>>(p);
-  } else {
-    if (a.D == 128) paged_decode_kernel<__nv_bfloat16, 128><<<grid, 128, 0, st>>>(p);
-    else paged_decode_kernel<__nv_bfloat16, 64><<<grid, 128, 0, st>>>(p);
-  }
-  MOA_CUDA_CHECK(cudaGetLastError());
-  if (a.advance) {
-    paged_advance_kernel<<<(unsigned)ceil_div64(a.B, 256), 256, 0, st>>>(a.lengths, nullptr, 1, (int)a.B);
-    MOA_CUDA_CHECK(cudaGetLastError());
-  }
-  return MOA_OK;
+  return a.dtype == MOA_F16 ? launch_decode<__half>(p, (int)a.D, grid, st)
+                            : launch_decode<__nv_bfloat16>(p, (int)a.D, grid, st);
 }
 
 int moa_paged_status(int32_t status[4]) {

@@ -27,59 +27,73 @@ _workspaces: Dict = {}
 _touched = set()      # devices that a paged call has run on
 
 
-def _workspace(device, stream: int) -> Tensor:
+def _workspace(index: int, stream: int) -> Tensor:
     """Scratch of ``paged_decode``: kept per device and stream; a call that is being captured gets one of its own,
     from the graph's memory, so that two graphs never share one."""
     if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(lib.moa_paged_decode_workspace_bytes(), dtype=torch.uint8, device=device)
+        ws = torch.empty(lib.moa_paged_decode_workspace_bytes(), dtype=torch.uint8, device=index)
         ws[:_COUNTER_BYTES].zero_()
         return ws
-    key = (device.index, stream)
-    ws = _workspaces.get(key)
+    ws = _workspaces.get((index, stream))
     if ws is None:
-        ws = _workspaces[key] = torch.zeros(lib.moa_paged_decode_workspace_bytes(), dtype=torch.uint8, device=device)
+        ws = _workspaces[index, stream] = torch.zeros(lib.moa_paged_decode_workspace_bytes(), dtype=torch.uint8,
+                                                      device=index)
     return ws
 
 
+# The checks below run on every call, and at decode sizes the host's share of a call is larger than the
+# kernel's: they ask a tensor for each property once (get_device() instead of device, all strides at once).
+
 def _pool_arguments(key_pages: Tensor, value_pages: Tensor, page_table: Tensor, lengths: Tensor, B: int, KV: int,
-                    D: int, dtype, device):
+                    D: int, dtype, device: int):
     assert dtype in _DTYPES, f"the paged cache supports float16 and bfloat16 only, got {dtype}"
-    assert key_pages.dim() == 4 and key_pages.shape == value_pages.shape, "pages must be (num_pages, KV, page_size, D)"
-    num_pages, kv, page_size, d = key_pages.shape
-    assert kv == KV and d == D, "pages must be (num_pages, KV, page_size, D)"
-    assert key_pages.dtype == dtype and value_pages.dtype == dtype, "pages and tokens must have the same dtype"
+    shape = key_pages.shape
+    assert len(shape) == 4 and value_pages.shape == shape and shape[1] == KV and shape[3] == D, \
+        "pages must be (num_pages, KV, page_size, D)"
+    assert key_pages.dtype is dtype and value_pages.dtype is dtype, "pages and tokens must have the same dtype"
     ks, vs = key_pages.stride(), value_pages.stride()
     assert ks[3] == 1 and vs[3] == 1, "rows of the pages must be contiguous"
-    assert page_table.dim() == 2 and page_table.shape[0] == B and page_table.dtype == torch.int32, \
-        "page_table must be int32 (B, max_pages)"
-    assert page_table.stride(1) == 1 or page_table.shape[1] == 1, "rows of page_table must be contiguous"
-    assert lengths.shape == (B,) and lengths.dtype == torch.int32 and lengths.is_contiguous(), \
-        "lengths must be contiguous int32 (B,)"
-    assert key_pages.device == device and value_pages.device == device and page_table.device == device and \
-        lengths.device == device, "all tensors must be on the same device"
-    return (ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], page_table.stride(0), page_table.shape[1], num_pages, page_size)
+    ts, width = page_table.stride(), page_table.shape
+    assert len(width) == 2 and width[0] == B and page_table.dtype is torch.int32, "page_table must be int32 (B, max_pages)"
+    assert ts[1] == 1 or width[1] == 1, "rows of page_table must be contiguous"
+    _check_row_of_ints(lengths, B, device, torch.int32, "lengths must be contiguous int32 (B,)")
+    assert key_pages.get_device() == device and value_pages.get_device() == device and \
+        page_table.get_device() == device, "all tensors must be on the same device"
+    return (ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], ts[0], width[1], shape[0], shape[2])
 
 
-def _rope_arguments(rope: Tuple[Tensor, Tensor], B: int, N: int, D: int, dtype, device):
+def _check_row_of_ints(t: Tensor, n: int, device: int, dtype, what: str) -> None:
+    assert t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous(), what
+    assert t.get_device() == device, "all tensors must be on the same device"
+
+
+def _rope_arguments(rope: Tuple[Tensor, Tensor], B: int, N: int, D: int, dtype, device: int):
     cos, sin = rope
-    assert cos.shape == sin.shape and cos.stride() == sin.stride() and cos.stride(-1) == 1 and cos.shape[-1] == D, \
+    shape, stride = cos.shape, cos.stride()
+    assert sin.shape == shape and sin.stride() == stride and stride[-1] == 1 and shape[-1] == D, \
         "rope tables must be two tensors of one shape and layout with rows of D"
-    assert cos.dtype == sin.dtype and (cos.dtype == dtype or cos.dtype == torch.float32), \
+    kind = cos.dtype
+    assert sin.dtype is kind and (kind is dtype or kind is torch.float32), \
         "rope tables must have the tensors' dtype or be float32"
-    assert cos.device == device and sin.device == device, "all tensors must be on the same device"
-    if cos.dim() == 2:
-        assert cos.shape[0] > 0, "a rope table by position needs rows"
-        where = (0, cos.stride(0), cos.shape[0])
-    else:
-        assert cos.dim() == 3 and cos.shape[0] in (1, B) and cos.shape[1] == N, \
-            "rope tables must be (positions, D), (B, N, D) or (1, N, D)"
-        where = (0 if cos.shape[0] == 1 else cos.stride(0), cos.stride(1), 0)
-    return (cos.data_ptr(), sin.data_ptr(), *where, int(cos.dtype == torch.float32))
+    assert cos.get_device() == device and sin.get_device() == device, "all tensors must be on the same device"
+    if len(shape) == 2:
+        assert shape[0] > 0, "a rope table by position needs rows"
+        return (cos.data_ptr(), sin.data_ptr(), 0, stride[0], shape[0], kind is torch.float32)
+    assert len(shape) == 3 and (shape[0] == 1 or shape[0] == B) and shape[1] == N, \
+        "rope tables must be (positions, D), (B, N, D) or (1, N, D)"
+    return (cos.data_ptr(), sin.data_ptr(), 0 if shape[0] == 1 else stride[0], stride[1], 0, kind is torch.float32)
 
 
-def _rows(t: Tensor) -> Tensor:
-    """``t``, or a copy of it in rows that the kernels can read."""
-    return t if _lib.rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
+def _rows(t: Tensor):
+    """``t`` (.., .., N, D), or a copy of it whose rows the kernels can read, with its address and first three strides
+    (that of a dimension of one is of no interest)."""
+    a, b, n, d = t.stride()
+    if t.shape[2] == 1:
+        n = 0
+    if d != 1 or (a | b | n) & 7 or t.data_ptr() & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        a, b, n, d = t.stride()
+    return t, t.data_ptr(), (a, b, n)
 
 
 def _inference_only(*tensors) -> None:
@@ -87,9 +101,24 @@ def _inference_only(*tensors) -> None:
         raise NotImplementedError("the paged cache has no gradient (inference only): call it under torch.no_grad()")
 
 
-def _on(device):
-    """The device guard of a launch; nothing to do when it is the current device already."""
-    return _lib.NO_RANGE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _cuda_only(device: int) -> None:
+    if device < 0:
+        raise RuntimeError("moa_b200 runs on CUDA tensors only (there is no CPU path)")
+
+
+def _launch(name: str, entry, arguments, device: int) -> None:
+    """``entry(arguments(stream), stream)`` on the device's current stream, with the device current; ``arguments``
+    packs the struct once the stream is known (the scratch belongs to it)."""
+    if _lib.NVTX or torch.cuda.current_device() != device:
+        with torch.cuda.device(device), _lib.nvtx_range("moa_b200." + name):
+            stream = torch.cuda.current_stream(device).cuda_stream
+            status = entry(arguments(stream), stream)
+    else:
+        stream = torch.cuda.current_stream(device).cuda_stream
+        status = entry(arguments(stream), stream)
+    if status:
+        _lib.check("moa_" + name, status)
+    _touched.add(device)
 
 
 def paged_append(key: Tensor, value: Tensor, key_pages: Tensor, value_pages: Tensor, page_table: Tensor,
@@ -115,43 +144,38 @@ def paged_append(key: Tensor, value: Tensor, key_pages: Tensor, value_pages: Ten
 
     A token whose page (or row of a table by position) does not exist is not stored, and
     ``check_device_status()`` raises for it.  Two tokens of one call must not have the same place."""
-    assert key.dim() == 4 and key.shape == value.shape, "key and value must be (B, KV, N, D)"
-    B, KV, N, D = key.shape
-    dtype, device = key.dtype, key.device
+    shape = key.shape
+    assert len(shape) == 4 and value.shape == shape, "key and value must be (B, KV, N, D)"
+    B, KV, N, D = shape
+    dtype, device = key.dtype, key.get_device()
     pool = _pool_arguments(key_pages, value_pages, page_table, lengths, B, KV, D, dtype, device)
-    assert value.dtype == dtype and value.device == device
-    key, value = _rows(key), _rows(value)
-    H, q_ptr, q_strides = KV, 0, (0, 0, 0)
+    assert value.dtype is dtype and value.get_device() == device, "key and value must be alike"
+    H = KV
     if query is not None:
         assert rope is not None, "a query is given to be rotated: rope is needed"
-        assert query.dim() == 4 and query.shape[0] == B and query.shape[2:] == (N, D), "query must be (B, H, N, D)"
-        assert query.dtype == dtype and query.device == device
-        query = _rows(query)
-        H, q_ptr, q_strides = query.shape[1], query.data_ptr(), query.stride()[:3]
+        shape = query.shape
+        assert len(shape) == 4 and shape[0] == B and shape[2] == N and shape[3] == D, "query must be (B, H, N, D)"
+        assert query.dtype is dtype and query.get_device() == device, "query and key must be alike"
+        H = shape[1]
     if counts is not None:
-        assert counts.shape == (B,) and counts.dtype == torch.int32 and counts.is_contiguous(), \
-            "counts must be contiguous int32 (B,)"
-        assert counts.device == device, "all tensors must be on the same device"
+        _check_row_of_ints(counts, B, device, torch.int32, "counts must be contiguous int32 (B,)")
     r = _NO_ROPE if rope is None else _rope_arguments(rope, B, N, D, dtype, device)
     _inference_only(key, value, query)
-    if device.type != "cuda":
-        raise RuntimeError("moa_b200 runs on CUDA tensors only (there is no CPU path)")
-    result = None
+    _cuda_only(device)
+    result, q_ptr, q_strides, out_ptrs = None, 0, (0, 0, 0), (0, 0)
     if query is not None:
-        result = (torch.empty(B, H, N, D, dtype=dtype, device=device),
-                  torch.empty(B, KV, N, D, dtype=dtype, device=device))
+        result = (torch.empty((B, H, N, D), dtype=dtype, device=query.device),
+                  torch.empty((B, KV, N, D), dtype=dtype, device=query.device))
+        query, q_ptr, q_strides = _rows(query)
+        out_ptrs = result[0].data_ptr(), result[1].data_ptr()
     if B == 0 or N == 0 or KV == 0:
         return result
-    args = _APPEND.pack(
-        key.data_ptr(), value.data_ptr(), q_ptr, key_pages.data_ptr(), value_pages.data_ptr(), page_table.data_ptr(),
-        lengths.data_ptr(), _lib.ptr(counts), r[0], r[1], 0 if result is None else result[0].data_ptr(),
-        0 if result is None else result[1].data_ptr(),
-        *key.stride()[:3], *value.stride()[:3], *q_strides, *pool, *r[2:], B, H, KV, N, D, _DTYPES[dtype], advance)
-    _touched.add(device.index)
-    with _on(device), _lib.nvtx_range("moa_b200.paged_append"):
-        status = lib.moa_paged_append(args, _lib.current_stream(device))
-    if status:
-        _lib.check("moa_paged_append", status)
+    key, k_ptr, k_strides = _rows(key)
+    value, v_ptr, v_strides = _rows(value)
+    _launch("paged_append", lib.moa_paged_append, lambda stream: _APPEND.pack(
+        k_ptr, v_ptr, q_ptr, key_pages.data_ptr(), value_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
+        0 if counts is None else counts.data_ptr(), r[0], r[1], *out_ptrs, *k_strides, *v_strides, *q_strides, *pool,
+        *r[2:], B, H, KV, N, D, _DTYPES[dtype], advance), device)
     return result
 
 
@@ -177,55 +201,58 @@ def paged_decode(query: Tensor, key_pages: Tensor, value_pages: Tensor, page_tab
     of every sequence; ``lengths[b] < 0`` marks a row without a sequence: nothing is stored and its output is zero.
 
     Tokens whose page does not exist are left out, and ``check_device_status()`` raises for them."""
-    assert query.dim() == 4 and query.shape[2] == 1, "query must be (B, H, 1, D)"
-    B, H, _, D = query.shape
-    dtype, device = query.dtype, query.device
+    shape = query.shape
+    assert len(shape) == 4 and shape[2] == 1, "query must be (B, H, 1, D)"
+    B, H, _, D = shape
+    dtype, device = query.dtype, query.get_device()
     KV = key_pages.shape[1]
     pool = _pool_arguments(key_pages, value_pages, page_table, lengths, B, KV, D, dtype, device)
     assert KV > 0 and H % KV == 0, "the query heads must be a multiple of the pool's key/value heads"
-    q = _rows(query.select(2, 0))
     k_ptr = v_ptr = 0
-    k_strides = v_strides = (0, 0)
-    assert (key is None) == (value is None), "key and value go together"
-    assert rope is None or key is not None, "rope is for the step with a new token"
-    assert not advance or key is not None, "advance is for the step with a new token"
+    k_strides = v_strides = (0, 0, 0)
+    r = _NO_ROPE
     if key is not None:
+        assert value is not None, "key and value go together"
         assert key.shape == (B, KV, 1, D) and value.shape == (B, KV, 1, D), "key and value must be (B, KV, 1, D)"
-        assert key.dtype == dtype and value.dtype == dtype and key.device == device and value.device == device
-        k, v = _rows(key.select(2, 0)), _rows(value.select(2, 0))
-        k_ptr, v_ptr, k_strides, v_strides = k.data_ptr(), v.data_ptr(), k.stride()[:2], v.stride()[:2]
-    r = _NO_ROPE if rope is None else _rope_arguments(rope, B, 1, D, dtype, device)
+        assert key.dtype is dtype and value.dtype is dtype and key.get_device() == device and \
+            value.get_device() == device, "query, key and value must be alike"
+        if rope is not None:
+            r = _rope_arguments(rope, B, 1, D, dtype, device)
+        key, k_ptr, k_strides = _rows(key)
+        value, v_ptr, v_strides = _rows(value)
+    else:
+        assert value is None, "key and value go together"
+        assert rope is None, "rope is for the step with a new token"
+        assert not advance, "advance is for the step with a new token"
     assert (sink_size is None) == (local_size is None), "sink_size and local_size go together"
+    sink_ptr = local_ptr = 0
     if sink_size is not None:
         for t in (sink_size, local_size):
-            assert t.shape == (KV,) and t.dtype == torch.int64 and t.is_contiguous(), \
-                "sink_size and local_size must be contiguous int64 (KV,)"
-            assert t.device == device, "all tensors must be on the same device"
+            _check_row_of_ints(t, KV, device, torch.int64, "sink_size and local_size must be contiguous int64 (KV,)")
+        sink_ptr, local_ptr = sink_size.data_ptr(), local_size.data_ptr()
     _inference_only(query, key, value)
-    if device.type != "cuda":
-        raise RuntimeError("moa_b200 runs on CUDA tensors only (there is no CPU path)")
+    _cuda_only(device)
     if out is None:
-        assert out_dtype is None or out_dtype == dtype or out_dtype == torch.float32
-        out = torch.empty(B, 1, H, D, dtype=out_dtype or dtype, device=device)
+        assert out_dtype is None or out_dtype is dtype or out_dtype is torch.float32
+        out = torch.empty((B, 1, H, D), dtype=out_dtype or dtype, device=query.device)
     else:
-        assert out.shape == (B, 1, H, D) and out.stride(3) == 1 and out.device == device
-        assert out.dtype == dtype or out.dtype == torch.float32, "out must have the query's dtype or be float32"
-        assert out_dtype is None or out_dtype == out.dtype
+        assert out.shape == (B, 1, H, D) and out.stride(3) == 1 and out.get_device() == device, "out must be (B, 1, H, D)"
+        assert out.dtype is dtype or out.dtype is torch.float32, "out must have the query's dtype or be float32"
+        assert out_dtype is None or out_dtype is out.dtype
     if B == 0 or H == 0:
         return out
+    query, q_ptr, q_strides = _rows(query)
     o_strides = out.stride()
-    _touched.add(device.index)
-    with _on(device), _lib.nvtx_range("moa_b200.paged_decode"):
-        stream = _lib.current_stream(device)
+
+    def arguments(stream):
         ws = _workspace(device, stream)
-        args = _DECODE.pack(
-            q.data_ptr(), k_ptr, v_ptr, key_pages.data_ptr(), value_pages.data_ptr(), out.data_ptr(),
-            page_table.data_ptr(), lengths.data_ptr(), _lib.ptr(sink_size), _lib.ptr(local_size), r[0], r[1],
-            ws.data_ptr(), *q.stride()[:2], *k_strides, *v_strides, o_strides[0], o_strides[2], *pool, *r[2:],
-            B, H, KV, D, _DTYPES[dtype], out.dtype == torch.float32, advance, ws.numel(), sm_scale)
-        status = lib.moa_paged_decode(args, stream)
-    if status:
-        _lib.check("moa_paged_decode", status)
+        return _DECODE.pack(
+            q_ptr, k_ptr, v_ptr, key_pages.data_ptr(), value_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(),
+            lengths.data_ptr(), sink_ptr, local_ptr, r[0], r[1], ws.data_ptr(), q_strides[0], q_strides[1],
+            k_strides[0], k_strides[1], v_strides[0], v_strides[1], o_strides[0], o_strides[2], *pool, *r[2:],
+            B, H, KV, D, _DTYPES[dtype], out.dtype is torch.float32, advance, ws.numel(), sm_scale)
+
+    _launch("paged_decode", lib.moa_paged_decode, arguments, device)
     return out
 
 
