@@ -276,7 +276,7 @@ int moa_rope_qk(void* q, void* k, int64_t sb, int64_t sh, int64_t sn, const void
  *
  * moa_paged_decode: attention of one query token per sequence over its pages.
  *   q (B, H, D) through (q_sb, q_sh), H a multiple of KV, query head h reads key head h / (H / KV);
- *   out[b*o_sb + h*o_sh + d], the dtype of q or float32 (out_f32).
+ *   out[b*o_sb + h*o_sh + d], the dtype of q or float32 (out_f32), rows aligned like those of q.
  *   sink_size, local_size (KV) int64, both or none: key head g of a sequence of n tokens attends positions
  *   < sink_size[g] and >= n - local_size[g]; none: all n.  A head that attends nothing gets zeros.
  *   k_new, v_new NULL: n = lengths[b].  Given, (B, KV, D) through their strides: the new token is stored at

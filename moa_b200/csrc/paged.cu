@@ -201,7 +201,7 @@ __global__ void paged_advance_kernel(int32_t* lengths, const int32_t* counts, in
 // and so is the rotated query of the fused step.  Rows 8-15 would idle otherwise (G is small), so the result has
 // fp32 weights at no cost.  MT = 2 serves 9..16 heads with one pass over the keys.
 constexpr int kWarps = 8, kDecodeThreads = kWarps * 32;
-constexpr int kUnit = 16;                   // rows of a unit (k of the second product)
+constexpr int kUnit = 16;                   // positions of a unit (k of the second product)
 constexpr int kItemCost = 2;                // an item's epilogue, in units
 constexpr int kMinUnits = 8;                // least share of a block: fewer blocks work when there is less
 constexpr int kJoin = 16;                   // partial results joined at once
@@ -224,9 +224,18 @@ struct DecodeParams {
   float* records;                           // 2 per block
 };
 
-// The rows of one (sequence, key head): positions [0, sink) and [n - (rows - sink), n).
+// The units of one (sequence, key head): 16 positions each, aligned, so that with pages of 16 and more a unit
+// lies in one page.  Units 0 .. head-1 hold the first `sink` positions, the others begin at unit `tail` and hold the
+// positions from `from` on; positions < n outside both are masked.
 struct Span {
-  int n, sink, rows;
+  int n, sink, from, head, tail, units;
+  __device__ __forceinline__ int unit(int u) const { return u < head ? u : u - head + tail; }
+  // Which of the 16 positions of aligned unit `x` are attended.
+  __device__ __forceinline__ uint32_t mask(int x) const {
+    const int p0 = x * 16;
+    return below(n - p0) & (below(sink - p0) | ~below(from - p0));
+  }
+  static __device__ __forceinline__ uint32_t below(int m) { return m >= 16 ? 0xffffu : m <= 0 ? 0u : (1u << m) - 1u; }
 };
 
 __device__ __forceinline__ int tokens_of(const DecodeParams& p, int b) {
@@ -240,14 +249,17 @@ __device__ __forceinline__ Span span_of(const DecodeParams& p, int n, int kh) {
   Span s;
   s.n = n;
   s.sink = n;
-  s.rows = n;
+  s.from = n;
   if (p.sink) {
     s.sink = (int)min(max(p.sink[kh], (int64_t)0), (int64_t)n);
-    s.rows = (int)min((int64_t)n, s.sink + min(max(p.local[kh], (int64_t)0), (int64_t)n));
+    s.from = n - (int)min(max(p.local[kh], (int64_t)0), (int64_t)n);
   }
+  const int end = (n + 15) >> 4;
+  s.head = (s.sink + 15) >> 4;
+  s.tail = s.from == n ? end : max(s.head, s.from >> 4);
+  s.units = s.head + end - s.tail;
   return s;
 }
-__device__ __forceinline__ int units_of(int rows) { return (rows + kUnit - 1) / kUnit; }
 
 // A walk over the items of a block's part [lo, hi) of the line.
 struct Cursor {
@@ -259,7 +271,7 @@ struct Cursor {
   int u0, u1;                               // the units of the item that are in the part
   __device__ __forceinline__ void enter(const DecodeParams& p, int64_t lo, int64_t hi) {
     span = span_of(p, n, kh);
-    units = units_of(span.rows);
+    units = span.units;
     u0 = (int)min(max(lo - at, (int64_t)0), (int64_t)units);
     u1 = (int)min(hi - at, (int64_t)units);
   }
@@ -363,9 +375,9 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
   const int b_lo = min(tid * per, p.B), b_hi = min(b_lo + per, p.B);
   auto cost_of = [&](int b) {
     const int n = tokens_of(p, b);
-    if (!p.sink) return (int64_t)items_per_seq * (units_of(n) + kItemCost);
+    if (!p.sink) return (int64_t)items_per_seq * (((n + 15) >> 4) + kItemCost);
     int64_t sum = 0;
-    for (int kh = 0; kh < p.KV; ++kh) sum += units_of(span_of(p, n, kh).rows) + kItemCost;
+    for (int kh = 0; kh < p.KV; ++kh) sum += span_of(p, n, kh).units + kItemCost;
     return sum * p.tiles;
   };
   int64_t mine = 0;
@@ -398,7 +410,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
       const int n = tokens_of(p, b);
       int item = 0;
       for (;; ++item) {
-        const int64_t c = units_of(span_of(p, n, item / p.tiles).rows) + kItemCost;
+        const int64_t c = span_of(p, n, item / p.tiles).units + kItemCost;
         if (lo < at + c) break;
         at += c;
       }
@@ -419,26 +431,42 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
     Cursor ld = cur;
     bool ld_more = true;
     int ld_u = ld.u0 + warp;
-    int32_t ld_page = -1;                          // of row `lane % 16` of the unit that is loaded next
-    int ld_pos = -1;
+    int ld_x = 0;                                  // aligned unit that is loaded next, its attended positions and its page
+    uint32_t ld_mask = 0;                          // (of position lane % 16 when pages are smaller than a unit)
+    int32_t ld_page = -1;
+    bool ld_new_here = false;                      // sequence ld.b gets a new token at position ld.n - 1
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * kStages * L::kStageBytes;
     uint32_t* my_mask = sm_mask + warp * kStages;
+    const int l_row = lane / LPR, l_chunk = lane % LPR;
+    // where this lane's 16 bytes of rows l_row, l_row + RPI, ... go; the pattern repeats after 8 rows
+    uint32_t l_dst[8 / RPI];
+#pragma unroll
+    for (int i = 0; i < 8 / RPI; ++i) {
+      const int row = i * RPI + l_row;
+      l_dst[i] = row * RB + ((l_chunk ^ (row & 7)) << 4);
+    }
 
-    auto ld_seek = [&]() {                         // to the next unit of this warp, and look up its rows' pages
+    auto ld_look = [&]() {                         // look up the next unit's page
+      ld_x = ld.span.unit(ld_u);
+      ld_mask = ld.span.mask(ld_x);
+      const int32_t* row = p.pool.table + (int64_t)ld.b * p.pool.table_stride;
+      if (p.pool.shift >= 4) {
+        ld_page = row[ld_x >> (p.pool.shift - 4)];
+      } else {
+        const int pos = ld_x * 16 + (lane & 15);
+        ld_page = (ld_mask >> (lane & 15)) & 1 ? row[pos >> p.pool.shift] : -1;
+      }
+    };
+    auto ld_seek = [&]() {                         // to the next unit of this warp
       while (ld_u >= ld.u1) {
         if (!ld.next(p, lo, hi)) {
           ld_more = false;
           return;
         }
         ld_u = ld.u0 + warp;
+        ld_new_here = p.k_new && ld.n == (int64_t)p.lengths[ld.b] + 1;
       }
-      const int r = ld_u * kUnit + (lane & 15);
-      ld_pos = -1;
-      ld_page = -1;
-      if (r < ld.span.rows) {
-        ld_pos = r < ld.span.sink ? r : r + (ld.span.n - ld.span.rows);
-        ld_page = p.pool.table[(int64_t)ld.b * p.pool.table_stride + (ld_pos >> p.pool.shift)];
-      }
+      ld_look();
     };
 
     // The new token's row of (b, kh): rotated and rounded, into shared memory (stage address and row, row < 0:
@@ -486,39 +514,72 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
     auto ld_issue = [&](int stage) {
       if (ld_more) {
         const uint32_t dst = ring + stage * L::kStageBytes;
-        bool ok = (uint32_t)ld_page < (uint32_t)p.pool.num_pages && ld_pos >= 0;
-        const bool is_new = p.k_new && ld_pos >= 0 && ld_pos == ld.n - 1 && ld.n == (int64_t)p.lengths[ld.b] + 1;
-        if (ld_pos >= 0 && !ok && !is_new && lane < 16) report(kStatusAttend, ld.b, ld_pos, ld.kh);
-        const bool take = ok && !is_new;
-        const T* kp = reinterpret_cast<const T*>(p.pool.k);
-        const T* vp = reinterpret_cast<const T*>(p.pool.v);
-        if (take) {
-          kp += ld_page * p.pool.k_page + ld.kh * p.pool.k_head + (ld_pos & slot_mask) * p.pool.k_slot;
-          vp += ld_page * p.pool.v_page + ld.kh * p.pool.v_head + (ld_pos & slot_mask) * p.pool.v_slot;
-        }
-        const uint32_t taken = __ballot_sync(0xffffffffu, take) & 0xffffu;
-        const uint32_t fresh = __ballot_sync(0xffffffffu, is_new) & 0xffffu;     // written below, not copied
+        const uint32_t fresh = ld_new_here && ld_x == (ld.n - 1) >> 4 ? ld_mask & (1u << ((ld.n - 1) & 15)) : 0u;
+        uint32_t present = ld_mask & ~fresh;
+        if (p.pool.shift >= 4) {
+          const bool ok = (uint32_t)ld_page < (uint32_t)p.pool.num_pages;
+          if (!ok) {
+            if (present && lane == 0) report(kStatusAttend, ld.b, ld_x * 16 + __ffs(present) - 1, ld.kh);
+            present = 0;
+          }
+          const int64_t page = ok ? ld_page : 0, slot = ((ld_x << 4) & (int)slot_mask) + l_row;
+          const T* ks = reinterpret_cast<const T*>(p.pool.k) + page * p.pool.k_page + ld.kh * p.pool.k_head + slot * p.pool.k_slot + l_chunk * 8;
+          const T* vs = reinterpret_cast<const T*>(p.pool.v) + page * p.pool.v_page + ld.kh * p.pool.v_head + slot * p.pool.v_slot + l_chunk * 8;
+          const int64_t k_step = RPI * p.pool.k_slot, v_step = RPI * p.pool.v_slot;
+          if (present == 0xffffu) {
 #pragma unroll
-        for (int i = 0; i < kUnit / RPI; ++i) {
-          const int row = i * RPI + lane / LPR, chunk = lane % LPR;
-          const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(kp), row));
-          if (!((fresh >> row) & 1)) cp_async16(dst + row * RB + ((chunk ^ (row & 7)) << 4), src + chunk * 8, (taken >> row) & 1);
-        }
+            for (int i = 0; i < kUnit / RPI; ++i, ks += k_step)
+              cp_async16(dst + l_dst[i % (8 / RPI)] + i / (8 / RPI) * 8 * RB, ks, true);
 #pragma unroll
-        for (int i = 0; i < kUnit / RPI; ++i) {
-          const int row = i * RPI + lane / LPR, chunk = lane % LPR;
-          const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(vp), row));
-          if (!((fresh >> row) & 1)) cp_async16(dst + L::kTileBytes + row * RB + ((chunk ^ (row & 7)) << 4), src + chunk * 8, (taken >> row) & 1);
+            for (int i = 0; i < kUnit / RPI; ++i, vs += v_step)
+              cp_async16(dst + L::kTileBytes + l_dst[i % (8 / RPI)] + i / (8 / RPI) * 8 * RB, vs, true);
+          } else {
+#pragma unroll
+            for (int i = 0; i < kUnit / RPI; ++i, ks += k_step, vs += v_step) {
+              const int row = i * RPI + l_row;
+              const uint32_t to = dst + l_dst[i % (8 / RPI)] + i / (8 / RPI) * 8 * RB;
+              if ((fresh >> row) & 1) continue;
+              cp_async16(to, ks, (present >> row) & 1);
+              cp_async16(to + L::kTileBytes, vs, (present >> row) & 1);
+            }
+          }
+        } else {
+          // pages smaller than a unit: every row has its own place
+          const int pos = ld_x * 16 + (lane & 15);
+          bool take = (present >> (lane & 15)) & 1;
+          if (take && (uint32_t)ld_page >= (uint32_t)p.pool.num_pages) {
+            if (lane < 16) report(kStatusAttend, ld.b, pos, ld.kh);
+            take = false;
+          }
+          const T* ks = reinterpret_cast<const T*>(p.pool.k);
+          const T* vs = reinterpret_cast<const T*>(p.pool.v);
+          if (take) {
+            ks += ld_page * p.pool.k_page + ld.kh * p.pool.k_head + (pos & slot_mask) * p.pool.k_slot;
+            vs += ld_page * p.pool.v_page + ld.kh * p.pool.v_head + (pos & slot_mask) * p.pool.v_slot;
+          }
+          present = __ballot_sync(0xffffffffu, take) & 0xffffu;
+#pragma unroll 1
+          for (int i = 0; i < kUnit / RPI; ++i) {
+            const int row = i * RPI + l_row;
+            const T* k_row = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ks), row));
+            const T* v_row = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(vs), row));
+            const uint32_t to = dst + row * RB + ((l_chunk ^ (row & 7)) << 4);
+            if ((fresh >> row) & 1) continue;
+            cp_async16(to, k_row + l_chunk * 8, (present >> row) & 1);
+            cp_async16(to + L::kTileBytes, v_row + l_chunk * 8, (present >> row) & 1);
+          }
+          __syncwarp();
         }
-        uint32_t present = taken;
-        if (fresh && new_row(ld.b, ld.kh, ld.n, dst, __ffs(fresh) - 1, ld.tile == 0)) present |= fresh;
+        if (fresh && new_row(ld.b, ld.kh, ld.n, dst, (ld.n - 1) & 15, ld.tile == 0)) present |= fresh;
         if (lane == 0) my_mask[stage] = present;
         ld_u += kWarps;
-        ld_seek();
+        if (ld_u < ld.u1) ld_look();
+        else ld_seek();
       }
       cp_async_commit();
     };
 
+    ld_new_here = p.k_new && ld.n == (int64_t)p.lengths[ld.b] + 1;
     ld_seek();
 #pragma unroll 1
     for (int s = 0; s < kStages; ++s) ld_issue(s);
@@ -532,19 +593,22 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
       const bool owner = cur.at >= lo;             // the item begins in this part
       const bool with_new = p.k_new && cur.n > 0 && cur.n == (int64_t)p.lengths[cur.b] + 1;
       if (owner && warp == 0) {
-        if (with_new && cur.tile == 0 && !(cur.span.rows > cur.span.sink || cur.span.rows == cur.n))
+        if (with_new && cur.tile == 0 && cur.n > cur.span.sink && cur.span.from == cur.n)
           new_row(cur.b, cur.kh, cur.n, 0, -1, true);     // stored although the span does not reach it
         if (lane == 0 && cur.kh == 0 && cur.tile == 0 && p.lengths[cur.b] >= 0 &&
             (int64_t)p.lengths[cur.b] + (p.k_new ? 1 : 0) > p.capacity)
           report(kStatusLength, cur.b, (int64_t)p.lengths[cur.b] + (p.k_new ? 1 : 0), 0);
       }
-      auto store_out = [&](int head, int d, float o) {
+      // four coordinates of a head's result, sum of values over sum of weights (zeros where there is no weight)
+      auto store_out4 = [&](int head, int d, float4 O, float sum) {
         const int64_t off = (int64_t)cur.b * p.o_sb + (int64_t)(cur.kh * p.G + heads0 + head) * p.o_sh + d;
-        if (p.out_f32) reinterpret_cast<float*>(p.out)[off] = o;
-        else reinterpret_cast<T*>(p.out)[off] = static_cast<T>(o);
+        if (sum == 0.f) O = make_float4(0.f, 0.f, 0.f, 0.f);
+        else O = make_float4(O.x / sum, O.y / sum, O.z / sum, O.w / sum);
+        if (p.out_f32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + off) = O;
+        else *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + off) = make_uint2(Cvt<T>::pack(O.x, O.y), Cvt<T>::pack(O.z, O.w));
       };
       if (cur.units == 0) {                        // nothing to attend (only its owner gets here)
-        for (int i = tid; i < heads * D; i += kDecodeThreads) store_out(i / D, i % D, 0.f);
+        for (int i = tid * 4; i < heads * D; i += kDecodeThreads * 4) store_out4(i / D, i % D, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
         continue;
       }
       if (cur.u0 >= cur.u1) continue;              // only the item's cost lies in this part
@@ -685,20 +749,22 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
           }
         }
         __syncthreads();
-        for (int i = tid; i < here * D; i += kDecodeThreads) {
+        for (int i = tid * 4; i < here * D; i += kDecodeThreads * 4) {
           const int head = i / D, d = i % D;
-          float M = -INFINITY, Ls = 0.f, O = 0.f;
+          float M = -INFINITY, Ls = 0.f;
           for (int w = 0; w < nw; ++w) M = fmaxf(M, sm_m[w * 8 + head]);
           const float base = M == -INFINITY ? 0.f : M;
+          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
           for (int w = 0; w < nw; ++w) {
             const float f = exp2f(sm_m[w * 8 + head] - base);
+            const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * 8 + head) * L::kPitch + d);
             Ls += f * sm_l[w * 8 + head];
-            O += f * sm_o[(w * 8 + head) * L::kPitch + d];
+            O.x += f * x.x; O.y += f * x.y; O.z += f * x.z; O.w += f * x.w;
           }
           if (whole) {
-            store_out(mt * 8 + head, d, Ls == 0.f ? 0.f : O / Ls);
+            store_out4(mt * 8 + head, d, O, Ls);
           } else {
-            rec[(mt * 8 + head) * D + d] = O;
+            *reinterpret_cast<float4*>(rec + (mt * 8 + head) * D + d) = O;
             if (d == 0) *reinterpret_cast<float2*>(rec + kRecHeads * 128 + (mt * 8 + head) * 2) = make_float2(M, Ls);
           }
         }
@@ -757,11 +823,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
               O.x += f * x[i].x; O.y += f * x[i].y; O.z += f * x[i].z; O.w += f * x[i].w;
             }
           if (final) {
-            const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
-            store_out(head, d, Ls == 0.f ? 0.f : O.x * inv);
-            store_out(head, d + 1, Ls == 0.f ? 0.f : O.y * inv);
-            store_out(head, d + 2, Ls == 0.f ? 0.f : O.z * inv);
-            store_out(head, d + 3, Ls == 0.f ? 0.f : O.w * inv);
+            store_out4(head, d, O, Ls);
           } else {
             // (each element of the group's first record is read by the thread that writes it)
             *reinterpret_cast<float4*>(to + i4 * 4) = O;
@@ -934,6 +996,8 @@ int moa_paged_decode(const moa_paged_decode_args* args, moa_stream_t stream) {
   MOA_REQUIRE(aligned16(a.q) && aligned16(a.k_new) && aligned16(a.v_new) &&
                   multiples_of_8({a.q_sb, a.q_sh, a.k_sb, a.k_sh, a.v_sb, a.v_sh}),
               "paged_decode: rows must be 16-byte aligned with strides that are multiples of 8 elements");
+  MOA_REQUIRE(aligned16(a.out) && multiples_of_8({a.o_sb, a.o_sh}),
+              "paged_decode: rows of out must be 16-byte aligned with strides that are multiples of 8 elements");
   if (!a.workspace || a.workspace_bytes < moa_paged_decode_workspace_bytes()) {
     set_error_text("paged_decode: workspace missing or smaller than moa_paged_decode_workspace_bytes()");
     return MOA_ERR_WORKSPACE;

@@ -173,7 +173,7 @@ def test_append_entry_checks_its_arguments(changes, status, text):
     (dict(q=0), 1, b"null"), (dict(out=0), 1, b"null"), (dict(page_table=0), 1, b"null"), (dict(KV=0), 1, b"shape"),
     (dict(H=5), 1, b"multiple"), (dict(k_new=A), 1, b"go together"), (dict(sink_size=A), 1, b"go together"),
     (dict(advance=1), 1, b"new token"), (dict(rope_cos=A, rope_sin=A), 1, b"new token"), (dict(q=A + 2), 1, b"aligned"),
-    (dict(page_size=0), 1, b"power of two"), (dict(workspace=0), 4, b"workspace"), (dict(workspace_bytes=100), 4, b"workspace"),
+    (dict(out=A + 8), 1, b"rows of out"), (dict(o_sh=68), 1, b"rows of out"), (dict(page_size=0), 1, b"power of two"), (dict(workspace=0), 4, b"workspace"), (dict(workspace_bytes=100), 4, b"workspace"),
     (dict(D=80), 2, b"head_dim"), (dict(dtype=2), 2, b"dtype"),
 ])
 def test_decode_entry_checks_its_arguments(changes, status, text):
