@@ -263,7 +263,8 @@ int moa_rope_qk(void* q, void* k, int64_t sb, int64_t sh, int64_t sn, const void
  * reported by moa_paged_status:
  *   {31, sequence, position, 0} an appended token, {32, sequence, position, head} an attended one without a page,
  *   {33, sequence, position, 0} a position behind the last rope row, {34, sequence, length, 0} a length beyond
- *   the page table's width (the tokens behind it are left out).
+ *   the page table's width (the tokens behind it are left out), {35, block, thread, 0} a load that did not arrive
+ *   within a second (the output is then invalid).
  * Pages may be shared between sequences for reading.  Two tokens of one call that land in the same place are
  * the caller's mistake: one of them is stored.
  *

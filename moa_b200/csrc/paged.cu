@@ -8,12 +8,14 @@
 #include <initializer_list>
 #include <type_traits>
 
+#include <cuda.h>
+
 #include "common.cuh"
 
 namespace moa {
 namespace {
 
-constexpr int kStatusAppend = 31, kStatusAttend = 32, kStatusRope = 33, kStatusLength = 34;
+constexpr int kStatusAppend = 31, kStatusAttend = 32, kStatusRope = 33, kStatusLength = 34, kStatusWait = 35;
 __device__ int32_t g_paged_status[4];
 
 __device__ __noinline__ void report(int code, int64_t b, int64_t at, int more) {
@@ -193,8 +195,10 @@ __global__ void paged_advance_kernel(int32_t* lengths, const int32_t* counts, in
 // order, so results do not depend on timing.  No block waits for another.
 //
 // Loads.  The 8 warps of a block take the units of a segment in turn.  Each warp runs its own ring of kStages
-// units in shared memory, filled with cp.async by a cursor that runs ahead of the arithmetic, over the ends of
-// items too, so the epilogue of one item overlaps with the loads of the next: 192 KB in flight per SM.
+// units in shared memory, filled by a cursor that runs ahead of the arithmetic, over the ends of items too, so the
+// epilogue of one item overlaps with the loads of the next: 192 KB in flight per SM.  A unit that is attended in
+// full comes with TMA (one lane's few instructions; the warps' issue slots are what runs out first), one that is
+// not with cp.async, which leaves masked rows zero: what a page holds behind its last token may be anything.
 //
 // Arithmetic.  m16n8k16 tensor instructions with the 8 query heads of a tile in rows 0-7 and, where an operand
 // does not fit 16 bits, its remainder in rows 8-15: the weights w are held to 16 + 16 bits that way (hi + lo),
@@ -207,6 +211,7 @@ constexpr int kMinUnits = 8;                // least share of a block: fewer blo
 constexpr int kJoin = 16;                   // partial results joined at once
 constexpr int kMaxBlocks = 256;           // kJoin * kJoin: two levels of joining reach it
 constexpr int kRecHeads = 16;
+constexpr uint32_t kByHand = 0x80000000u;   // in a stage's mask: filled with cp.async
 constexpr int64_t kRecFloats = kRecHeads * (128 + 2);
 
 struct DecodeParams {
@@ -219,7 +224,7 @@ struct DecodeParams {
   int B, H, KV, G, tiles;                   // tiles of query heads per key head
   int capacity;                             // positions that a row of the page table reaches
   float scale_log2;
-  int out_f32, advance;
+  int out_f32, advance, tma;
   int* counters;                            // 3 per block, zero between launches, and one behind them
   float* records;                           // 2 per block
 };
@@ -295,9 +300,44 @@ struct Cursor {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// orders this thread's ordinary writes to shared memory before later TMA writes to the same place
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void bar_init(uint32_t bar) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+constexpr long long kWaitCycles = 2000000000ll;       // about a second
+// Bounded: a load that never arrives is reported, the warp stops waiting and the kernel goes on to its end.
+__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity) {
+  const long long start = clock64();
+  while (!bar_try(bar, parity))
+    if (clock64() - start > kWaitCycles) {
+      report(kStatusWait, blockIdx.x, threadIdx.x, 0);
+      return false;
+    }
+  return true;
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+  return bar_try(bar, parity) || bar_wait_slow(bar, parity);
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int d, int slot, int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(d), "r"(slot), "r"(head), "r"(page) : "memory");
+}
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -323,9 +363,10 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uin
 }
 
 // x = hi + lo with both in T, for two values; hi of an fp16 that does not fit is its largest, lo takes the rest.
-template <typename T>
+// (A weight fits: it is 1 at most.)
+template <typename T, bool LARGE>
 __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-  if (std::is_same<T, __half>::value) {
+  if (LARGE && std::is_same<T, __half>::value) {
     hi = Cvt<T>::pack(fminf(fmaxf(x0, -65504.f), 65504.f), fminf(fmaxf(x1, -65504.f), 65504.f));
   } else {
     hi = Cvt<T>::pack(x0, x1);
@@ -342,25 +383,36 @@ __device__ __forceinline__ float2 load_table2(const Pool& p, const void* t, int6
   return Cvt<T>::unpack(*reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(t) + off));
 }
 
+// A unit's keys (and values) are D/64 panels of 16 rows of 128 bytes, 16-byte chunk c of row r at c ^ (r % 8): TMA's
+// 128-byte swizzle, which ldmatrix reads without bank conflicts.
 template <int D>
 struct Layout {
-  static constexpr int kRowBytes = D * 2, kTileBytes = kUnit * kRowBytes, kStageBytes = 2 * kTileBytes;
+  static constexpr int kPanelBytes = kUnit * 128, kTileBytes = kUnit * D * 2, kStageBytes = 2 * kTileBytes;
   static constexpr int kStages = D == 128 ? 3 : 6;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kPitch = D + 8;                                 // floats per head in the join buffer
+  static constexpr int kPitch = D + 4;                                 // floats per head in the join buffer
   static constexpr int kJoinBytes = kWarps * 8 * kPitch * 4;
-  static constexpr int kBytes = kRing + kJoinBytes + kWarps * kStages * 4 + 2 * kWarps * 8 * 4 + 128;
+  static constexpr int kBarBytes = kWarps * kStages * 8, kMaskBytes = kWarps * kStages * 4;
+  static constexpr int kBytes = 1024 + kRing + kJoinBytes + kBarBytes + kMaskBytes + 2 * kWarps * 8 * 4 + 128;
+  static_assert(kBytes <= 232448, "shared memory");
+  static __device__ __forceinline__ uint32_t at(int row, int chunk) {
+    return (chunk >> 3) * kPanelBytes + row * 128 + (((chunk ^ row) & 7) << 4);
+  }
 };
 
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                        const __grid_constant__ CUtensorMap map_v,
+                                                                        const __grid_constant__ DecodeParams p) {
   using L = Layout<D>;
-  constexpr int kStages = L::kStages, RB = L::kRowBytes;
+  constexpr int kStages = L::kStages;
   constexpr int LPR = D / 8, RPI = 32 / LPR;      // lanes per row, rows per load instruction
   constexpr int KS = D / 16;                      // k steps of the first product, pairs of n tiles of the second
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* sm_o = reinterpret_cast<float*>(smem + L::kRing);
-  uint32_t* sm_mask = reinterpret_cast<uint32_t*>(smem + L::kRing + L::kJoinBytes);
+  unsigned char* sm_bar = smem + L::kRing + L::kJoinBytes;
+  uint32_t* sm_mask = reinterpret_cast<uint32_t*>(sm_bar + L::kBarBytes);
   float* sm_m = reinterpret_cast<float*>(sm_mask + kWarps * kStages);
   float* sm_l = sm_m + kWarps * 8;
   int64_t* sm_scan = reinterpret_cast<int64_t*>(sm_l + kWarps * 8);   // 8 warp sums, then {b, item of b, at} of the part
@@ -437,14 +489,12 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
     bool ld_new_here = false;                      // sequence ld.b gets a new token at position ld.n - 1
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * kStages * L::kStageBytes;
     uint32_t* my_mask = sm_mask + warp * kStages;
-    const int l_row = lane / LPR, l_chunk = lane % LPR;
-    // where this lane's 16 bytes of rows l_row, l_row + RPI, ... go; the pattern repeats after 8 rows
-    uint32_t l_dst[8 / RPI];
-#pragma unroll
-    for (int i = 0; i < 8 / RPI; ++i) {
-      const int row = i * RPI + l_row;
-      l_dst[i] = row * RB + ((l_chunk ^ (row & 7)) << 4);
+    const uint32_t bars = (uint32_t)__cvta_generic_to_shared(sm_bar) + warp * kStages * 8;
+    if (lane < kStages) {
+      bar_init(bars + lane * 8);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncwarp();
 
     auto ld_look = [&]() {                         // look up the next unit's page
       ld_x = ld.span.unit(ld_u);
@@ -503,7 +553,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int chunk = lane + (i & 1) * (D / 16);
-            const uint32_t a = stage_addr + (i >> 1) * L::kTileBytes + row * RB + ((chunk ^ (row & 7)) << 4);
+            const uint32_t a = stage_addr + (i >> 1) * L::kTileBytes + L::at(row, chunk);
             asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x[i].x), "r"(x[i].y), "r"(x[i].z), "r"(x[i].w) : "memory");
           }
         }
@@ -511,72 +561,62 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
       return placed;
     };
 
+    // The rows of a unit one by one: zeros where nothing is attended, nothing in place of the new token's.  `present` loses
+    // the rows without a page.
+    auto ld_rows = [&](uint32_t dst, uint32_t& present, uint32_t fresh) {
+      const int pos = ld_x * 16 + (lane & 15);
+      bool take = (present >> (lane & 15)) & 1;
+      if (take && (uint32_t)ld_page >= (uint32_t)p.pool.num_pages) {
+        if (lane < 16) report(kStatusAttend, ld.b, pos, ld.kh);
+        take = false;
+      }
+      const T* ks = reinterpret_cast<const T*>(p.pool.k);
+      const T* vs = reinterpret_cast<const T*>(p.pool.v);
+      if (take) {
+        ks += ld_page * p.pool.k_page + ld.kh * p.pool.k_head + (pos & slot_mask) * p.pool.k_slot;
+        vs += ld_page * p.pool.v_page + ld.kh * p.pool.v_head + (pos & slot_mask) * p.pool.v_slot;
+      }
+      present = __ballot_sync(0xffffffffu, take) & 0xffffu;
+#pragma unroll 2
+      for (int i = 0; i < kUnit / RPI; ++i) {
+        const int row = i * RPI + lane / LPR, chunk = lane % LPR;
+        const T* k_row = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ks), row));
+        const T* v_row = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(vs), row));
+        if ((fresh >> row) & 1) continue;
+        cp_async16(dst + L::at(row, chunk), k_row + chunk * 8, (present >> row) & 1);
+        cp_async16(dst + L::kTileBytes + L::at(row, chunk), v_row + chunk * 8, (present >> row) & 1);
+      }
+      __syncwarp();
+    };
+
     auto ld_issue = [&](int stage) {
       if (ld_more) {
         const uint32_t dst = ring + stage * L::kStageBytes;
         const uint32_t fresh = ld_new_here && ld_x == (ld.n - 1) >> 4 ? ld_mask & (1u << ((ld.n - 1) & 15)) : 0u;
         uint32_t present = ld_mask & ~fresh;
-        if (p.pool.shift >= 4) {
-          const bool ok = (uint32_t)ld_page < (uint32_t)p.pool.num_pages;
-          if (!ok) {
-            if (present && lane == 0) report(kStatusAttend, ld.b, ld_x * 16 + __ffs(present) - 1, ld.kh);
-            present = 0;
-          }
-          const int64_t page = ok ? ld_page : 0, slot = ((ld_x << 4) & (int)slot_mask) + l_row;
-          const T* ks = reinterpret_cast<const T*>(p.pool.k) + page * p.pool.k_page + ld.kh * p.pool.k_head + slot * p.pool.k_slot + l_chunk * 8;
-          const T* vs = reinterpret_cast<const T*>(p.pool.v) + page * p.pool.v_page + ld.kh * p.pool.v_head + slot * p.pool.v_slot + l_chunk * 8;
-          const int64_t k_step = RPI * p.pool.k_slot, v_step = RPI * p.pool.v_slot;
-          if (present == 0xffffu) {
+        if (present == 0xffffu && p.tma && (uint32_t)ld_page < (uint32_t)p.pool.num_pages) {
+          if (lane == 0) {
+            const int slot = (ld_x << 4) & (int)slot_mask;
+            const uint32_t bar = bars + stage * 8;
+            my_mask[stage] = 0xffffu;          // seen by the other lanes when they have waited on the barrier
+            bar_expect(bar, L::kStageBytes);
 #pragma unroll
-            for (int i = 0; i < kUnit / RPI; ++i, ks += k_step)
-              cp_async16(dst + l_dst[i % (8 / RPI)] + i / (8 / RPI) * 8 * RB, ks, true);
+            for (int i = 0; i < D / 64; ++i) tma_load(dst + i * L::kPanelBytes, &map_k, bar, i * 64, slot, ld.kh, ld_page);
 #pragma unroll
-            for (int i = 0; i < kUnit / RPI; ++i, vs += v_step)
-              cp_async16(dst + L::kTileBytes + l_dst[i % (8 / RPI)] + i / (8 / RPI) * 8 * RB, vs, true);
-          } else {
-#pragma unroll
-            for (int i = 0; i < kUnit / RPI; ++i, ks += k_step, vs += v_step) {
-              const int row = i * RPI + l_row;
-              const uint32_t to = dst + l_dst[i % (8 / RPI)] + i / (8 / RPI) * 8 * RB;
-              if ((fresh >> row) & 1) continue;
-              cp_async16(to, ks, (present >> row) & 1);
-              cp_async16(to + L::kTileBytes, vs, (present >> row) & 1);
-            }
+            for (int i = 0; i < D / 64; ++i) tma_load(dst + L::kTileBytes + i * L::kPanelBytes, &map_v, bar, i * 64, slot, ld.kh, ld_page);
           }
         } else {
-          // pages smaller than a unit: every row has its own place
-          const int pos = ld_x * 16 + (lane & 15);
-          bool take = (present >> (lane & 15)) & 1;
-          if (take && (uint32_t)ld_page >= (uint32_t)p.pool.num_pages) {
-            if (lane < 16) report(kStatusAttend, ld.b, pos, ld.kh);
-            take = false;
+          ld_rows(dst, present, fresh);
+          if (fresh && new_row(ld.b, ld.kh, ld.n, dst, (ld.n - 1) & 15, ld.tile == 0)) present |= fresh;
+          if (lane == 0) {
+            my_mask[stage] = present | kByHand;
+            bar_arrive(bars + stage * 8);
           }
-          const T* ks = reinterpret_cast<const T*>(p.pool.k);
-          const T* vs = reinterpret_cast<const T*>(p.pool.v);
-          if (take) {
-            ks += ld_page * p.pool.k_page + ld.kh * p.pool.k_head + (pos & slot_mask) * p.pool.k_slot;
-            vs += ld_page * p.pool.v_page + ld.kh * p.pool.v_head + (pos & slot_mask) * p.pool.v_slot;
-          }
-          present = __ballot_sync(0xffffffffu, take) & 0xffffu;
-#pragma unroll 1
-          for (int i = 0; i < kUnit / RPI; ++i) {
-            const int row = i * RPI + l_row;
-            const T* k_row = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ks), row));
-            const T* v_row = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(vs), row));
-            const uint32_t to = dst + row * RB + ((l_chunk ^ (row & 7)) << 4);
-            if ((fresh >> row) & 1) continue;
-            cp_async16(to, k_row + l_chunk * 8, (present >> row) & 1);
-            cp_async16(to + L::kTileBytes, v_row + l_chunk * 8, (present >> row) & 1);
-          }
-          __syncwarp();
         }
-        if (fresh && new_row(ld.b, ld.kh, ld.n, dst, (ld.n - 1) & 15, ld.tile == 0)) present |= fresh;
-        if (lane == 0) my_mask[stage] = present;
         ld_u += kWarps;
         if (ld_u < ld.u1) ld_look();
         else ld_seek();
       }
-      cp_async_commit();
     };
 
     ld_new_here = p.k_new && ld.n == (int64_t)p.lengths[ld.b] + 1;
@@ -587,6 +627,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
     // ---- items
     const int g = lane >> 2, t = lane & 3;         // row (query head of a tile) and column pair of a fragment
     int stage = 0;
+    uint32_t parity = 0;
+    bool waiting = true;                           // until a wait runs out
     do {
       const int heads0 = cur.tile * 8 * MT;        // first query head of the tile within its key head's group
       const int heads = min(p.G - heads0, 8 * MT);
@@ -647,34 +689,37 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
                 const float2 cl = load_table2<T>(p.pool, p.pool.cos, rope + d), ch = load_table2<T>(p.pool, p.pool.cos, rope + d + D / 2);
                 const float2 sl = load_table2<T>(p.pool, p.pool.sin, rope + d), sh = load_table2<T>(p.pool, p.pool.sin, rope + d + D / 2);
                 const float2 a = Cvt<T>::unpack(qa[mt][ks][e]), b = Cvt<T>::unpack(qa[mt][ks + KS / 2][e]);
-                split2<T>(fmaf(a.x, cl.x, -b.x * sl.x), fmaf(a.y, cl.y, -b.y * sl.y), qa[mt][ks][e], qa[mt][ks][e + 1]);
-                split2<T>(fmaf(b.x, ch.x, a.x * sh.x), fmaf(b.y, ch.y, a.y * sh.y), qa[mt][ks + KS / 2][e], qa[mt][ks + KS / 2][e + 1]);
+                split2<T, true>(fmaf(a.x, cl.x, -b.x * sl.x), fmaf(a.y, cl.y, -b.y * sl.y), qa[mt][ks][e], qa[mt][ks][e + 1]);
+                split2<T, true>(fmaf(b.x, ch.x, a.x * sh.x), fmaf(b.y, ch.y, a.y * sh.y), qa[mt][ks + KS / 2][e], qa[mt][ks + KS / 2][e + 1]);
               }
           }
         }
+        // ldmatrix addresses within a tile: four chunk pairs of a panel, the other panel behind them
         const int mi = lane >> 3, r8 = lane & 7;
+        const uint32_t k_at = ((mi >> 1) * 8 + r8) * 128 + (((mi & 1) ^ r8) << 4);
+        const uint32_t v_at = L::kTileBytes + ((mi & 1) * 8 + r8) * 128 + (((mi >> 1) ^ r8) << 4);
 #pragma unroll 1
         for (int u = cur.u0 + warp; u < cur.u1; u += kWarps) {
-          cp_async_wait<kStages - 1>();
-          __syncwarp();
-          const uint32_t ka = ring + stage * L::kStageBytes, va = ka + L::kTileBytes;
-          const uint32_t present = my_mask[stage] >> (2 * t);
+          if (waiting) waiting = __all_sync(0xffffffffu, bar_wait(bars + stage * 8, parity));
+          const uint32_t base = ring + stage * L::kStageBytes;
+          const uint32_t present = my_mask[stage];
+          if (present & kByHand) {
+            cp_async_wait_all();
+            __syncwarp();
+          }
           float sc[MT][2][4];
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[mt][0][e] = sc[mt][1][e] = 0.f;
-          {
-            const uint32_t base = ka + ((mi >> 1) * 8 + r8) * RB;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-              uint32_t kb[4];
-              ldmatrix4(kb, base + (((2 * ks + (mi & 1)) ^ r8) << 4));
+          for (int ks = 0; ks < KS; ++ks) {
+            uint32_t kb[4];
+            ldmatrix4(kb, ((base + k_at) ^ ((ks & 3) << 5)) + (ks >> 2) * L::kPanelBytes);
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                mma16816<T>(sc[mt][0], qa[mt][ks], kb[0], kb[1]);
-                mma16816<T>(sc[mt][1], qa[mt][ks], kb[2], kb[3]);
-              }
+            for (int mt = 0; mt < MT; ++mt) {
+              mma16816<T>(sc[mt][0], qa[mt][ks], kb[0], kb[1]);
+              mma16816<T>(sc[mt][1], qa[mt][ks], kb[2], kb[3]);
             }
           }
           uint32_t pa[MT][4];
@@ -682,46 +727,56 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
           for (int mt = 0; mt < MT; ++mt) {
             float s[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float hi_part = sc[mt][e >> 1][e & 1], lo_part = sc[mt][e >> 1][(e & 1) + 2];
-              const float v = (split ? joined(hi_part, lo_part) : hi_part) * p.scale_log2;
-              s[e] = (present >> ((e >> 1) * 8 + (e & 1))) & 1 ? v : -INFINITY;
+            for (int e = 0; e < 4; ++e) s[e] = sc[mt][e >> 1][e & 1];
+            if (split) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[e] = joined(s[e], sc[mt][e >> 1][(e & 1) + 2]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] *= p.scale_log2;
+            if (present != 0xffffu) {
+              const uint32_t mine16 = present >> (2 * t);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (!((mine16 >> ((e >> 1) * 8 + (e & 1))) & 1)) s[e] = -INFINITY;
             }
             float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float m_new = fmaxf(m[mt], top), base = m_new == -INFINITY ? 0.f : m_new;
-            const float corr = exp2f(m[mt] - base);
-            float w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = exp2f(s[e] - base);
-            l[mt] = l[mt] * corr + ((w[0] + w[1]) + (w[2] + w[3]));
-            split2<T>(w[0], w[1], pa[mt][0], pa[mt][1]);
-            split2<T>(w[2], w[3], pa[mt][2], pa[mt][3]);
-            if (__any_sync(0xffffffffu, m_new != m[mt])) {
+            if (__any_sync(0xffffffffu, top > m[mt])) {      // a new maximum: what there is so far is scaled down
+              const float m_new = fmaxf(m[mt], top);
+              const float corr = m_new == -INFINITY ? 1.f : exp2f(m[mt] - m_new);
+              m[mt] = m_new;
+              l[mt] *= corr;
 #pragma unroll
               for (int j = 0; j < D / 8; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[mt][j][e] *= corr;
             }
-            m[mt] = m_new;
+            const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] = exp2f(s[e] - ref);
+            l[mt] += (s[0] + s[1]) + (s[2] + s[3]);
+            split2<T, false>(s[0], s[1], pa[mt][0], pa[mt][1]);
+            split2<T, false>(s[2], s[3], pa[mt][2], pa[mt][3]);
           }
-          {
-            const uint32_t base = va + ((mi & 1) * 8 + r8) * RB;
 #pragma unroll
-            for (int j = 0; j < KS; ++j) {
-              uint32_t vb[4];
-              ldmatrix4_trans(vb, base + (((2 * j + (mi >> 1)) ^ r8) << 4));
+          for (int j = 0; j < KS; ++j) {
+            uint32_t vb[4];
+            ldmatrix4_trans(vb, ((base + v_at) ^ ((j & 3) << 5)) + (j >> 2) * L::kPanelBytes);
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                mma16816<T>(acc[mt][2 * j], pa[mt], vb[0], vb[1]);
-                mma16816<T>(acc[mt][2 * j + 1], pa[mt], vb[2], vb[3]);
-              }
+            for (int mt = 0; mt < MT; ++mt) {
+              mma16816<T>(acc[mt][2 * j], pa[mt], vb[0], vb[1]);
+              mma16816<T>(acc[mt][2 * j + 1], pa[mt], vb[2], vb[3]);
             }
           }
+          if (present & kByHand) proxy_fence();
           __syncwarp();
           ld_issue(stage);
-          stage = stage + 1 == kStages ? 0 : stage + 1;
+          if (++stage == kStages) {
+            stage = 0;
+            parity ^= 1;
+          }
         }
       }
 
@@ -834,7 +889,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
       }
       __syncthreads();                             // sm_o is free again
     } while (cur.next(p, lo, hi));
-    cp_async_wait<0>();
   }
 
   if (p.advance) {                                 // the last block to get here: every block has read the lengths
@@ -867,8 +921,35 @@ int sm_count() {
   return cached[dev];
 }
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The pool as a tensor (D, slots, heads, pages) that is loaded in panels of 16 rows of 64 values.  False when the
+// strides are none that TMA takes.
+bool make_map(CUtensorMap* map, const void* base, const DecodeParams& p, int64_t page, int64_t head, int64_t slot, int D,
+              bool bf16) {
+  static EncodeTiledFn encode = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      (void)cudaGetLastError();
+      ptr = nullptr;
+    }
+    return reinterpret_cast<EncodeTiledFn>(ptr);
+  }();
+  if (!encode) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)1 << p.pool.shift, (cuuint64_t)p.KV, (cuuint64_t)p.pool.num_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)slot * 2, (cuuint64_t)head * 2, (cuuint64_t)page * 2};
+  const cuuint32_t box[4] = {64, kUnit, 1, 1}, step[4] = {1, 1, 1, 1};
+  return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
+                dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D, int MT>
-int launch_decode(const DecodeParams& p, int grid, cudaStream_t stream) {
+int launch_decode(DecodeParams& p, int grid, cudaStream_t stream) {
   static bool ready[kMaxDevices];
   int dev = 0;
   MOA_CUDA_CHECK(cudaGetDevice(&dev));
@@ -876,12 +957,17 @@ int launch_decode(const DecodeParams& p, int grid, cudaStream_t stream) {
     MOA_CUDA_CHECK(cudaFuncSetAttribute(paged_decode_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kBytes));
     if (dev >= 0 && dev < kMaxDevices) ready[dev] = true;
   }
-  paged_decode_kernel<T, D, MT><<<grid, kDecodeThreads, Layout<D>::kBytes, stream>>>(p);
+  CUtensorMap map_k, map_v;
+  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  p.tma = p.pool.shift >= 4 &&      // a unit lies in one page
+          make_map(&map_k, p.pool.k, p, p.pool.k_page, p.pool.k_head, p.pool.k_slot, D, bf16) &&
+          make_map(&map_v, p.pool.v, p, p.pool.v_page, p.pool.v_head, p.pool.v_slot, D, bf16);
+  paged_decode_kernel<T, D, MT><<<grid, kDecodeThreads, Layout<D>::kBytes, stream>>>(map_k, map_v, p);
   MOA_CUDA_CHECK(cudaGetLastError());
   return MOA_OK;
 }
 template <typename T>
-int launch_decode(const DecodeParams& p, int D, int grid, cudaStream_t stream) {
+int launch_decode(DecodeParams& p, int D, int grid, cudaStream_t stream) {
   if (D == 128) return p.G > 8 ? launch_decode<T, 128, 2>(p, grid, stream) : launch_decode<T, 128, 1>(p, grid, stream);
   return p.G > 8 ? launch_decode<T, 64, 2>(p, grid, stream) : launch_decode<T, 64, 1>(p, grid, stream);
 }

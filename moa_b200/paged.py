@@ -259,7 +259,8 @@ def paged_decode(query: Tensor, key_pages: Tensor, value_pages: Tensor, page_tab
 _STATUS = {31: ("moa_paged_append", "no page for a new token of sequence {0} at position {1}: it was not stored"),
            32: ("moa_paged_decode", "no page for position {1} of sequence {0} (head {2}): it was not attended"),
            33: ("moa_paged_append", "no rope row for a new token of sequence {0} at position {1}: it was not stored"),
-           34: ("moa_paged_decode", "sequence {0} has {1} tokens, more than its row of the page table holds")}
+           34: ("moa_paged_decode", "sequence {0} has {1} tokens, more than its row of the page table holds"),
+           35: ("moa_paged_decode", "a load did not arrive (block {0}, thread {1}): the output is invalid")}
 
 
 def check_status(device=None) -> None:
