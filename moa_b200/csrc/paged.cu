@@ -186,31 +186,39 @@ __global__ void paged_advance_kernel(int32_t* lengths, const int32_t* counts, in
 // Every key and value row is read once and used for all query heads that share it, G flops a byte: the kernel
 // is bound by memory, and is built to keep loads in flight.
 //
-// Work.  An item is (sequence, key head, tile of up to 8*MT query heads).  Its rows are counted in units of 16;
+// Work.  An item is (sequence, key head, tile of up to 8*MT query heads).  Its positions are counted in units of 16;
 // all items' units, and kItemCost more per item for its epilogue, are laid out on one line that is cut into
-// equal parts, one per block (one block per SM).  A block therefore moves the same number of bytes however
+// equal parts, one per block (two blocks per SM).  A block therefore moves the same number of bytes however
 // ragged the lengths are, and the cut is computed on the device from `lengths` alone: nothing is planned on the
 // host, and a captured launch stays right when the lengths change.  An item that is cut leaves one partial
 // result (maximum, sum, sum of values) per block; the block that finishes last joins them, in the blocks'
 // order, so results do not depend on timing.  No block waits for another.
 //
-// Loads.  The 8 warps of a block take the units of a segment in turn.  Each warp runs its own ring of kStages
+// Loads.  The warps of a block take the units of a segment in turn.  Each warp runs its own ring of kStages
 // units in shared memory, filled by a cursor that runs ahead of the arithmetic, over the ends of items too, so the
-// epilogue of one item overlaps with the loads of the next: 192 KB in flight per SM.  A unit that is attended in
-// full comes with TMA (one lane's few instructions; the warps' issue slots are what runs out first), one that is
-// not with cp.async, which leaves masked rows zero: what a page holds behind its last token may be anything.
+// epilogue of one item overlaps with the loads of the next.  128 KB are in flight per SM: less leaves bandwidth
+// unused, more only makes every load, look-up and join wait longer in the memory's queues (192 KB: 3 % slower).
+// A unit that is attended in full comes with TMA (one lane's few instructions), one that is not with cp.async,
+// which leaves masked rows zero: what a page holds behind its last token may be anything.  What else an item
+// needs (queries, the new token's rows) is fetched while the item before it is worked on.
 //
 // Arithmetic.  m16n8k16 tensor instructions with the 8 query heads of a tile in rows 0-7 and, where an operand
 // does not fit 16 bits, its remainder in rows 8-15: the weights w are held to 16 + 16 bits that way (hi + lo),
 // and so is the rotated query of the fused step.  Rows 8-15 would idle otherwise (G is small), so the result has
 // fp32 weights at no cost.  MT = 2 serves 9..16 heads with one pass over the keys.
-constexpr int kWarps = 8, kDecodeThreads = kWarps * 32;
+//
+// The fused step's new token is where one warp of the block that ends the item starts from (its score is the first
+// maximum, its value the first sum); it is stored into its page at the same time and read from no page.
+constexpr int kWarps = 4, kDecodeThreads = kWarps * 32;
+constexpr int kPerSm = 2;                   // resident blocks per SM
 constexpr int kUnit = 16;                   // positions of a unit (k of the second product)
 constexpr int kItemCost = 2;                // an item's epilogue, in units
 constexpr int kMinUnits = 8;                // least share of a block: fewer blocks work when there is less
-constexpr int kJoin = 16;                   // partial results joined at once
-constexpr int kMaxBlocks = 256;           // kJoin * kJoin: two levels of joining reach it
+constexpr int kJoin = 18;                   // partial results joined at once
+constexpr int kMaxParts = kJoin * kJoin;    // two levels of joining
+constexpr int kCounters = 3;                // per part
 constexpr int kRecHeads = 16;
+constexpr int kCached = 256;                // lengths and spans held in shared memory; the others are read where they are
 constexpr uint32_t kByHand = 0x80000000u;   // in a stage's mask: filled with cp.async
 constexpr int64_t kRecFloats = kRecHeads * (128 + 2);
 
@@ -225,8 +233,33 @@ struct DecodeParams {
   int capacity;                             // positions that a row of the page table reaches
   float scale_log2;
   int out_f32, advance, tma;
-  int* counters;                            // 3 per block, zero between launches, and one behind them
-  float* records;                           // 2 per block
+  int* counters;                            // kCounters per part, zero between launches, and one behind them
+  float* records;                           // 2 per part
+};
+
+// The lengths and spans as a block sees them.
+struct Sizes {
+  const DecodeParams& p;
+  const int* len;                           // shared memory, kCached each
+  const int2* span;
+  __device__ __forceinline__ int length(int b) const { return b < kCached ? len[b] : p.lengths[b]; }
+  // Tokens of sequence b, the new one included, as far as the page table reaches.
+  __device__ __forceinline__ int tokens(int b) const {
+    const int n = length(b);
+    return n < 0 ? 0 : min(n + (p.k_new && n < p.capacity ? 1 : 0), p.capacity);
+  }
+  // Whether the new token of sequence b is one of them.
+  __device__ __forceinline__ bool fresh(int b) const {
+    const int n = length(b);
+    return p.k_new && n >= 0 && n < p.capacity;
+  }
+  static __device__ __forceinline__ int2 clamped(int64_t sink, int64_t local) {
+    const int64_t most = 2147483647;
+    return make_int2((int)min(max(sink, (int64_t)0), most), (int)min(max(local, (int64_t)0), most));
+  }
+  __device__ __forceinline__ int2 sink_local(int kh) const {
+    return kh < kCached ? span[kh] : clamped(p.sink[kh], p.local[kh]);
+  }
 };
 
 // The units of one (sequence, key head): 16 positions each, aligned, so that with pages of 16 and more a unit
@@ -234,6 +267,19 @@ struct DecodeParams {
 // positions from `from` on; positions < n outside both are masked.
 struct Span {
   int n, sink, from, head, tail, units;
+  __device__ __forceinline__ Span() {}
+  __device__ __forceinline__ Span(const Sizes& s, int tokens, int kh) {
+    n = sink = from = tokens;
+    if (s.p.sink) {
+      const int2 sl = s.sink_local(kh);
+      sink = min(sl.x, n);
+      from = n - min(sl.y, n);
+    }
+    const int end = (n + 15) >> 4;
+    head = (sink + 15) >> 4;
+    tail = from == n ? end : max(head, from >> 4);
+    units = head + end - tail;
+  }
   __device__ __forceinline__ int unit(int u) const { return u < head ? u : u - head + tail; }
   // Which of the 16 positions of aligned unit `x` are attended.
   __device__ __forceinline__ uint32_t mask(int x) const {
@@ -241,30 +287,27 @@ struct Span {
     return below(n - p0) & (below(sink - p0) | ~below(from - p0));
   }
   static __device__ __forceinline__ uint32_t below(int m) { return m >= 16 ? 0xffffu : m <= 0 ? 0u : (1u << m) - 1u; }
+  __device__ __forceinline__ bool sees_last() const { return n > 0 && (sink == n || from < n); }
 };
 
-__device__ __forceinline__ int tokens_of(const DecodeParams& p, int b) {
-  const int len = p.lengths[b];
-  if (len < 0) return 0;
-  const int64_t n = (int64_t)len + (p.k_new ? 1 : 0);
-  return (int)min(n, (int64_t)p.capacity);
-}
-
-__device__ __forceinline__ Span span_of(const DecodeParams& p, int n, int kh) {
-  Span s;
-  s.n = n;
-  s.sink = n;
-  s.from = n;
-  if (p.sink) {
-    s.sink = (int)min(max(p.sink[kh], (int64_t)0), (int64_t)n);
-    s.from = n - (int)min(max(p.local[kh], (int64_t)0), (int64_t)n);
+// The line in equal parts, one per block.
+struct Cut {
+  int64_t total, each;                      // units of the line; of a part, rounded down
+  int parts, rest;                          // total = each * parts + rest
+  __device__ __forceinline__ Cut(int64_t t, int most) : total(t) {
+    parts = (int)min(max(t / kMinUnits, (int64_t)1), (int64_t)most);
+    each = t / parts;
+    rest = (int)(t - each * parts);
   }
-  const int end = (n + 15) >> 4;
-  s.head = (s.sink + 15) >> 4;
-  s.tail = s.from == n ? end : max(s.head, s.from >> 4);
-  s.units = s.head + end - s.tail;
-  return s;
-}
+  __device__ __forceinline__ int64_t begin(int c) const { return each * c + rest * c / parts; }
+  // The last c with begin(c) <= x.
+  __device__ __forceinline__ int part_of(int64_t x) const {
+    int c = min((int)((float)x / (float)total * parts), parts - 1);
+    while (begin(c) > x) --c;
+    while (c + 1 < parts && begin(c + 1) <= x) ++c;
+    return c;
+  }
+};
 
 // A walk over the items of a block's part [lo, hi) of the line.
 struct Cursor {
@@ -272,27 +315,25 @@ struct Cursor {
   int n;                                    // tokens of sequence b
   Span span;
   int64_t at;                               // where the item begins on the line
-  int units;
   int u0, u1;                               // the units of the item that are in the part
-  __device__ __forceinline__ void enter(const DecodeParams& p, int64_t lo, int64_t hi) {
-    span = span_of(p, n, kh);
-    units = span.units;
-    u0 = (int)min(max(lo - at, (int64_t)0), (int64_t)units);
-    u1 = (int)min(hi - at, (int64_t)units);
+  __device__ __forceinline__ void enter(const Sizes& s, int64_t lo, int64_t hi) {
+    span = Span(s, n, kh);
+    u0 = (int)min(max(lo - at, (int64_t)0), (int64_t)span.units);
+    u1 = (int)min(hi - at, (int64_t)span.units);
   }
   // To the next item; false when it is not in the part.
-  __device__ __forceinline__ bool next(const DecodeParams& p, int64_t lo, int64_t hi) {
-    at += units + kItemCost;
+  __device__ __forceinline__ bool next(const Sizes& s, int64_t lo, int64_t hi) {
+    at += span.units + kItemCost;
     if (at >= hi) return false;
-    if (++tile == p.tiles) {
+    if (++tile == s.p.tiles) {
       tile = 0;
-      if (++kh == p.KV) {
+      if (++kh == s.p.KV) {
         kh = 0;
         ++b;
-        n = tokens_of(p, b);
+        n = s.tokens(b);
       }
     }
-    enter(p, lo, hi);
+    enter(s, lo, hi);
     return true;
   }
 };
@@ -300,7 +341,13 @@ struct Cursor {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // orders this thread's ordinary writes to shared memory before later TMA writes to the same place
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -377,59 +424,253 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_
 // hi + lo of a sum that was split; an infinity of hi is the result (its lo is inf - inf or 0 * inf).
 __device__ __forceinline__ float joined(float hi, float lo) { return isinf(hi) ? hi : hi + lo; }
 
-template <typename T>
-__device__ __forceinline__ float2 load_table2(const Pool& p, const void* t, int64_t off) {
-  if (p.rope_f32) return *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(t) + off);
-  return Cvt<T>::unpack(*reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(t) + off));
-}
-
 // A unit's keys (and values) are D/64 panels of 16 rows of 128 bytes, 16-byte chunk c of row r at c ^ (r % 8): TMA's
 // 128-byte swizzle, which ldmatrix reads without bank conflicts.
-template <int D>
+template <int D, int MT>
 struct Layout {
   static constexpr int kPanelBytes = kUnit * 128, kTileBytes = kUnit * D * 2, kStageBytes = 2 * kTileBytes;
-  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kStages = D == 128 ? 2 : 4;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kPitch = D + 4;                                 // floats per head in the join buffer
-  static constexpr int kJoinBytes = kWarps * 8 * kPitch * 4;
+  static constexpr int kJoinBytes = kWarps * 8 * D * 4;                // a head's row: value d at d ^ 4 * head
+  // what an item needs: queries (rows padded by 16 bytes), the new token's key, value, cos and sin, its page
+  static constexpr int kQPitch = D * 2 + 16, kKey = 8 * MT * kQPitch, kValue = kKey + D * 2, kCos = kValue + D * 2,
+                       kSin = kCos + D * 4, kPage = kSin + D * 4, kItemBytes = kPage + 16;
   static constexpr int kBarBytes = kWarps * kStages * 8, kMaskBytes = kWarps * kStages * 4;
-  static constexpr int kBytes = 1024 + kRing + kJoinBytes + kBarBytes + kMaskBytes + 2 * kWarps * 8 * 4 + 128;
-  static_assert(kBytes <= 232448, "shared memory");
+  static constexpr int kBytes = 1024 + kRing + kJoinBytes + 2 * kItemBytes + kBarBytes + kMaskBytes + 2 * kWarps * 8 * 4 + 128 +
+                                kCached * 12;
+  static_assert(kPerSm * (kBytes + 1024) <= 233472, "shared memory");
   static __device__ __forceinline__ uint32_t at(int row, int chunk) {
     return (chunk >> 3) * kPanelBytes + row * 128 + (((chunk ^ row) & 7) << 4);
   }
 };
 
+// What follows up to the kernel runs once or twice per item and stays out of the loop's registers.
+
+// Four coordinates of head h's result: sum of values over sum of weights (zeros where there is no weight).
+template <typename T>
+__device__ __forceinline__ void store_out4(const DecodeParams& p, int b, int h, int d, float4 O, float sum) {
+  const int64_t off = (int64_t)b * p.o_sb + (int64_t)h * p.o_sh + d;
+  if (sum == 0.f) O = make_float4(0.f, 0.f, 0.f, 0.f);
+  else O = make_float4(O.x / sum, O.y / sum, O.z / sum, O.w / sum);
+  if (p.out_f32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + off) = O;
+  else *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + off) = make_uint2(Cvt<T>::pack(O.x, O.y), Cvt<T>::pack(O.z, O.w));
+}
+
+// Fetches what an item needs into its buffer, with cp.async; called by the whole block.
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k,
-                                                                        const __grid_constant__ CUtensorMap map_v,
-                                                                        const __grid_constant__ DecodeParams p) {
-  using L = Layout<D>;
+__device__ __forceinline__ void fetch_item(const DecodeParams& p, const Cursor& c, bool fresh, uint32_t buf) {
+  using L = Layout<D, MT>;
+  constexpr int CPR = D / 8;                       // 16-byte chunks per row
+  const int tid = threadIdx.x;
+  const int h0 = c.kh * p.G + c.tile * 8 * MT, heads = min(p.G - c.tile * 8 * MT, 8 * MT);
+#pragma unroll
+  for (int i = tid; i < 8 * MT * CPR; i += kDecodeThreads) {
+    const int row = i / CPR, chunk = i % CPR;
+    const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)c.b * p.q_sb + (int64_t)(h0 + min(row, heads - 1)) * p.q_sh;
+    cp_async16(buf + row * L::kQPitch + chunk * 16, src + chunk * 8, row < heads);
+  }
+  if (fresh) {
+    const int64_t pos = c.n - 1;
+    if (tid < 2 * CPR) {
+      const int chunk = tid % CPR;
+      const T* src = tid < CPR ? reinterpret_cast<const T*>(p.k_new) + c.b * p.k_sb + c.kh * p.k_sh
+                               : reinterpret_cast<const T*>(p.v_new) + c.b * p.v_sb + c.kh * p.v_sh;
+      cp_async16(buf + (tid < CPR ? L::kKey : L::kValue) + chunk * 16, src + chunk * 8, true);
+    }
+    const int64_t row = p.pool.cos ? rope_row(p.pool, c.b, 0, pos) : -1;
+    const int cells = p.pool.rope_f32 ? 4 : 2, chunks = D * cells / 16;      // bytes of a table's value
+    if (row >= 0 && tid >= kDecodeThreads - 2 * chunks) {
+      const int i = tid - (kDecodeThreads - 2 * chunks), chunk = i % chunks;
+      const char* src = reinterpret_cast<const char*>(i < chunks ? p.pool.cos : p.pool.sin) + row * cells;
+      cp_async16(buf + (i < chunks ? L::kCos : L::kSin) + chunk * 16, src + chunk * 16, true);
+    }
+    if (tid == 0) cp_async4(buf + L::kPage, p.pool.table + (int64_t)c.b * p.pool.table_stride + (pos >> p.pool.shift));
+  }
+  cp_async_commit();
+}
+
+// Two neighbouring values of a table row in shared memory.
+template <typename T>
+__device__ __forceinline__ float2 table2(const unsigned char* row, int d, bool f32) {
+  if (f32) return *reinterpret_cast<const float2*>(row + d * 4);
+  return Cvt<T>::unpack(*reinterpret_cast<const uint32_t*>(row + d * 2));
+}
+
+// The new token's key is rotated in its buffer (a warp's work) and stored, with its value, into its page.
+template <typename T, int D, int MT>
+__device__ __noinline__ void place_new(const DecodeParams& p, unsigned char* item, int kh, int slot, int page, bool store) {
+  using L = Layout<D, MT>;
+  const int lane = threadIdx.x & 31;
+  T* key = reinterpret_cast<T*>(item + L::kKey);
+  const T* value = reinterpret_cast<const T*>(item + L::kValue);
+  if (lane < D / 4) {                              // a pair of coordinates of either half
+#pragma unroll
+    for (int d = lane * 2; d < D / 2; d += 64) {
+      uint32_t* lo = reinterpret_cast<uint32_t*>(key + d);
+      uint32_t* hi = reinterpret_cast<uint32_t*>(key + d + D / 2);
+      if (p.pool.cos) {
+        const bool f32 = p.pool.rope_f32;
+        const float2 a = Cvt<T>::unpack(*lo), b = Cvt<T>::unpack(*hi);
+        const float2 cl = table2<T>(item + L::kCos, d, f32), ch = table2<T>(item + L::kCos, d + D / 2, f32);
+        const float2 sl = table2<T>(item + L::kSin, d, f32), sh = table2<T>(item + L::kSin, d + D / 2, f32);
+        *lo = Cvt<T>::pack(fmaf(a.x, cl.x, -b.x * sl.x), fmaf(a.y, cl.y, -b.y * sl.y));
+        *hi = Cvt<T>::pack(fmaf(b.x, ch.x, a.x * sh.x), fmaf(b.y, ch.y, a.y * sh.y));
+      }
+    }
+  }
+  __syncwarp();
+  if (store && lane < D / 8) {
+    T* kd = reinterpret_cast<T*>(p.pool.k) + page * p.pool.k_page + kh * p.pool.k_head + slot * p.pool.k_slot + lane * 8;
+    T* vd = reinterpret_cast<T*>(p.pool.v) + page * p.pool.v_page + kh * p.pool.v_head + slot * p.pool.v_slot + lane * 8;
+    *reinterpret_cast<uint4*>(kd) = *reinterpret_cast<const uint4*>(key + lane * 8);
+    *reinterpret_cast<uint4*>(vd) = *reinterpret_cast<const uint4*>(value + lane * 8);
+  }
+}
+
+// The rows of aligned unit x one by one, with cp.async, and zeros where nothing is attended.  `page`: of the unit, or of
+// position lane % 16 when pages are smaller.  Returns `present` without the rows that have no page.  Called by a
+// whole warp.
+template <typename T, int D, int MT>
+__device__ __noinline__ uint32_t load_rows(const DecodeParams& p, int b, int kh, int x, int32_t page, uint32_t present,
+                                           uint32_t dst) {
+  using L = Layout<D, MT>;
+  constexpr int LPR = D / 8, RPI = 32 / LPR;       // lanes per row, rows per load instruction
+  const int lane = threadIdx.x & 31;
+  const int pos = x * 16 + (lane & 15);
+  bool take = (present >> (lane & 15)) & 1;
+  if (take && (uint32_t)page >= (uint32_t)p.pool.num_pages) {
+    if (lane < 16) report(kStatusAttend, b, pos, kh);
+    take = false;
+  }
+  const T* ks = reinterpret_cast<const T*>(p.pool.k);
+  const T* vs = reinterpret_cast<const T*>(p.pool.v);
+  if (take) {
+    const int64_t slot = pos & ((1ll << p.pool.shift) - 1);
+    ks += page * p.pool.k_page + kh * p.pool.k_head + slot * p.pool.k_slot;
+    vs += page * p.pool.v_page + kh * p.pool.v_head + slot * p.pool.v_slot;
+  }
+  present = __ballot_sync(0xffffffffu, take) & 0xffffu;
+#pragma unroll 2
+  for (int i = 0; i < kUnit / RPI; ++i) {
+    const int row = i * RPI + lane / LPR, chunk = lane % LPR;
+    const T* k_row = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ks), row));
+    const T* v_row = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(vs), row));
+    cp_async16(dst + L::at(row, chunk), k_row + chunk * 8, (present >> row) & 1);
+    cp_async16(dst + L::kTileBytes + L::at(row, chunk), v_row + chunk * 8, (present >> row) & 1);
+  }
+  __syncwarp();
+  return present;
+}
+
+// Joins the records that parts c0 .. c1 of the line left of one item (`heads` query heads from h0 of sequence b);
+// called by every block that left one.  kJoin neighbours are joined by the last of them, their results by the last
+// of those that joined, and so on; no block waits.
+template <typename T, int D>
+__device__ __noinline__ void join_parts(const DecodeParams& p, int c0, int c1, int b, int h0, int heads, float* scratch,
+                                        int* flag) {
+  const int tid = threadIdx.x;
+  float* wm = scratch;                             // (record, head): maximum and sum
+  float* wl = scratch + kJoin * kRecHeads;
+  auto record_of = [&](int i) { return p.records + (int64_t)(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * kRecFloats; };
+  // at each level groups of kJoin neighbours; `step` parts lie behind one of them
+  int index = (int)blockIdx.x - c0, there = c1 - c0 + 1, step = 1;
+  for (int level = 0;; ++level) {
+    const int group = index / kJoin, first = group * kJoin * step, count = min(there - group * kJoin, kJoin);
+    // counters of a part: of the item that begins in it 0 and 1 by level, of the one that began before 2
+    int* counter = p.counters + kCounters * (c0 + first) + (group == 0 ? level : 2);
+    const bool final = there <= kJoin;
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      *flag = atomicAdd(counter, 1) == count - 1;
+      if (*flag) *counter = 0;
+    }
+    __syncthreads();
+    if (!*flag) return;
+    __threadfence();
+    for (int k = tid; k < kJoin * kRecHeads; k += kDecodeThreads) {
+      const int i = k / kRecHeads, head = k % kRecHeads;
+      if (i < count && head < heads) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(record_of(first + i * step) + kRecHeads * 128 + head * 2));
+        wm[k] = ml.x;
+        wl[k] = ml.y;
+      }
+    }
+    __syncthreads();
+    float* to = record_of(first);
+    for (int i4 = tid; i4 < heads * D / 4; i4 += kDecodeThreads) {
+      const int head = i4 * 4 / D, d = i4 * 4 % D;
+      float4 x[kJoin];
+#pragma unroll
+      for (int i = 0; i < kJoin; ++i)
+        if (i < count) x[i] = __ldcg(reinterpret_cast<const float4*>(record_of(first + i * step) + i4 * 4));
+      float M = -INFINITY, Ls = 0.f;
+      for (int i = 0; i < count; ++i) M = fmaxf(M, wm[i * kRecHeads + head]);
+      const float base = M == -INFINITY ? 0.f : M;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kJoin; ++i)
+        if (i < count) {
+          const float f = exp2f(wm[i * kRecHeads + head] - base);
+          Ls += f * wl[i * kRecHeads + head];
+          O.x += f * x[i].x; O.y += f * x[i].y; O.z += f * x[i].z; O.w += f * x[i].w;
+        }
+      if (final) {
+        store_out4<T>(p, b, h0 + head, d, O, Ls);
+      } else {
+        // (each element of the group's first record is read by the thread that writes it)
+        *reinterpret_cast<float4*>(to + i4 * 4) = O;
+        if (d == 0) *reinterpret_cast<float2*>(to + kRecHeads * 128 + head * 2) = make_float2(M, Ls);
+      }
+    }
+    if (final) return;
+    index = group;
+    there = (there + kJoin - 1) / kJoin;
+    step *= kJoin;
+  }
+}
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                              const __grid_constant__ CUtensorMap map_v,
+                                                                              const __grid_constant__ DecodeParams p) {
+  using L = Layout<D, MT>;
   constexpr int kStages = L::kStages;
-  constexpr int LPR = D / 8, RPI = 32 / LPR;      // lanes per row, rows per load instruction
-  constexpr int KS = D / 16;                      // k steps of the first product, pairs of n tiles of the second
-  extern __shared__ unsigned char smem_raw[];
+  constexpr int KS = D / 16;                       // k steps of the first product, pairs of n tiles of the second
+  extern __shared__ unsigned char smem_raw[];      // the swizzle goes by the address: panels start at multiples of 1024
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* sm_o = reinterpret_cast<float*>(smem + L::kRing);
-  unsigned char* sm_bar = smem + L::kRing + L::kJoinBytes;
+  unsigned char* sm_item = smem + L::kRing + L::kJoinBytes;
+  unsigned char* sm_bar = sm_item + 2 * L::kItemBytes;
   uint32_t* sm_mask = reinterpret_cast<uint32_t*>(sm_bar + L::kBarBytes);
   float* sm_m = reinterpret_cast<float*>(sm_mask + kWarps * kStages);
   float* sm_l = sm_m + kWarps * 8;
-  int64_t* sm_scan = reinterpret_cast<int64_t*>(sm_l + kWarps * 8);   // 8 warp sums, then {b, item of b, at} of the part
+  int64_t* sm_scan = reinterpret_cast<int64_t*>(sm_l + kWarps * 8);   // warp sums, then {b, item of b, at} of the part
   int* sm_flag = reinterpret_cast<int*>(sm_scan + 12);
+  int* sm_len = reinterpret_cast<int*>(sm_scan + 16);
+  int2* sm_span = reinterpret_cast<int2*>(sm_len + kCached);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int items_per_seq = p.KV * p.tiles;
-  const int64_t slot_mask = (1ll << p.pool.shift) - 1;
+  const Sizes sizes = {p, sm_len, sm_span};
 
-  // ---- the line: total length, and where this block's part begins
+  // ---- the line: its length, and where this block's part begins
+  for (int b = tid; b < min(p.B, kCached); b += kDecodeThreads) sm_len[b] = p.lengths[b];
+  if (p.sink)
+    for (int kh = tid; kh < min(p.KV, kCached); kh += kDecodeThreads) sm_span[kh] = Sizes::clamped(p.sink[kh], p.local[kh]);
+  const uint32_t bars = (uint32_t)__cvta_generic_to_shared(sm_bar) + warp * kStages * 8;
+  if (lane < kStages) {
+    bar_init(bars + lane * 8);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
   const int per = (p.B + kDecodeThreads - 1) / kDecodeThreads;
   const int b_lo = min(tid * per, p.B), b_hi = min(b_lo + per, p.B);
   auto cost_of = [&](int b) {
-    const int n = tokens_of(p, b);
-    if (!p.sink) return (int64_t)items_per_seq * (((n + 15) >> 4) + kItemCost);
+    const int n = sizes.tokens(b);
+    if (!p.sink) return (int64_t)p.KV * p.tiles * (((n + 15) >> 4) + kItemCost);
     int64_t sum = 0;
-    for (int kh = 0; kh < p.KV; ++kh) sum += span_of(p, n, kh).units + kItemCost;
+#pragma unroll 4
+    for (int kh = 0; kh < p.KV; ++kh) sum += Span(sizes, n, kh).units + kItemCost;
     return sum * p.tiles;
   };
   int64_t mine = 0;
@@ -449,35 +690,40 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
     if (w < warp) before += sm_scan[w];
     total += sm_scan[w];
   }
-  const int64_t blocks = min(max(total / kMinUnits, (int64_t)1), (int64_t)gridDim.x);
-  const int64_t block = blockIdx.x;
-  const int64_t lo = block * total / blocks, hi = (block + 1) * total / blocks;
-  const bool busy = block < blocks && lo < hi;
+  const Cut cut(total, gridDim.x);
+  const int block = blockIdx.x;
 
-  if (busy) {
-    if (before <= lo && lo < before + mine) {     // one thread: the part begins among its sequences
+  if (block < cut.parts) {
+    const int64_t lo = cut.begin(block), hi = cut.begin(block + 1);
+    if (before <= lo && lo < before + mine) {      // one thread: the part begins among its sequences
       int64_t at = before;
       int b = b_lo;
       for (int64_t c; lo >= at + (c = cost_of(b)); ++b) at += c;
-      const int n = tokens_of(p, b);
-      int item = 0;
-      for (;; ++item) {
-        const int64_t c = span_of(p, n, item / p.tiles).units + kItemCost;
+      const int n = sizes.tokens(b);
+      int kh = 0, tile = 0;
+      for (;;) {
+        const int c = Span(sizes, n, kh).units + kItemCost;
         if (lo < at + c) break;
         at += c;
+        if (++tile == p.tiles) {
+          tile = 0;
+          ++kh;
+        }
       }
       sm_scan[8] = b;
-      sm_scan[9] = item;
+      sm_scan[9] = (int64_t)kh << 32 | tile;
       sm_scan[10] = at;
     }
     __syncthreads();
     Cursor cur;
     cur.b = (int)sm_scan[8];
-    cur.kh = (int)sm_scan[9] / p.tiles;
-    cur.tile = (int)sm_scan[9] % p.tiles;
+    cur.kh = (int)(sm_scan[9] >> 32);
+    cur.tile = (int)sm_scan[9];
     cur.at = sm_scan[10];
-    cur.n = tokens_of(p, cur.b);
-    cur.enter(p, lo, hi);
+    cur.n = sizes.tokens(cur.b);
+    cur.enter(sizes, lo, hi);
+    const uint32_t item_at = (uint32_t)__cvta_generic_to_shared(sm_item);
+    fetch_item<T, D, MT>(p, cur, sizes.fresh(cur.b), item_at);
 
     // ---- loads: a cursor of this warp's own
     Cursor ld = cur;
@@ -486,15 +732,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
     int ld_x = 0;                                  // aligned unit that is loaded next, its attended positions and its page
     uint32_t ld_mask = 0;                          // (of position lane % 16 when pages are smaller than a unit)
     int32_t ld_page = -1;
-    bool ld_new_here = false;                      // sequence ld.b gets a new token at position ld.n - 1
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * kStages * L::kStageBytes;
     uint32_t* my_mask = sm_mask + warp * kStages;
-    const uint32_t bars = (uint32_t)__cvta_generic_to_shared(sm_bar) + warp * kStages * 8;
-    if (lane < kStages) {
-      bar_init(bars + lane * 8);
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncwarp();
 
     auto ld_look = [&]() {                         // look up the next unit's page
       ld_x = ld.span.unit(ld_u);
@@ -506,99 +745,25 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
         const int pos = ld_x * 16 + (lane & 15);
         ld_page = (ld_mask >> (lane & 15)) & 1 ? row[pos >> p.pool.shift] : -1;
       }
+      if (ld_x == (ld.n - 1) >> 4 && sizes.fresh(ld.b)) ld_mask &= ~(1u << ((ld.n - 1) & 15));    // the new token is in no page
     };
     auto ld_seek = [&]() {                         // to the next unit of this warp
       while (ld_u >= ld.u1) {
-        if (!ld.next(p, lo, hi)) {
+        if (!ld.next(sizes, lo, hi)) {
           ld_more = false;
           return;
         }
         ld_u = ld.u0 + warp;
-        ld_new_here = p.k_new && ld.n == (int64_t)p.lengths[ld.b] + 1;
       }
       ld_look();
     };
-
-    // The new token's row of (b, kh): rotated and rounded, into shared memory (stage address and row, row < 0:
-    // not there) and, `store`, into its page.  Called by a whole warp.  False when it has no place.
-    auto new_row = [&](int b, int kh, int n, uint32_t stage_addr, int row, bool store) {
-      const int64_t pos = n - 1;
-      const int64_t rope = p.pool.cos ? rope_row(p.pool, b, 0, pos) : 0;
-      const int32_t page = page_of(p.pool, p.pool.table + (int64_t)b * p.pool.table_stride, pos);
-      const bool placed = rope >= 0 && page >= 0;
-      if (!placed && lane == 0) report(rope < 0 ? kStatusRope : kStatusAppend, b, pos, kh);
-      if (lane < D / 16) {
-        uint4 x[4];                                // key and value, lower and upper half; zeros without a place
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = make_uint4(0, 0, 0, 0);
-        if (placed) {
-          const T* ks = reinterpret_cast<const T*>(p.k_new) + b * p.k_sb + kh * p.k_sh + lane * 8;
-          const T* vs = reinterpret_cast<const T*>(p.v_new) + b * p.v_sb + kh * p.v_sh + lane * 8;
-          x[0] = *reinterpret_cast<const uint4*>(ks);
-          x[1] = *reinterpret_cast<const uint4*>(ks + D / 2);
-          x[2] = *reinterpret_cast<const uint4*>(vs);
-          x[3] = *reinterpret_cast<const uint4*>(vs + D / 2);
-          if (p.pool.cos) rotate_pair<T, D>(p.pool, rope, lane, x[0], x[1]);
-        }
-        if (placed && store) {
-          const int64_t slot = pos & slot_mask;
-          T* kd = reinterpret_cast<T*>(p.pool.k) + page * p.pool.k_page + kh * p.pool.k_head + slot * p.pool.k_slot + lane * 8;
-          T* vd = reinterpret_cast<T*>(p.pool.v) + page * p.pool.v_page + kh * p.pool.v_head + slot * p.pool.v_slot + lane * 8;
-          *reinterpret_cast<uint4*>(kd) = x[0];
-          *reinterpret_cast<uint4*>(kd + D / 2) = x[1];
-          *reinterpret_cast<uint4*>(vd) = x[2];
-          *reinterpret_cast<uint4*>(vd + D / 2) = x[3];
-        }
-        if (row >= 0) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int chunk = lane + (i & 1) * (D / 16);
-            const uint32_t a = stage_addr + (i >> 1) * L::kTileBytes + L::at(row, chunk);
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x[i].x), "r"(x[i].y), "r"(x[i].z), "r"(x[i].w) : "memory");
-          }
-        }
-      }
-      return placed;
-    };
-
-    // The rows of a unit one by one: zeros where nothing is attended, nothing in place of the new token's.  `present` loses
-    // the rows without a page.
-    auto ld_rows = [&](uint32_t dst, uint32_t& present, uint32_t fresh) {
-      const int pos = ld_x * 16 + (lane & 15);
-      bool take = (present >> (lane & 15)) & 1;
-      if (take && (uint32_t)ld_page >= (uint32_t)p.pool.num_pages) {
-        if (lane < 16) report(kStatusAttend, ld.b, pos, ld.kh);
-        take = false;
-      }
-      const T* ks = reinterpret_cast<const T*>(p.pool.k);
-      const T* vs = reinterpret_cast<const T*>(p.pool.v);
-      if (take) {
-        ks += ld_page * p.pool.k_page + ld.kh * p.pool.k_head + (pos & slot_mask) * p.pool.k_slot;
-        vs += ld_page * p.pool.v_page + ld.kh * p.pool.v_head + (pos & slot_mask) * p.pool.v_slot;
-      }
-      present = __ballot_sync(0xffffffffu, take) & 0xffffu;
-#pragma unroll 2
-      for (int i = 0; i < kUnit / RPI; ++i) {
-        const int row = i * RPI + lane / LPR, chunk = lane % LPR;
-        const T* k_row = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ks), row));
-        const T* v_row = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(vs), row));
-        if ((fresh >> row) & 1) continue;
-        cp_async16(dst + L::at(row, chunk), k_row + chunk * 8, (present >> row) & 1);
-        cp_async16(dst + L::kTileBytes + L::at(row, chunk), v_row + chunk * 8, (present >> row) & 1);
-      }
-      __syncwarp();
-    };
-
     auto ld_issue = [&](int stage) {
       if (ld_more) {
-        const uint32_t dst = ring + stage * L::kStageBytes;
-        const uint32_t fresh = ld_new_here && ld_x == (ld.n - 1) >> 4 ? ld_mask & (1u << ((ld.n - 1) & 15)) : 0u;
-        uint32_t present = ld_mask & ~fresh;
-        if (present == 0xffffu && p.tma && (uint32_t)ld_page < (uint32_t)p.pool.num_pages) {
+        const uint32_t dst = ring + stage * L::kStageBytes, bar = bars + stage * 8;
+        if (ld_mask == 0xffffu && p.tma && (uint32_t)ld_page < (uint32_t)p.pool.num_pages) {
           if (lane == 0) {
-            const int slot = (ld_x << 4) & (int)slot_mask;
-            const uint32_t bar = bars + stage * 8;
-            my_mask[stage] = 0xffffu;          // seen by the other lanes when they have waited on the barrier
+            const int slot = (ld_x << 4) & ((1 << p.pool.shift) - 1);
+            my_mask[stage] = 0xffffu;              // seen by the other lanes when they have waited on the barrier
             bar_expect(bar, L::kStageBytes);
 #pragma unroll
             for (int i = 0; i < D / 64; ++i) tma_load(dst + i * L::kPanelBytes, &map_k, bar, i * 64, slot, ld.kh, ld_page);
@@ -606,295 +771,269 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) paged_decode_kernel(const _
             for (int i = 0; i < D / 64; ++i) tma_load(dst + L::kTileBytes + i * L::kPanelBytes, &map_v, bar, i * 64, slot, ld.kh, ld_page);
           }
         } else {
-          ld_rows(dst, present, fresh);
-          if (fresh && new_row(ld.b, ld.kh, ld.n, dst, (ld.n - 1) & 15, ld.tile == 0)) present |= fresh;
+          const uint32_t present = load_rows<T, D, MT>(p, ld.b, ld.kh, ld_x, ld_page, ld_mask, dst);
           if (lane == 0) {
             my_mask[stage] = present | kByHand;
-            bar_arrive(bars + stage * 8);
+            bar_arrive(bar);
           }
         }
         ld_u += kWarps;
         if (ld_u < ld.u1) ld_look();
         else ld_seek();
       }
+      cp_async_commit();                           // a group per call, empty or not: they are counted
     };
 
-    ld_new_here = p.k_new && ld.n == (int64_t)p.lengths[ld.b] + 1;
     ld_seek();
 #pragma unroll 1
     for (int s = 0; s < kStages; ++s) ld_issue(s);
 
     // ---- items
     const int g = lane >> 2, t = lane & 3;         // row (query head of a tile) and column pair of a fragment
-    int stage = 0;
+    int stage = 0, buf = 0;
     uint32_t parity = 0;
     bool waiting = true;                           // until a wait runs out
-    do {
-      const int heads0 = cur.tile * 8 * MT;        // first query head of the tile within its key head's group
-      const int heads = min(p.G - heads0, 8 * MT);
-      const bool owner = cur.at >= lo;             // the item begins in this part
-      const bool with_new = p.k_new && cur.n > 0 && cur.n == (int64_t)p.lengths[cur.b] + 1;
-      if (owner && warp == 0) {
-        if (with_new && cur.tile == 0 && cur.n > cur.span.sink && cur.span.from == cur.n)
-          new_row(cur.b, cur.kh, cur.n, 0, -1, true);     // stored although the span does not reach it
-        if (lane == 0 && cur.kh == 0 && cur.tile == 0 && p.lengths[cur.b] >= 0 &&
-            (int64_t)p.lengths[cur.b] + (p.k_new ? 1 : 0) > p.capacity)
-          report(kStatusLength, cur.b, (int64_t)p.lengths[cur.b] + (p.k_new ? 1 : 0), 0);
-      }
-      // four coordinates of a head's result, sum of values over sum of weights (zeros where there is no weight)
-      auto store_out4 = [&](int head, int d, float4 O, float sum) {
-        const int64_t off = (int64_t)cur.b * p.o_sb + (int64_t)(cur.kh * p.G + heads0 + head) * p.o_sh + d;
-        if (sum == 0.f) O = make_float4(0.f, 0.f, 0.f, 0.f);
-        else O = make_float4(O.x / sum, O.y / sum, O.z / sum, O.w / sum);
-        if (p.out_f32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + off) = O;
-        else *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + off) = make_uint2(Cvt<T>::pack(O.x, O.y), Cvt<T>::pack(O.z, O.w));
-      };
-      if (cur.units == 0) {                        // nothing to attend (only its owner gets here)
-        for (int i = tid * 4; i < heads * D; i += kDecodeThreads * 4) store_out4(i / D, i % D, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
-        continue;
-      }
-      if (cur.u0 >= cur.u1) continue;              // only the item's cost lies in this part
+    for (bool more = true; more; buf ^= 1) {
+      Cursor next = cur;
+      more = next.next(sizes, lo, hi);
+      cp_async_wait_all();                         // the item's own data; its buffers were fetched an item ago
+      __syncthreads();                             // (and the item before is through with the join buffer)
+      if (more) fetch_item<T, D, MT>(p, next, sizes.fresh(next.b), item_at + (buf ^ 1) * L::kItemBytes);
 
-      float m[MT], l[MT], acc[MT][D / 8][4];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        m[mt] = -INFINITY;
-        l[mt] = 0.f;
-#pragma unroll
-        for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[mt][j][e] = 0.f;
+      unsigned char* item = sm_item + buf * L::kItemBytes;
+      const int h0 = cur.kh * p.G + cur.tile * 8 * MT;                   // first query head of the item
+      const int heads = min(p.G - cur.tile * 8 * MT, 8 * MT);
+      const int units = cur.span.units;
+      const bool owner = cur.at >= lo;             // the item begins in this part
+      const bool ends = units == 0 ? owner : cur.u0 < cur.u1 && cur.u1 == units;
+      const bool fresh = sizes.fresh(cur.b);
+      const bool turn = fresh && p.pool.cos && rope_row(p.pool, cur.b, 0, cur.n - 1) >= 0;
+      bool with_new = false;                       // this block attends the new token
+      if (fresh && ends) {
+        const int page = *reinterpret_cast<const int*>(item + L::kPage);
+        const bool placed = (uint32_t)page < (uint32_t)p.pool.num_pages && (turn || !p.pool.cos);
+        with_new = placed && cur.span.sees_last();
+        if (warp == 0) {
+          if (placed) place_new<T, D, MT>(p, item, cur.kh, (cur.n - 1) & ((1 << p.pool.shift) - 1), page, cur.tile == 0);
+          else if (lane == 0) report(p.pool.cos && !turn ? kStatusRope : kStatusAppend, cur.b, cur.n - 1, cur.kh);
+        }
       }
-      if (cur.u0 + warp < cur.u1) {
-        // query fragments: rows 0-7 the heads, rows 8-15 what a rotated query has beyond 16 bits
-        uint32_t qa[MT][KS][4];
-        const int64_t rope = with_new && p.pool.cos ? rope_row(p.pool, cur.b, 0, cur.n - 1) : -1;
-        const bool split = rope >= 0;
+      if (owner && cur.kh == 0 && cur.tile == 0 && tid == 0) {
+        const int64_t wanted = (int64_t)sizes.length(cur.b) + (p.k_new ? 1 : 0);
+        if (wanted > p.capacity) report(kStatusLength, cur.b, wanted, 0);
+      }
+
+      if (units == 0) {                            // nothing to attend (a part's first item may not be its own)
+        if (owner)
+          for (int i = tid * 4; i < heads * D; i += kDecodeThreads * 4)
+            store_out4<T>(p, cur.b, h0 + i / D, i % D, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
+      } else if (cur.u0 < cur.u1) {
+        float m[MT], l[MT], acc[MT][D / 8][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          const int head = mt * 8 + g;
-          const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)cur.b * p.q_sb + (int64_t)(cur.kh * p.G + heads0 + head) * p.q_sh + 2 * t;
+          m[mt] = -INFINITY;
+          l[mt] = 0.f;
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            qa[mt][ks][0] = head < heads ? *reinterpret_cast<const uint32_t*>(q + ks * 16) : 0u;
-            qa[mt][ks][2] = head < heads ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8) : 0u;
-            qa[mt][ks][1] = qa[mt][ks][3] = 0u;
-          }
-          if (split) {
+          for (int j = 0; j < D / 8; ++j)
 #pragma unroll
-            for (int ks = 0; ks < KS / 2; ++ks)
-#pragma unroll
-              for (int e = 0; e < 4; e += 2) {
-                const int d = ks * 16 + e * 4 + 2 * t;
-                const float2 cl = load_table2<T>(p.pool, p.pool.cos, rope + d), ch = load_table2<T>(p.pool, p.pool.cos, rope + d + D / 2);
-                const float2 sl = load_table2<T>(p.pool, p.pool.sin, rope + d), sh = load_table2<T>(p.pool, p.pool.sin, rope + d + D / 2);
-                const float2 a = Cvt<T>::unpack(qa[mt][ks][e]), b = Cvt<T>::unpack(qa[mt][ks + KS / 2][e]);
-                split2<T, true>(fmaf(a.x, cl.x, -b.x * sl.x), fmaf(a.y, cl.y, -b.y * sl.y), qa[mt][ks][e], qa[mt][ks][e + 1]);
-                split2<T, true>(fmaf(b.x, ch.x, a.x * sh.x), fmaf(b.y, ch.y, a.y * sh.y), qa[mt][ks + KS / 2][e], qa[mt][ks + KS / 2][e + 1]);
-              }
-          }
+            for (int e = 0; e < 4; ++e) acc[mt][j][e] = 0.f;
         }
-        // ldmatrix addresses within a tile: four chunk pairs of a panel, the other panel behind them
-        const int mi = lane >> 3, r8 = lane & 7;
-        const uint32_t k_at = ((mi >> 1) * 8 + r8) * 128 + (((mi & 1) ^ r8) << 4);
-        const uint32_t v_at = L::kTileBytes + ((mi & 1) * 8 + r8) * 128 + (((mi >> 1) ^ r8) << 4);
-#pragma unroll 1
-        for (int u = cur.u0 + warp; u < cur.u1; u += kWarps) {
-          if (waiting) waiting = __all_sync(0xffffffffu, bar_wait(bars + stage * 8, parity));
-          const uint32_t base = ring + stage * L::kStageBytes;
-          const uint32_t present = my_mask[stage];
-          if (present & kByHand) {
-            cp_async_wait_all();
-            __syncwarp();
-          }
-          float sc[MT][2][4];
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[mt][0][e] = sc[mt][1][e] = 0.f;
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            uint32_t kb[4];
-            ldmatrix4(kb, ((base + k_at) ^ ((ks & 3) << 5)) + (ks >> 2) * L::kPanelBytes);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              mma16816<T>(sc[mt][0], qa[mt][ks], kb[0], kb[1]);
-              mma16816<T>(sc[mt][1], qa[mt][ks], kb[2], kb[3]);
-            }
-          }
-          uint32_t pa[MT][4];
+        if (cur.u0 + warp < cur.u1) {
+          // query fragments: rows 0-7 the heads, rows 8-15 what a rotated query has beyond 16 bits
+          uint32_t qa[MT][KS][4];
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            float s[4];
+            const unsigned char* q = item + (mt * 8 + g) * L::kQPitch + 4 * t;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] = sc[mt][e >> 1][e & 1];
-            if (split) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[e] = joined(s[e], sc[mt][e >> 1][(e & 1) + 2]);
+            for (int ks = 0; ks < KS; ++ks) {
+              qa[mt][ks][0] = *reinterpret_cast<const uint32_t*>(q + ks * 32);
+              qa[mt][ks][2] = *reinterpret_cast<const uint32_t*>(q + ks * 32 + 16);
+              qa[mt][ks][1] = qa[mt][ks][3] = 0u;
             }
+            if (turn) {
+              const bool f32 = p.pool.rope_f32;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] *= p.scale_log2;
-            if (present != 0xffffu) {
-              const uint32_t mine16 = present >> (2 * t);
+              for (int ks = 0; ks < KS / 2; ++ks)
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (!((mine16 >> ((e >> 1) * 8 + (e & 1))) & 1)) s[e] = -INFINITY;
+                for (int e = 0; e < 4; e += 2) {
+                  const int d = ks * 16 + e * 4 + 2 * t;
+                  const float2 cl = table2<T>(item + L::kCos, d, f32), ch = table2<T>(item + L::kCos, d + D / 2, f32);
+                  const float2 sl = table2<T>(item + L::kSin, d, f32), sh = table2<T>(item + L::kSin, d + D / 2, f32);
+                  const float2 a = Cvt<T>::unpack(qa[mt][ks][e]), b = Cvt<T>::unpack(qa[mt][ks + KS / 2][e]);
+                  split2<T, true>(fmaf(a.x, cl.x, -b.x * sl.x), fmaf(a.y, cl.y, -b.y * sl.y), qa[mt][ks][e], qa[mt][ks][e + 1]);
+                  split2<T, true>(fmaf(b.x, ch.x, a.x * sh.x), fmaf(b.y, ch.y, a.y * sh.y), qa[mt][ks + KS / 2][e], qa[mt][ks + KS / 2][e + 1]);
+                }
             }
-            float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            if (__any_sync(0xffffffffu, top > m[mt])) {      // a new maximum: what there is so far is scaled down
-              const float m_new = fmaxf(m[mt], top);
-              const float corr = m_new == -INFINITY ? 1.f : exp2f(m[mt] - m_new);
-              m[mt] = m_new;
-              l[mt] *= corr;
-#pragma unroll
-              for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[mt][j][e] *= corr;
-            }
-            const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] = exp2f(s[e] - ref);
-            l[mt] += (s[0] + s[1]) + (s[2] + s[3]);
-            split2<T, false>(s[0], s[1], pa[mt][0], pa[mt][1]);
-            split2<T, false>(s[2], s[3], pa[mt][2], pa[mt][3]);
           }
-#pragma unroll
-          for (int j = 0; j < KS; ++j) {
-            uint32_t vb[4];
-            ldmatrix4_trans(vb, ((base + v_at) ^ ((j & 3) << 5)) + (j >> 2) * L::kPanelBytes);
+          if (with_new && warp == 0) {             // start from the new token: column 0 of a tile of keys, weight 1
+            const uint32_t* key = reinterpret_cast<const uint32_t*>(item + L::kKey);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              mma16816<T>(acc[mt][2 * j], pa[mt], vb[0], vb[1]);
-              mma16816<T>(acc[mt][2 * j + 1], pa[mt], vb[2], vb[3]);
+              float sc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int ks = 0; ks < KS; ++ks)
+                mma16816<T>(sc, qa[mt][ks], g == 0 ? key[ks * 8 + t] : 0u, g == 0 ? key[ks * 8 + 4 + t] : 0u);
+              const float score = (turn ? joined(sc[0], sc[2]) : sc[0]) * p.scale_log2;
+              m[mt] = __shfl_sync(0xffffffffu, score, lane & ~3);
+              // (weights of scores that are no numbers follow the formula: exp(inf - inf) and the like)
+              const float w = m[mt] == -INFINITY ? 0.f : exp2f(m[mt] - m[mt]);
+              l[mt] = t == 0 ? w : 0.f;
+#pragma unroll
+              for (int j = 0; j < D / 8; ++j) {
+                const float2 v = Cvt<T>::unpack(*reinterpret_cast<const uint32_t*>(item + L::kValue + (j * 8 + 2 * t) * 2));
+                acc[mt][j][0] = w * v.x;
+                acc[mt][j][1] = w * v.y;
+              }
+              if (m[mt] != m[mt]) m[mt] = -INFINITY;           // (a maximum passes over NaN)
             }
           }
-          if (present & kByHand) proxy_fence();
-          __syncwarp();
-          ld_issue(stage);
-          if (++stage == kStages) {
-            stage = 0;
-            parity ^= 1;
-          }
-        }
-      }
-
-      // ---- the warps' results joined
-      const bool whole = cur.u0 == 0 && cur.u1 == cur.units;
-      const int nw = min(kWarps, cur.u1 - cur.u0);
-      float* rec = p.records + (2 * block + (owner ? 1 : 0)) * kRecFloats;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const int here = min(heads - mt * 8, 8);
-        if (MT > 1 && here <= 0) break;
-        if (warp < nw) {
-          float sum = l[mt];
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          if (t == 0) {
-            sm_m[warp * 8 + g] = m[mt];
-            sm_l[warp * 8 + g] = sum;
-          }
-          if (g < here) {
-            float* o = sm_o + (warp * 8 + g) * L::kPitch + 2 * t;
-#pragma unroll
-            for (int j = 0; j < D / 8; ++j)
-              *reinterpret_cast<float2*>(o + j * 8) = make_float2(joined(acc[mt][j][0], acc[mt][j][2]), joined(acc[mt][j][1], acc[mt][j][3]));
-          }
-        }
-        __syncthreads();
-        for (int i = tid * 4; i < here * D; i += kDecodeThreads * 4) {
-          const int head = i / D, d = i % D;
-          float M = -INFINITY, Ls = 0.f;
-          for (int w = 0; w < nw; ++w) M = fmaxf(M, sm_m[w * 8 + head]);
-          const float base = M == -INFINITY ? 0.f : M;
-          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int w = 0; w < nw; ++w) {
-            const float f = exp2f(sm_m[w * 8 + head] - base);
-            const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * 8 + head) * L::kPitch + d);
-            Ls += f * sm_l[w * 8 + head];
-            O.x += f * x.x; O.y += f * x.y; O.z += f * x.z; O.w += f * x.w;
-          }
-          if (whole) {
-            store_out4(mt * 8 + head, d, O, Ls);
-          } else {
-            *reinterpret_cast<float4*>(rec + (mt * 8 + head) * D + d) = O;
-            if (d == 0) *reinterpret_cast<float2*>(rec + kRecHeads * 128 + (mt * 8 + head) * 2) = make_float2(M, Ls);
-          }
-        }
-        __syncthreads();
-      }
-      if (whole) continue;
-
-      // ---- the blocks' results joined: kJoin neighbours by the last of them, then their results by the last of those
-      auto block_of = [&](int64_t x) { return ((x + 1) * blocks - 1) / total; };
-      const int64_t c0 = block_of(cur.at);
-      const int parts = (int)(block_of(cur.at + cur.units - 1) - c0) + 1;
-      const int group = (int)(block - c0) / kJoin, groups = (parts + kJoin - 1) / kJoin;
-      auto record_of = [&](int i) { return p.records + (i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * kRecFloats; };
-      bool final = false;
-      for (int level = 0; level < 2; ++level) {
-        const int first = level == 0 ? group * kJoin : 0, step = level == 0 ? 1 : kJoin;
-        const int count = level == 0 ? min(parts - first, kJoin) : groups;
-        int* counter = p.counters + (level == 0 ? 3 * (c0 + first) + (group == 0 ? 0 : 1) : 3 * c0 + 2);
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-          *sm_flag = atomicAdd(counter, 1) == count - 1;
-          if (*sm_flag) *counter = 0;
-        }
-        __syncthreads();
-        if (!*sm_flag) break;
-        __threadfence();
-        final = level == 1 || groups == 1;
-        float* wm = sm_o;                          // (record, head): maximum, then weight; and sum
-        float* wl = sm_o + kJoin * kRecHeads;
-        {
-          const int i = tid / kRecHeads, head = tid % kRecHeads;
-          if (i < count && head < heads) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(record_of(first + i * step) + kRecHeads * 128 + head * 2));
-            wm[tid] = ml.x;
-            wl[tid] = ml.y;
-          }
-        }
-        __syncthreads();
-        float* to = record_of(first);
-        for (int i4 = tid; i4 < heads * D / 4; i4 += kDecodeThreads) {
-          const int head = i4 * 4 / D, d = i4 * 4 % D;
-          float4 x[kJoin];
-#pragma unroll
-          for (int i = 0; i < kJoin; ++i)
-            if (i < count) x[i] = __ldcg(reinterpret_cast<const float4*>(record_of(first + i * step) + i4 * 4));
-          float M = -INFINITY, Ls = 0.f;
-          for (int i = 0; i < count; ++i) M = fmaxf(M, wm[i * kRecHeads + head]);
-          const float base = M == -INFINITY ? 0.f : M;
-          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-          for (int i = 0; i < kJoin; ++i)
-            if (i < count) {
-              const float f = exp2f(wm[i * kRecHeads + head] - base);
-              Ls += f * wl[i * kRecHeads + head];
-              O.x += f * x[i].x; O.y += f * x[i].y; O.z += f * x[i].z; O.w += f * x[i].w;
+          // ldmatrix addresses within a tile: four chunk pairs of a panel, the other panel behind them
+          const int mi = lane >> 3, r8 = lane & 7;
+          const uint32_t k_at = ((mi >> 1) * 8 + r8) * 128 + (((mi & 1) ^ r8) << 4);
+          const uint32_t v_at = L::kTileBytes + ((mi & 1) * 8 + r8) * 128 + (((mi >> 1) ^ r8) << 4);
+#pragma unroll 1
+          for (int u = cur.u0 + warp; u < cur.u1; u += kWarps) {
+            if (waiting) waiting = __all_sync(0xffffffffu, bar_wait(bars + stage * 8, parity));
+            const uint32_t base = ring + stage * L::kStageBytes;
+            const uint32_t present = my_mask[stage];
+            if (present & kByHand) {
+              cp_async_wait<kStages - 1>();        // one group per unit that was asked for after this one may be open
+              __syncwarp();
             }
-          if (final) {
-            store_out4(head, d, O, Ls);
-          } else {
-            // (each element of the group's first record is read by the thread that writes it)
-            *reinterpret_cast<float4*>(to + i4 * 4) = O;
-            if (d == 0) *reinterpret_cast<float2*>(to + kRecHeads * 128 + head * 2) = make_float2(M, Ls);
+            float sc[MT][2][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[mt][0][e] = sc[mt][1][e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+              uint32_t kb[4];
+              ldmatrix4(kb, ((base + k_at) ^ ((ks & 3) << 5)) + (ks >> 2) * L::kPanelBytes);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                mma16816<T>(sc[mt][0], qa[mt][ks], kb[0], kb[1]);
+                mma16816<T>(sc[mt][1], qa[mt][ks], kb[2], kb[3]);
+              }
+            }
+            uint32_t pa[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              float s[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[e] = sc[mt][e >> 1][e & 1];
+              if (turn) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] = joined(s[e], sc[mt][e >> 1][(e & 1) + 2]);
+              }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[e] *= p.scale_log2;
+              if (present != 0xffffu) {
+                const uint32_t mine16 = present >> (2 * t);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (!((mine16 >> ((e >> 1) * 8 + (e & 1))) & 1)) s[e] = -INFINITY;
+              }
+              float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+              if (__any_sync(0xffffffffu, top > m[mt])) {      // a new maximum: what there is so far is scaled down
+                const float m_new = fmaxf(m[mt], top);
+                const float corr = m_new == m[mt] ? 1.f : exp2f(m[mt] - m_new);
+                m[mt] = m_new;
+                l[mt] *= corr;
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) acc[mt][j][e] *= corr;
+              }
+              const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[e] = exp2f(s[e] - ref);
+              l[mt] += (s[0] + s[1]) + (s[2] + s[3]);
+              split2<T, false>(s[0], s[1], pa[mt][0], pa[mt][1]);
+              split2<T, false>(s[2], s[3], pa[mt][2], pa[mt][3]);
+            }
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+              uint32_t vb[4];
+              ldmatrix4_trans(vb, ((base + v_at) ^ ((j & 3) << 5)) + (j >> 2) * L::kPanelBytes);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                mma16816<T>(acc[mt][2 * j], pa[mt], vb[0], vb[1]);
+                mma16816<T>(acc[mt][2 * j + 1], pa[mt], vb[2], vb[3]);
+              }
+            }
+            if (present & kByHand) proxy_fence();
+            __syncwarp();
+            ld_issue(stage);
+            if (++stage == kStages) {
+              stage = 0;
+              parity ^= 1;
+            }
           }
         }
-        if (final) break;
+
+        // ---- the warps' results joined
+        const bool whole = cur.u0 == 0 && cur.u1 == units;
+        const int nw = min(kWarps, cur.u1 - cur.u0);
+        float* rec = p.records + (int64_t)(2 * block + (owner ? 1 : 0)) * kRecFloats;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const int here = min(heads - mt * 8, 8);
+          if (MT > 1 && here <= 0) break;
+          if (mt > 0) __syncthreads();
+          if (warp < nw) {
+            float sum = l[mt];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (t == 0) {
+              sm_m[warp * 8 + g] = m[mt];
+              sm_l[warp * 8 + g] = sum;
+            }
+            if (g < here) {
+              float* o = sm_o + (warp * 8 + g) * D;
+#pragma unroll
+              for (int j = 0; j < D / 8; ++j)
+                *reinterpret_cast<float2*>(o + ((j * 8 + 2 * t) ^ (g << 2))) =
+                    make_float2(joined(acc[mt][j][0], acc[mt][j][2]), joined(acc[mt][j][1], acc[mt][j][3]));
+            }
+          }
+          __syncthreads();
+          for (int i = tid * 4; i < here * D; i += kDecodeThreads * 4) {
+            const int head = i / D, d = i % D;
+            float M = -INFINITY, Ls = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w)
+              if (w < nw) M = fmaxf(M, sm_m[w * 8 + head]);
+            const float base = M == -INFINITY ? 0.f : M;
+            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w)
+              if (w < nw) {
+                const float f = exp2f(sm_m[w * 8 + head] - base);
+                const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * 8 + head) * D + (d ^ (head << 2)));
+                Ls += f * sm_l[w * 8 + head];
+                O.x += f * x.x; O.y += f * x.y; O.z += f * x.z; O.w += f * x.w;
+              }
+            if (whole) {
+              store_out4<T>(p, cur.b, h0 + mt * 8 + head, d, O, Ls);
+            } else {
+              *reinterpret_cast<float4*>(rec + (mt * 8 + head) * D + d) = O;
+              if (d == 0) *reinterpret_cast<float2*>(rec + kRecHeads * 128 + (mt * 8 + head) * 2) = make_float2(M, Ls);
+            }
+          }
+        }
+        if (!whole)
+          join_parts<T, D>(p, cut.part_of(cur.at), cut.part_of(cur.at + units - 1), cur.b, h0, heads, sm_o, sm_flag);
       }
-      __syncthreads();                             // sm_o is free again
-    } while (cur.next(p, lo, hi));
+      if (more) cur = next;
+    }
   }
 
   if (p.advance) {                                 // the last block to get here: every block has read the lengths
     __syncthreads();
     if (tid == 0) {
-      int* done = p.counters + 3 * kMaxBlocks;
+      int* done = p.counters + kCounters * kMaxParts;
       *sm_flag = atomicAdd(done, 1) == (int)gridDim.x - 1;
       if (*sm_flag) *done = 0;
     }
@@ -917,7 +1056,7 @@ int sm_count() {
     (void)cudaGetLastError();
     return 148;
   }
-  if (cached[dev] == 0) cached[dev] = sms < kMaxBlocks ? sms : kMaxBlocks;
+  if (cached[dev] == 0) cached[dev] = std::min(sms, kMaxParts / kPerSm);
   return cached[dev];
 }
 
@@ -954,7 +1093,7 @@ int launch_decode(DecodeParams& p, int grid, cudaStream_t stream) {
   int dev = 0;
   MOA_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= kMaxDevices || !ready[dev]) {
-    MOA_CUDA_CHECK(cudaFuncSetAttribute(paged_decode_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kBytes));
+    MOA_CUDA_CHECK(cudaFuncSetAttribute(paged_decode_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D, MT>::kBytes));
     if (dev >= 0 && dev < kMaxDevices) ready[dev] = true;
   }
   CUtensorMap map_k, map_v;
@@ -962,7 +1101,7 @@ int launch_decode(DecodeParams& p, int grid, cudaStream_t stream) {
   p.tma = p.pool.shift >= 4 &&      // a unit lies in one page
           make_map(&map_k, p.pool.k, p, p.pool.k_page, p.pool.k_head, p.pool.k_slot, D, bf16) &&
           make_map(&map_v, p.pool.v, p, p.pool.v_page, p.pool.v_head, p.pool.v_slot, D, bf16);
-  paged_decode_kernel<T, D, MT><<<grid, kDecodeThreads, Layout<D>::kBytes, stream>>>(map_k, map_v, p);
+  paged_decode_kernel<T, D, MT><<<grid, kDecodeThreads, Layout<D, MT>::kBytes, stream>>>(map_k, map_v, p);
   MOA_CUDA_CHECK(cudaGetLastError());
   return MOA_OK;
 }
@@ -1062,8 +1201,9 @@ int moa_paged_append(const moa_paged_append_args* args, moa_stream_t stream) {
 }
 
 int64_t moa_paged_decode_workspace_bytes(void) {
-  static_assert((3 * moa::kMaxBlocks + 1) * 4 <= MOA_PAGED_COUNTER_BYTES, "counters");
-  return MOA_PAGED_COUNTER_BYTES + (int64_t)moa::sm_count() * 2 * moa::kRecFloats * 4;
+  using namespace moa;
+  static_assert((kCounters * kMaxParts + 1) * 4 <= MOA_PAGED_COUNTER_BYTES, "counters");
+  return MOA_PAGED_COUNTER_BYTES + (int64_t)sm_count() * kPerSm * 2 * kRecFloats * 4;
 }
 
 int moa_paged_decode(const moa_paged_decode_args* args, moa_stream_t stream) {
@@ -1099,9 +1239,9 @@ int moa_paged_decode(const moa_paged_decode_args* args, moa_stream_t stream) {
   p.out_f32 = a.out_f32 != 0; p.advance = a.advance != 0;
   p.counters = reinterpret_cast<int*>(a.workspace);
   p.records = reinterpret_cast<float*>(reinterpret_cast<char*>(a.workspace) + MOA_PAGED_COUNTER_BYTES);
-  // one block per SM, or as many as the longest sequences that the table allows could employ
+  // as many blocks as the longest sequences that the table allows could employ
   const int64_t most = a.B * a.KV * p.tiles * (std::min(ceil_div64(p.capacity, kUnit), (int64_t)4096) + kItemCost);
-  const int grid = (int)std::max((int64_t)1, std::min((int64_t)sm_count(), most / kMinUnits));
+  const int grid = (int)std::max((int64_t)1, std::min((int64_t)sm_count() * kPerSm, most / kMinUnits));
   cudaStream_t st = (cudaStream_t)stream;
   return a.dtype == MOA_F16 ? launch_decode<__half>(p, (int)a.D, grid, st)
                             : launch_decode<__nv_bfloat16>(p, (int)a.D, grid, st);

@@ -452,7 +452,8 @@ def test_step(dtype, D, H, KV, page, layout, lengths, kind, spanned):
     # the two calls that the step stands for, without the rotation of the query
     if rope is None:
         n = torch.where(c.lengths < 0, c.lengths, c.lengths + 1)
-        assert torch.equal(out, moa_b200.paged_decode(q, c.kp, c.vp, c.table, n, D ** -0.5, sink_size=sink, local_size=local))
+        two = moa_b200.paged_decode(q, c.kp, c.vp, c.table, n, D ** -0.5, sink_size=sink, local_size=local)
+        close(two, ref, tol)     # not bit for bit: the step adds the new token first, and fp32 sums depend on their order
 
 
 def test_step_advances_and_decodes_on():
