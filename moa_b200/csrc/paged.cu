@@ -212,7 +212,7 @@ __global__ void paged_advance_kernel(int32_t* lengths, const int32_t* counts, in
 constexpr int kWarps = 4, kDecodeThreads = kWarps * 32;
 constexpr int kPerSm = 2;                   // resident blocks per SM
 constexpr int kUnit = 16;                   // positions of a unit (k of the second product)
-constexpr int kItemCost = 2;                // an item's epilogue, in units
+constexpr int kItemCost = 12;               // an item's epilogue, in units
 constexpr int kMinUnits = 8;                // least share of a block: fewer blocks work when there is less
 constexpr int kJoin = 18;                   // partial results joined at once
 constexpr int kMaxParts = kJoin * kJoin;    // two levels of joining
@@ -236,6 +236,14 @@ struct DecodeParams {
   int* counters;                            // kCounters per part, zero between launches, and one behind them
   float* records;                           // 2 per part
 };
+
+// A flag that the compiler takes to change: loops are not made in two versions for it (the kernel has to be
+// fetched through the caches that the keys run through, its size counts).
+__device__ __forceinline__ bool opaque(bool flag) {
+  int x = flag;
+  asm volatile("" : "+r"(x));
+  return x != 0;
+}
 
 // The lengths and spans as a block sees them.
 struct Sizes {
@@ -270,7 +278,7 @@ struct Span {
   __device__ __forceinline__ Span() {}
   __device__ __forceinline__ Span(const Sizes& s, int tokens, int kh) {
     n = sink = from = tokens;
-    if (s.p.sink) {
+    if (opaque(s.p.sink != nullptr)) {
       const int2 sl = s.sink_local(kh);
       sink = min(sl.x, n);
       from = n - min(sl.y, n);
@@ -303,7 +311,9 @@ struct Cut {
   // The last c with begin(c) <= x.
   __device__ __forceinline__ int part_of(int64_t x) const {
     int c = min((int)((float)x / (float)total * parts), parts - 1);
+#pragma unroll 1
     while (begin(c) > x) --c;
+#pragma unroll 1
     while (c + 1 < parts && begin(c + 1) <= x) ++c;
     return c;
   }
@@ -435,8 +445,9 @@ struct Layout {
   // what an item needs: queries (rows padded by 16 bytes), the new token's key, value, cos and sin, its page
   static constexpr int kQPitch = D * 2 + 16, kKey = 8 * MT * kQPitch, kValue = kKey + D * 2, kCos = kValue + D * 2,
                        kSin = kCos + D * 4, kPage = kSin + D * 4, kItemBytes = kPage + 16;
+  static constexpr int kLowBytes = 8 * MT * kQPitch;                   // what rotated queries have beyond 16 bits
   static constexpr int kBarBytes = kWarps * kStages * 8, kMaskBytes = kWarps * kStages * 4;
-  static constexpr int kBytes = 1024 + kRing + kJoinBytes + 2 * kItemBytes + kBarBytes + kMaskBytes + 2 * kWarps * 8 * 4 + 128 +
+  static constexpr int kBytes = 1024 + kRing + kJoinBytes + 2 * kItemBytes + kLowBytes + kBarBytes + kMaskBytes + 2 * kWarps * 8 * 4 + 128 +
                                 kCached * 12;
   static_assert(kPerSm * (kBytes + 1024) <= 233472, "shared memory");
   static __device__ __forceinline__ uint32_t at(int row, int chunk) {
@@ -496,6 +507,24 @@ __device__ __forceinline__ float2 table2(const unsigned char* row, int d, bool f
   return Cvt<T>::unpack(*reinterpret_cast<const uint32_t*>(row + d * 2));
 }
 
+// The item's queries are rotated in their buffer, by the whole block: what fits T stays there, the rest goes to `low`.
+template <typename T, int D, int MT>
+__device__ __forceinline__ void turn_queries(const DecodeParams& p, unsigned char* item, unsigned char* low, int heads) {
+  using L = Layout<D, MT>;
+  const bool f32 = p.pool.rope_f32;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < heads * (D / 4); i += kDecodeThreads) {
+    const int head = i / (D / 4), d = i % (D / 4) * 2;       // a pair of coordinates of either half
+    uint32_t* q = reinterpret_cast<uint32_t*>(item + head * L::kQPitch);
+    uint32_t* r = reinterpret_cast<uint32_t*>(low + head * L::kQPitch);
+    const float2 a = Cvt<T>::unpack(q[d / 2]), b = Cvt<T>::unpack(q[(d + D / 2) / 2]);
+    const float2 cl = table2<T>(item + L::kCos, d, f32), ch = table2<T>(item + L::kCos, d + D / 2, f32);
+    const float2 sl = table2<T>(item + L::kSin, d, f32), sh = table2<T>(item + L::kSin, d + D / 2, f32);
+    split2<T, true>(fmaf(a.x, cl.x, -b.x * sl.x), fmaf(a.y, cl.y, -b.y * sl.y), q[d / 2], r[d / 2]);
+    split2<T, true>(fmaf(b.x, ch.x, a.x * sh.x), fmaf(b.y, ch.y, a.y * sh.y), q[(d + D / 2) / 2], r[(d + D / 2) / 2]);
+  }
+}
+
 // The new token's key is rotated in its buffer (a warp's work) and stored, with its value, into its page.
 template <typename T, int D, int MT>
 __device__ __noinline__ void place_new(const DecodeParams& p, unsigned char* item, int kh, int slot, int page, bool store) {
@@ -550,7 +579,7 @@ __device__ __noinline__ uint32_t load_rows(const DecodeParams& p, int b, int kh,
     vs += page * p.pool.v_page + kh * p.pool.v_head + slot * p.pool.v_slot;
   }
   present = __ballot_sync(0xffffffffu, take) & 0xffffu;
-#pragma unroll 2
+#pragma unroll 1
   for (int i = 0; i < kUnit / RPI; ++i) {
     const int row = i * RPI + lane / LPR, chunk = lane % LPR;
     const T* k_row = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ks), row));
@@ -571,7 +600,6 @@ __device__ __noinline__ void join_parts(const DecodeParams& p, int c0, int c1, i
   const int tid = threadIdx.x;
   float* wm = scratch;                             // (record, head): maximum and sum
   float* wl = scratch + kJoin * kRecHeads;
-  auto record_of = [&](int i) { return p.records + (int64_t)(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * kRecFloats; };
   // at each level groups of kJoin neighbours; `step` parts lie behind one of them
   int index = (int)blockIdx.x - c0, there = c1 - c0 + 1, step = 1;
   for (int level = 0;; ++level) {
@@ -588,38 +616,48 @@ __device__ __noinline__ void join_parts(const DecodeParams& p, int c0, int c1, i
     __syncthreads();
     if (!*flag) return;
     __threadfence();
+    // record i of the group; a part's second record is of the item that begins in it
+    float* const records = p.records + (int64_t)(2 * (c0 + first)) * kRecFloats;
+    const uint32_t stride = 2 * step * (uint32_t)kRecFloats, shift0 = first == 0 ? (uint32_t)kRecFloats : 0;
+#pragma unroll 1
     for (int k = tid; k < kJoin * kRecHeads; k += kDecodeThreads) {
       const int i = k / kRecHeads, head = k % kRecHeads;
       if (i < count && head < heads) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(record_of(first + i * step) + kRecHeads * 128 + head * 2));
+        const float* rec = records + (i == 0 ? shift0 : i * stride);
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(rec + kRecHeads * 128 + head * 2));
         wm[k] = ml.x;
         wl[k] = ml.y;
       }
     }
     __syncthreads();
-    float* to = record_of(first);
-    for (int i4 = tid; i4 < heads * D / 4; i4 += kDecodeThreads) {
-      const int head = i4 * 4 / D, d = i4 * 4 % D;
-      float4 x[kJoin];
-#pragma unroll
-      for (int i = 0; i < kJoin; ++i)
-        if (i < count) x[i] = __ldcg(reinterpret_cast<const float4*>(record_of(first + i * step) + i4 * 4));
+    float* to = records + shift0;
+#pragma unroll 1
+    for (int i4 = tid * 4; i4 < heads * D; i4 += kDecodeThreads * 4) {
+      const int head = i4 / D, d = i4 % D;
       float M = -INFINITY, Ls = 0.f;
+#pragma unroll 1
       for (int i = 0; i < count; ++i) M = fmaxf(M, wm[i * kRecHeads + head]);
       const float base = M == -INFINITY ? 0.f : M;
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int i0 = 0; i0 < count; i0 += 9) {      // nine loads at a time
+        float4 x[9];
 #pragma unroll
-      for (int i = 0; i < kJoin; ++i)
-        if (i < count) {
-          const float f = exp2f(wm[i * kRecHeads + head] - base);
-          Ls += f * wl[i * kRecHeads + head];
-          O.x += f * x[i].x; O.y += f * x[i].y; O.z += f * x[i].z; O.w += f * x[i].w;
-        }
+        for (int i = 0; i < 9; ++i)
+          if (i0 + i < count) x[i] = __ldcg(reinterpret_cast<const float4*>(records + (i0 + i == 0 ? shift0 : (i0 + i) * stride) + i4));
+#pragma unroll
+        for (int i = 0; i < 9; ++i)
+          if (i0 + i < count) {
+            const float f = exp2f(wm[(i0 + i) * kRecHeads + head] - base);
+            Ls += f * wl[(i0 + i) * kRecHeads + head];
+            O.x += f * x[i].x; O.y += f * x[i].y; O.z += f * x[i].z; O.w += f * x[i].w;
+          }
+      }
       if (final) {
         store_out4<T>(p, b, h0 + head, d, O, Ls);
       } else {
         // (each element of the group's first record is read by the thread that writes it)
-        *reinterpret_cast<float4*>(to + i4 * 4) = O;
+        *reinterpret_cast<float4*>(to + i4) = O;
         if (d == 0) *reinterpret_cast<float2*>(to + kRecHeads * 128 + head * 2) = make_float2(M, Ls);
       }
     }
@@ -641,7 +679,8 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* sm_o = reinterpret_cast<float*>(smem + L::kRing);
   unsigned char* sm_item = smem + L::kRing + L::kJoinBytes;
-  unsigned char* sm_bar = sm_item + 2 * L::kItemBytes;
+  unsigned char* sm_low = sm_item + 2 * L::kItemBytes;
+  unsigned char* sm_bar = sm_low + L::kLowBytes;
   uint32_t* sm_mask = reinterpret_cast<uint32_t*>(sm_bar + L::kBarBytes);
   float* sm_m = reinterpret_cast<float*>(sm_mask + kWarps * kStages);
   float* sm_l = sm_m + kWarps * 8;
@@ -654,8 +693,10 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
   const Sizes sizes = {p, sm_len, sm_span};
 
   // ---- the line: its length, and where this block's part begins
+#pragma unroll 1
   for (int b = tid; b < min(p.B, kCached); b += kDecodeThreads) sm_len[b] = p.lengths[b];
   if (p.sink)
+#pragma unroll 1
     for (int kh = tid; kh < min(p.KV, kCached); kh += kDecodeThreads) sm_span[kh] = Sizes::clamped(p.sink[kh], p.local[kh]);
   const uint32_t bars = (uint32_t)__cvta_generic_to_shared(sm_bar) + warp * kStages * 8;
   if (lane < kStages) {
@@ -663,18 +704,22 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
-  const int per = (p.B + kDecodeThreads - 1) / kDecodeThreads;
-  const int b_lo = min(tid * per, p.B), b_hi = min(b_lo + per, p.B);
-  auto cost_of = [&](int b) {
-    const int n = sizes.tokens(b);
-    if (!p.sink) return (int64_t)p.KV * p.tiles * (((n + 15) >> 4) + kItemCost);
-    int64_t sum = 0;
-#pragma unroll 4
-    for (int kh = 0; kh < p.KV; ++kh) sum += Span(sizes, n, kh).units + kItemCost;
-    return sum * p.tiles;
-  };
+  // in rows of items that cost the same: a sequence's, or with spans a (sequence, key head)'s
+  const int per_seq = p.sink ? p.KV : 1, items = p.sink ? p.tiles : p.KV * p.tiles;
+  const uint32_t rows = (uint32_t)p.B * per_seq, per = (rows - 1) / kDecodeThreads + 1;      // (B, KV < 2^16)
+  const uint32_t row_lo = min(tid * per, rows), row_hi = row_lo + min(per, rows - row_lo);
+  const int b_lo = (int)(row_lo / per_seq), kh_lo = (int)(row_lo - (uint32_t)b_lo * per_seq);
+  auto cost_of = [&](int b, int kh) { return Span(sizes, sizes.tokens(b), kh).units + kItemCost; };
   int64_t mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += cost_of(b);
+  int b_at = b_lo, kh_at = kh_lo;
+#pragma unroll 1
+  for (uint32_t r = row_lo; r < row_hi; ++r) {
+    mine += (int64_t)items * cost_of(b_at, kh_at);
+    if (++kh_at == per_seq) {
+      kh_at = 0;
+      ++b_at;
+    }
+  }
   int64_t before = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -695,24 +740,24 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
 
   if (block < cut.parts) {
     const int64_t lo = cut.begin(block), hi = cut.begin(block + 1);
-    if (before <= lo && lo < before + mine) {      // one thread: the part begins among its sequences
+    if (before <= lo && lo < before + mine) {      // one thread: the part begins in one of its rows
       int64_t at = before;
-      int b = b_lo;
-      for (int64_t c; lo >= at + (c = cost_of(b)); ++b) at += c;
-      const int n = sizes.tokens(b);
-      int kh = 0, tile = 0;
+      int b = b_lo, kh = kh_lo, cost;
+#pragma unroll 1
       for (;;) {
-        const int c = Span(sizes, n, kh).units + kItemCost;
-        if (lo < at + c) break;
-        at += c;
-        if (++tile == p.tiles) {
-          tile = 0;
-          ++kh;
+        cost = cost_of(b, kh);
+        const int64_t end = at + (int64_t)items * cost;
+        if (lo < end) break;
+        at = end;
+        if (++kh == per_seq) {
+          kh = 0;
+          ++b;
         }
       }
+      const int item = (int)((lo - at) / cost);
       sm_scan[8] = b;
-      sm_scan[9] = (int64_t)kh << 32 | tile;
-      sm_scan[10] = at;
+      sm_scan[9] = (int64_t)(kh + item / p.tiles) << 32 | (item % p.tiles);
+      sm_scan[10] = at + (int64_t)item * cost;
     }
     __syncthreads();
     Cursor cur;
@@ -739,7 +784,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
       ld_x = ld.span.unit(ld_u);
       ld_mask = ld.span.mask(ld_x);
       const int32_t* row = p.pool.table + (int64_t)ld.b * p.pool.table_stride;
-      if (p.pool.shift >= 4) {
+      if (opaque(p.pool.shift >= 4)) {
         ld_page = row[ld_x >> (p.pool.shift - 4)];
       } else {
         const int pos = ld_x * 16 + (lane & 15);
@@ -760,7 +805,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
     auto ld_issue = [&](int stage) {
       if (ld_more) {
         const uint32_t dst = ring + stage * L::kStageBytes, bar = bars + stage * 8;
-        if (ld_mask == 0xffffu && p.tma && (uint32_t)ld_page < (uint32_t)p.pool.num_pages) {
+        if (ld_mask == 0xffffu && opaque(p.tma) && (uint32_t)ld_page < (uint32_t)p.pool.num_pages) {
           if (lane == 0) {
             const int slot = (ld_x << 4) & ((1 << p.pool.shift) - 1);
             my_mask[stage] = 0xffffu;              // seen by the other lanes when they have waited on the barrier
@@ -778,8 +823,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
           }
         }
         ld_u += kWarps;
-        if (ld_u < ld.u1) ld_look();
-        else ld_seek();
+        ld_seek();
       }
       cp_async_commit();                           // a group per call, empty or not: they are counted
     };
@@ -813,10 +857,14 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
         const int page = *reinterpret_cast<const int*>(item + L::kPage);
         const bool placed = (uint32_t)page < (uint32_t)p.pool.num_pages && (turn || !p.pool.cos);
         with_new = placed && cur.span.sees_last();
-        if (warp == 0) {
+        if (warp == kWarps - 1) {
           if (placed) place_new<T, D, MT>(p, item, cur.kh, (cur.n - 1) & ((1 << p.pool.shift) - 1), page, cur.tile == 0);
           else if (lane == 0) report(p.pool.cos && !turn ? kStatusRope : kStatusAppend, cur.b, cur.n - 1, cur.kh);
         }
+      }
+      if (turn) {
+        turn_queries<T, D, MT>(p, item, sm_low, heads);
+        __syncthreads();
       }
       if (owner && cur.kh == 0 && cur.tile == 0 && tid == 0) {
         const int64_t wanted = (int64_t)sizes.length(cur.b) + (p.k_new ? 1 : 0);
@@ -825,6 +873,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
 
       if (units == 0) {                            // nothing to attend (a part's first item may not be its own)
         if (owner)
+#pragma unroll 1
           for (int i = tid * 4; i < heads * D; i += kDecodeThreads * 4)
             store_out4<T>(p, cur.b, h0 + i / D, i % D, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
       } else if (cur.u0 < cur.u1) {
@@ -851,18 +900,12 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
               qa[mt][ks][1] = qa[mt][ks][3] = 0u;
             }
             if (turn) {
-              const bool f32 = p.pool.rope_f32;
+              const unsigned char* r = sm_low + (mt * 8 + g) * L::kQPitch + 4 * t;
 #pragma unroll
-              for (int ks = 0; ks < KS / 2; ++ks)
-#pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                  const int d = ks * 16 + e * 4 + 2 * t;
-                  const float2 cl = table2<T>(item + L::kCos, d, f32), ch = table2<T>(item + L::kCos, d + D / 2, f32);
-                  const float2 sl = table2<T>(item + L::kSin, d, f32), sh = table2<T>(item + L::kSin, d + D / 2, f32);
-                  const float2 a = Cvt<T>::unpack(qa[mt][ks][e]), b = Cvt<T>::unpack(qa[mt][ks + KS / 2][e]);
-                  split2<T, true>(fmaf(a.x, cl.x, -b.x * sl.x), fmaf(a.y, cl.y, -b.y * sl.y), qa[mt][ks][e], qa[mt][ks][e + 1]);
-                  split2<T, true>(fmaf(b.x, ch.x, a.x * sh.x), fmaf(b.y, ch.y, a.y * sh.y), qa[mt][ks + KS / 2][e], qa[mt][ks + KS / 2][e + 1]);
-                }
+              for (int ks = 0; ks < KS; ++ks) {
+                qa[mt][ks][1] = *reinterpret_cast<const uint32_t*>(r + ks * 32);
+                qa[mt][ks][3] = *reinterpret_cast<const uint32_t*>(r + ks * 32 + 16);
+              }
             }
           }
           if (with_new && warp == 0) {             // start from the new token: column 0 of a tile of keys, weight 1
@@ -893,7 +936,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
           const uint32_t v_at = L::kTileBytes + ((mi & 1) * 8 + r8) * 128 + (((mi >> 1) ^ r8) << 4);
 #pragma unroll 1
           for (int u = cur.u0 + warp; u < cur.u1; u += kWarps) {
-            if (waiting) waiting = __all_sync(0xffffffffu, bar_wait(bars + stage * 8, parity));
+            if (opaque(waiting)) waiting = __all_sync(0xffffffffu, bar_wait(bars + stage * 8, parity));
             const uint32_t base = ring + stage * L::kStageBytes;
             const uint32_t present = my_mask[stage];
             if (present & kByHand) {
@@ -921,7 +964,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
               float s[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) s[e] = sc[mt][e >> 1][e & 1];
-              if (turn) {
+              if (opaque(turn)) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[e] = joined(s[e], sc[mt][e >> 1][(e & 1) + 2]);
               }
@@ -999,6 +1042,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
             }
           }
           __syncthreads();
+#pragma unroll 1
           for (int i = tid * 4; i < here * D; i += kDecodeThreads * 4) {
             const int head = i / D, d = i % D;
             float M = -INFINITY, Ls = 0.f;
@@ -1039,6 +1083,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
     }
     __syncthreads();
     if (*sm_flag)
+#pragma unroll 1
       for (int b = tid; b < p.B; b += kDecodeThreads) {
         const int len = p.lengths[b];
         if (len >= 0 && len < 2147483647) p.lengths[b] = len + 1;
