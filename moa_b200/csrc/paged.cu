@@ -212,7 +212,7 @@ __global__ void paged_advance_kernel(int32_t* lengths, const int32_t* counts, in
 constexpr int kWarps = 4, kDecodeThreads = kWarps * 32;
 constexpr int kPerSm = 2;                   // resident blocks per SM
 constexpr int kUnit = 16;                   // positions of a unit (k of the second product)
-constexpr int kItemCost = 12;               // an item's epilogue, in units
+constexpr int kItemCost = 16;               // an item's epilogue, in units
 constexpr int kMinUnits = 8;                // least share of a block: fewer blocks work when there is less
 constexpr int kJoin = 18;                   // partial results joined at once
 constexpr int kMaxParts = kJoin * kJoin;    // two levels of joining
@@ -525,34 +525,35 @@ __device__ __forceinline__ void turn_queries(const DecodeParams& p, unsigned cha
   }
 }
 
-// The new token's key is rotated in its buffer (a warp's work) and stored, with its value, into its page.
+// The new token's key is rotated in its buffer (a warp's work).
 template <typename T, int D, int MT>
-__device__ __noinline__ void place_new(const DecodeParams& p, unsigned char* item, int kh, int slot, int page, bool store) {
+__device__ __forceinline__ void turn_key(const DecodeParams& p, unsigned char* item) {
   using L = Layout<D, MT>;
-  const int lane = threadIdx.x & 31;
-  T* key = reinterpret_cast<T*>(item + L::kKey);
-  const T* value = reinterpret_cast<const T*>(item + L::kValue);
-  if (lane < D / 4) {                              // a pair of coordinates of either half
-#pragma unroll
-    for (int d = lane * 2; d < D / 2; d += 64) {
-      uint32_t* lo = reinterpret_cast<uint32_t*>(key + d);
-      uint32_t* hi = reinterpret_cast<uint32_t*>(key + d + D / 2);
-      if (p.pool.cos) {
-        const bool f32 = p.pool.rope_f32;
-        const float2 a = Cvt<T>::unpack(*lo), b = Cvt<T>::unpack(*hi);
-        const float2 cl = table2<T>(item + L::kCos, d, f32), ch = table2<T>(item + L::kCos, d + D / 2, f32);
-        const float2 sl = table2<T>(item + L::kSin, d, f32), sh = table2<T>(item + L::kSin, d + D / 2, f32);
-        *lo = Cvt<T>::pack(fmaf(a.x, cl.x, -b.x * sl.x), fmaf(a.y, cl.y, -b.y * sl.y));
-        *hi = Cvt<T>::pack(fmaf(b.x, ch.x, a.x * sh.x), fmaf(b.y, ch.y, a.y * sh.y));
-      }
-    }
+  const int d = (threadIdx.x & 31) * 2;            // a pair of coordinates of either half
+  const bool f32 = p.pool.rope_f32;
+  if (d < D / 2) {
+    uint32_t* lo = reinterpret_cast<uint32_t*>(item + L::kKey + d * 2);
+    uint32_t* hi = reinterpret_cast<uint32_t*>(item + L::kKey + (d + D / 2) * 2);
+    const float2 a = Cvt<T>::unpack(*lo), b = Cvt<T>::unpack(*hi);
+    const float2 cl = table2<T>(item + L::kCos, d, f32), ch = table2<T>(item + L::kCos, d + D / 2, f32);
+    const float2 sl = table2<T>(item + L::kSin, d, f32), sh = table2<T>(item + L::kSin, d + D / 2, f32);
+    *lo = Cvt<T>::pack(fmaf(a.x, cl.x, -b.x * sl.x), fmaf(a.y, cl.y, -b.y * sl.y));
+    *hi = Cvt<T>::pack(fmaf(b.x, ch.x, a.x * sh.x), fmaf(b.y, ch.y, a.y * sh.y));
   }
-  __syncwarp();
-  if (store && lane < D / 8) {
-    T* kd = reinterpret_cast<T*>(p.pool.k) + page * p.pool.k_page + kh * p.pool.k_head + slot * p.pool.k_slot + lane * 8;
-    T* vd = reinterpret_cast<T*>(p.pool.v) + page * p.pool.v_page + kh * p.pool.v_head + slot * p.pool.v_slot + lane * 8;
-    *reinterpret_cast<uint4*>(kd) = *reinterpret_cast<const uint4*>(key + lane * 8);
-    *reinterpret_cast<uint4*>(vd) = *reinterpret_cast<const uint4*>(value + lane * 8);
+}
+
+// The new token's rows go into their page (a warp's work).
+template <typename T, int D, int MT>
+__device__ __forceinline__ void store_new(const DecodeParams& p, const unsigned char* item, int kh, int slot, int page) {
+  using L = Layout<D, MT>;
+  const int lane = threadIdx.x & 31, chunk = lane % (D / 8);
+  if (lane >= 2 * (D / 8)) return;
+  if (lane < D / 8) {
+    T* to = reinterpret_cast<T*>(p.pool.k) + page * p.pool.k_page + kh * p.pool.k_head + slot * p.pool.k_slot;
+    *reinterpret_cast<uint4*>(to + chunk * 8) = *reinterpret_cast<const uint4*>(item + L::kKey + chunk * 16);
+  } else {
+    T* to = reinterpret_cast<T*>(p.pool.v) + page * p.pool.v_page + kh * p.pool.v_head + slot * p.pool.v_slot;
+    *reinterpret_cast<uint4*>(to + chunk * 8) = *reinterpret_cast<const uint4*>(item + L::kValue + chunk * 16);
   }
 }
 
@@ -598,8 +599,9 @@ template <typename T, int D>
 __device__ __noinline__ void join_parts(const DecodeParams& p, int c0, int c1, int b, int h0, int heads, float* scratch,
                                         int* flag) {
   const int tid = threadIdx.x;
-  float* wm = scratch;                             // (record, head): maximum and sum
-  float* wl = scratch + kJoin * kRecHeads;
+  float* weight = scratch;                         // (record, head); then by head
+  float* top = scratch + kJoin * kRecHeads;
+  float* total = top + kRecHeads;
   // at each level groups of kJoin neighbours; `step` parts lie behind one of them
   int index = (int)blockIdx.x - c0, there = c1 - c0 + 1, step = 1;
   for (int level = 0;; ++level) {
@@ -619,46 +621,71 @@ __device__ __noinline__ void join_parts(const DecodeParams& p, int c0, int c1, i
     // record i of the group; a part's second record is of the item that begins in it
     float* const records = p.records + (int64_t)(2 * (c0 + first)) * kRecFloats;
     const uint32_t stride = 2 * step * (uint32_t)kRecFloats, shift0 = first == 0 ? (uint32_t)kRecFloats : 0;
-#pragma unroll 1
-    for (int k = tid; k < kJoin * kRecHeads; k += kDecodeThreads) {
-      const int i = k / kRecHeads, head = k % kRecHeads;
-      if (i < count && head < heads) {
-        const float* rec = records + (i == 0 ? shift0 : i * stride);
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(rec + kRecHeads * 128 + head * 2));
-        wm[k] = ml.x;
-        wl[k] = ml.y;
+    // four coordinates of kAtOnce records at a time (more would take registers from the kernel's loop); the first ones
+    // are asked for before the weights are known
+    constexpr int kAtOnce = kJoin / 2;
+    float4 x[kAtOnce];
+    auto load = [&](int e, int i0) {
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i)
+        if (i0 + i < count)
+          x[i] = __ldcg(reinterpret_cast<const float4*>(records + (i0 + i == 0 ? shift0 : (i0 + i) * stride) + e));
+    };
+    if (tid * 4 < heads * D) load(tid * 4, 0);
+    if (tid < kRecHeads * 8 && tid / 8 < heads) {  // eight threads a head: its maximum, and every record's weight
+      const int head = tid / 8;
+      float2 ml[(kJoin + 7) / 8];
+      float M = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < (kJoin + 7) / 8; ++k) {
+        const int i = tid % 8 + k * 8;
+        ml[k] = make_float2(-INFINITY, 0.f);
+        if (i < count)
+          ml[k] = __ldcg(reinterpret_cast<const float2*>(records + (i == 0 ? shift0 : i * stride) + kRecHeads * 128 + head * 2));
+      }
+#pragma unroll
+      for (int k = 0; k < (kJoin + 7) / 8; ++k) M = fmaxf(M, ml[k].x);
+#pragma unroll
+      for (int off = 1; off < 8; off <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffu << (tid & 24), M, off));
+      const float base = M == -INFINITY ? 0.f : M;
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < (kJoin + 7) / 8; ++k) {
+        const int i = tid % 8 + k * 8;
+        if (i >= count) break;
+        const float f = exp2f(ml[k].x - base);
+        weight[i * kRecHeads + head] = f;
+        sum += f * ml[k].y;
+      }
+#pragma unroll
+      for (int off = 1; off < 8; off <<= 1) sum += __shfl_xor_sync(0xffu << (tid & 24), sum, off);
+      if (tid % 8 == 0) {
+        top[head] = M;
+        total[head] = sum;
       }
     }
     __syncthreads();
-    float* to = records + shift0;
 #pragma unroll 1
-    for (int i4 = tid * 4; i4 < heads * D; i4 += kDecodeThreads * 4) {
-      const int head = i4 / D, d = i4 % D;
-      float M = -INFINITY, Ls = 0.f;
-#pragma unroll 1
-      for (int i = 0; i < count; ++i) M = fmaxf(M, wm[i * kRecHeads + head]);
-      const float base = M == -INFINITY ? 0.f : M;
+    for (int e = tid * 4; e < heads * D; e += kDecodeThreads * 4) {
+      const int head = e / D;
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-      for (int i0 = 0; i0 < count; i0 += 9) {      // nine loads at a time
-        float4 x[9];
+      for (int i0 = 0; i0 < count; i0 += kAtOnce) {
+        if (e >= kDecodeThreads * 4 || i0 > 0) load(e, i0);
 #pragma unroll
-        for (int i = 0; i < 9; ++i)
-          if (i0 + i < count) x[i] = __ldcg(reinterpret_cast<const float4*>(records + (i0 + i == 0 ? shift0 : (i0 + i) * stride) + i4));
-#pragma unroll
-        for (int i = 0; i < 9; ++i)
+        for (int i = 0; i < kAtOnce; ++i)
           if (i0 + i < count) {
-            const float f = exp2f(wm[(i0 + i) * kRecHeads + head] - base);
-            Ls += f * wl[(i0 + i) * kRecHeads + head];
+            const float f = weight[(i0 + i) * kRecHeads + head];
             O.x += f * x[i].x; O.y += f * x[i].y; O.z += f * x[i].z; O.w += f * x[i].w;
           }
       }
       if (final) {
-        store_out4<T>(p, b, h0 + head, d, O, Ls);
+        store_out4<T>(p, b, h0 + head, e % D, O, total[head]);
       } else {
-        // (each element of the group's first record is read by the thread that writes it)
-        *reinterpret_cast<float4*>(to + i4) = O;
-        if (d == 0) *reinterpret_cast<float2*>(to + kRecHeads * 128 + head * 2) = make_float2(M, Ls);
+        // (each element of the group's first record is read by the thread that writes it, maxima and sums above)
+        float* to = records + shift0;
+        *reinterpret_cast<float4*>(to + e) = O;
+        if (e % D == 0) *reinterpret_cast<float2*>(to + kRecHeads * 128 + head * 2) = make_float2(top[head], total[head]);
       }
     }
     if (final) return;
@@ -692,6 +719,10 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Sizes sizes = {p, sm_len, sm_span};
 
+  if (tid == 0 && p.tma) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+  }
   // ---- the line: its length, and where this block's part begins
 #pragma unroll 1
   for (int b = tid; b < min(p.B, kCached); b += kDecodeThreads) sm_len[b] = p.lengths[b];
@@ -712,7 +743,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
   auto cost_of = [&](int b, int kh) { return Span(sizes, sizes.tokens(b), kh).units + kItemCost; };
   int64_t mine = 0;
   int b_at = b_lo, kh_at = kh_lo;
-#pragma unroll 1
+#pragma unroll 4
   for (uint32_t r = row_lo; r < row_hi; ++r) {
     mine += (int64_t)items * cost_of(b_at, kh_at);
     if (++kh_at == per_seq) {
@@ -852,19 +883,20 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
       const bool ends = units == 0 ? owner : cur.u0 < cur.u1 && cur.u1 == units;
       const bool fresh = sizes.fresh(cur.b);
       const bool turn = fresh && p.pool.cos && rope_row(p.pool, cur.b, 0, cur.n - 1) >= 0;
+      if (turn) {
+        turn_queries<T, D, MT>(p, item, sm_low, heads);
+        if (warp == kWarps - 1 && ends) turn_key<T, D, MT>(p, item);
+        __syncthreads();
+      }
       bool with_new = false;                       // this block attends the new token
       if (fresh && ends) {
         const int page = *reinterpret_cast<const int*>(item + L::kPage);
         const bool placed = (uint32_t)page < (uint32_t)p.pool.num_pages && (turn || !p.pool.cos);
         with_new = placed && cur.span.sees_last();
-        if (warp == kWarps - 1) {
-          if (placed) place_new<T, D, MT>(p, item, cur.kh, (cur.n - 1) & ((1 << p.pool.shift) - 1), page, cur.tile == 0);
+        if (warp == kWarps - 1 && cur.tile == 0) {
+          if (placed) store_new<T, D, MT>(p, item, cur.kh, (cur.n - 1) & ((1 << p.pool.shift) - 1), page);
           else if (lane == 0) report(p.pool.cos && !turn ? kStatusRope : kStatusAppend, cur.b, cur.n - 1, cur.kh);
         }
-      }
-      if (turn) {
-        turn_queries<T, D, MT>(p, item, sm_low, heads);
-        __syncthreads();
       }
       if (owner && cur.kh == 0 && cur.tile == 0 && tid == 0) {
         const int64_t wanted = (int64_t)sizes.length(cur.b) + (p.k_new ? 1 : 0);
