@@ -23,6 +23,10 @@ _COUNTER_BYTES = 8192
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _NO_ROPE = (0, 0, 0, 0, 0, 0)
 
+# the stream's handle without a Stream object around it, as torch's own generated code asks for it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or _lib.current_stream
+_capturing = torch.cuda.is_current_stream_capturing
+
 _workspaces: Dict = {}
 _touched = set()      # devices that a paged call has run on
 
@@ -30,7 +34,7 @@ _touched = set()      # devices that a paged call has run on
 def _workspace(index: int, stream: int) -> Tensor:
     """Scratch of ``paged_decode``: kept per device and stream; a call that is being captured gets one of its own,
     from the graph's memory, so that two graphs never share one."""
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         ws = torch.empty(lib.moa_paged_decode_workspace_bytes(), dtype=torch.uint8, device=index)
         ws[:_COUNTER_BYTES].zero_()
         return ws
@@ -42,29 +46,28 @@ def _workspace(index: int, stream: int) -> Tensor:
 
 
 # The checks below run on every call, and at decode sizes the host's share of a call is larger than the
-# kernel's: they ask a tensor for each property once (get_device() instead of device, all strides at once).
+# kernel's: they ask a tensor for each property once, and for the cheapest form of it (get_device() instead of
+# device, all strides at once), and they are few functions.
 
-def _pool_arguments(key_pages: Tensor, value_pages: Tensor, page_table: Tensor, lengths: Tensor, B: int, KV: int,
-                    D: int, dtype, device: int):
+def _pool_arguments(key_pages: Tensor, value_pages: Tensor, page_table: Tensor, lengths: Tensor, B: int, D: int, dtype,
+                    device: int):
     assert dtype in _DTYPES, f"the paged cache supports float16 and bfloat16 only, got {dtype}"
     shape = key_pages.shape
-    assert len(shape) == 4 and value_pages.shape == shape and shape[1] == KV and shape[3] == D, \
-        "pages must be (num_pages, KV, page_size, D)"
+    assert len(shape) == 4 and value_pages.shape == shape and shape[3] == D, "pages must be (num_pages, KV, page_size, D)"
     assert key_pages.dtype is dtype and value_pages.dtype is dtype, "pages and tokens must have the same dtype"
-    ks, vs = key_pages.stride(), value_pages.stride()
-    assert ks[3] == 1 and vs[3] == 1, "rows of the pages must be contiguous"
-    ts, width = page_table.stride(), page_table.shape
+    ka, kb, kc, kd = key_pages.stride()
+    va, vb, vc, vd = value_pages.stride()
+    assert kd == 1 and vd == 1, "rows of the pages must be contiguous"
+    width = page_table.shape
     assert len(width) == 2 and width[0] == B and page_table.dtype is torch.int32, "page_table must be int32 (B, max_pages)"
-    assert ts[1] == 1 or width[1] == 1, "rows of page_table must be contiguous"
-    _check_row_of_ints(lengths, B, device, torch.int32, "lengths must be contiguous int32 (B,)")
-    assert key_pages.get_device() == device and value_pages.get_device() == device and \
-        page_table.get_device() == device, "all tensors must be on the same device"
-    return (ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], ts[0], width[1], shape[0], shape[2])
-
-
-def _check_row_of_ints(t: Tensor, n: int, device: int, dtype, what: str) -> None:
-    assert t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous(), what
-    assert t.get_device() == device, "all tensors must be on the same device"
+    width = width[1]
+    ta, tb = page_table.stride()
+    assert tb == 1 or width == 1, "rows of page_table must be contiguous"
+    assert lengths.dtype is torch.int32 and lengths.shape == (B,) and lengths.is_contiguous(), \
+        "lengths must be contiguous int32 (B,)"
+    assert device == key_pages.get_device() == value_pages.get_device() == page_table.get_device() == \
+        lengths.get_device(), "all tensors must be on the same device"
+    return ka, kb, kc, va, vb, vc, ta, width, shape[0], shape[2], shape[1]
 
 
 def _rope_arguments(rope: Tuple[Tensor, Tensor], B: int, N: int, D: int, dtype, device: int):
@@ -75,33 +78,35 @@ def _rope_arguments(rope: Tuple[Tensor, Tensor], B: int, N: int, D: int, dtype, 
     kind = cos.dtype
     assert sin.dtype is kind and (kind is dtype or kind is torch.float32), \
         "rope tables must have the tensors' dtype or be float32"
-    assert cos.get_device() == device and sin.get_device() == device, "all tensors must be on the same device"
+    assert device == cos.get_device() == sin.get_device(), "all tensors must be on the same device"
     if len(shape) == 2:
         assert shape[0] > 0, "a rope table by position needs rows"
-        return (cos.data_ptr(), sin.data_ptr(), 0, stride[0], shape[0], kind is torch.float32)
+        return cos.data_ptr(), sin.data_ptr(), 0, stride[0], shape[0], kind is torch.float32
     assert len(shape) == 3 and (shape[0] == 1 or shape[0] == B) and shape[1] == N, \
         "rope tables must be (positions, D), (B, N, D) or (1, N, D)"
-    return (cos.data_ptr(), sin.data_ptr(), 0 if shape[0] == 1 else stride[0], stride[1], 0, kind is torch.float32)
+    return cos.data_ptr(), sin.data_ptr(), 0 if shape[0] == 1 else stride[0], stride[1], 0, kind is torch.float32
 
 
-def _rows(t: Tensor):
+def _rows(t: Tensor, N: int):
     """``t`` (.., .., N, D), or a copy of it whose rows the kernels can read, with its address and first three strides
     (that of a dimension of one is of no interest)."""
     a, b, n, d = t.stride()
-    if t.shape[2] == 1:
+    ptr = t.data_ptr()
+    if N == 1:
         n = 0
-    if d != 1 or (a | b | n) & 7 or t.data_ptr() & 15:
+    if d != 1 or (a | b | n) & 7 or ptr & 15:
         t = t.clone(memory_format=torch.contiguous_format)
         a, b, n, d = t.stride()
-    return t, t.data_ptr(), (a, b, n)
+        ptr = t.data_ptr()
+    return t, ptr, a, b, n
 
 
-def _inference_only(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise NotImplementedError("the paged cache has no gradient (inference only): call it under torch.no_grad()")
-
-
-def _cuda_only(device: int) -> None:
+def _refuse(device: int, *tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise NotImplementedError(
+                    "the paged cache has no gradient (inference only): call it under torch.no_grad()")
     if device < 0:
         raise RuntimeError("moa_b200 runs on CUDA tensors only (there is no CPU path)")
 
@@ -111,10 +116,10 @@ def _launch(name: str, entry, arguments, device: int) -> None:
     packs the struct once the stream is known (the scratch belongs to it)."""
     if _lib.NVTX or torch.cuda.current_device() != device:
         with torch.cuda.device(device), _lib.nvtx_range("moa_b200." + name):
-            stream = torch.cuda.current_stream(device).cuda_stream
+            stream = _raw_stream(device)
             status = entry(arguments(stream), stream)
     else:
-        stream = torch.cuda.current_stream(device).cuda_stream
+        stream = _raw_stream(device)
         status = entry(arguments(stream), stream)
     if status:
         _lib.check("moa_" + name, status)
@@ -148,7 +153,8 @@ def paged_append(key: Tensor, value: Tensor, key_pages: Tensor, value_pages: Ten
     assert len(shape) == 4 and value.shape == shape, "key and value must be (B, KV, N, D)"
     B, KV, N, D = shape
     dtype, device = key.dtype, key.get_device()
-    pool = _pool_arguments(key_pages, value_pages, page_table, lengths, B, KV, D, dtype, device)
+    pool = _pool_arguments(key_pages, value_pages, page_table, lengths, B, D, dtype, device)
+    assert pool[10] == KV, "pages must be (num_pages, KV, page_size, D)"
     assert value.dtype is dtype and value.get_device() == device, "key and value must be alike"
     H = KV
     if query is not None:
@@ -157,25 +163,27 @@ def paged_append(key: Tensor, value: Tensor, key_pages: Tensor, value_pages: Ten
         assert len(shape) == 4 and shape[0] == B and shape[2] == N and shape[3] == D, "query must be (B, H, N, D)"
         assert query.dtype is dtype and query.get_device() == device, "query and key must be alike"
         H = shape[1]
+    counts_ptr = 0
     if counts is not None:
-        _check_row_of_ints(counts, B, device, torch.int32, "counts must be contiguous int32 (B,)")
+        assert counts.dtype is torch.int32 and counts.shape == (B,) and counts.is_contiguous(), \
+            "counts must be contiguous int32 (B,)"
+        assert counts.get_device() == device, "all tensors must be on the same device"
+        counts_ptr = counts.data_ptr()
     r = _NO_ROPE if rope is None else _rope_arguments(rope, B, N, D, dtype, device)
-    _inference_only(key, value, query)
-    _cuda_only(device)
-    result, q_ptr, q_strides, out_ptrs = None, 0, (0, 0, 0), (0, 0)
+    _refuse(device, key, value, query)
+    result, qo, ko, q_ptr, qa, qb, qn = None, 0, 0, 0, 0, 0, 0
     if query is not None:
-        result = (torch.empty((B, H, N, D), dtype=dtype, device=query.device),
-                  torch.empty((B, KV, N, D), dtype=dtype, device=query.device))
-        query, q_ptr, q_strides = _rows(query)
-        out_ptrs = result[0].data_ptr(), result[1].data_ptr()
+        result = query.new_empty((B, H, N, D)), query.new_empty((B, KV, N, D))
+        qo, ko = result[0].data_ptr(), result[1].data_ptr()
+        query, q_ptr, qa, qb, qn = _rows(query, N)
     if B == 0 or N == 0 or KV == 0:
         return result
-    key, k_ptr, k_strides = _rows(key)
-    value, v_ptr, v_strides = _rows(value)
+    key, k_ptr, ka, kb, kn = _rows(key, N)
+    value, v_ptr, va, vb, vn = _rows(value, N)
     _launch("paged_append", lib.moa_paged_append, lambda stream: _APPEND.pack(
         k_ptr, v_ptr, q_ptr, key_pages.data_ptr(), value_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
-        0 if counts is None else counts.data_ptr(), r[0], r[1], *out_ptrs, *k_strides, *v_strides, *q_strides, *pool,
-        *r[2:], B, H, KV, N, D, _DTYPES[dtype], advance), device)
+        counts_ptr, r[0], r[1], qo, ko, ka, kb, kn, va, vb, vn, qa, qb, qn, *pool[:10], *r[2:], B, H, KV, N, D,
+        _DTYPES[dtype], advance), device)
     return result
 
 
@@ -205,21 +213,21 @@ def paged_decode(query: Tensor, key_pages: Tensor, value_pages: Tensor, page_tab
     assert len(shape) == 4 and shape[2] == 1, "query must be (B, H, 1, D)"
     B, H, _, D = shape
     dtype, device = query.dtype, query.get_device()
-    KV = key_pages.shape[1]
-    pool = _pool_arguments(key_pages, value_pages, page_table, lengths, B, KV, D, dtype, device)
+    pool = _pool_arguments(key_pages, value_pages, page_table, lengths, B, D, dtype, device)
+    KV = pool[10]
     assert KV > 0 and H % KV == 0, "the query heads must be a multiple of the pool's key/value heads"
-    k_ptr = v_ptr = 0
-    k_strides = v_strides = (0, 0, 0)
+    k_ptr = v_ptr = ka = kb = va = vb = 0
     r = _NO_ROPE
     if key is not None:
         assert value is not None, "key and value go together"
-        assert key.shape == (B, KV, 1, D) and value.shape == (B, KV, 1, D), "key and value must be (B, KV, 1, D)"
-        assert key.dtype is dtype and value.dtype is dtype and key.get_device() == device and \
-            value.get_device() == device, "query, key and value must be alike"
+        shape = key.shape
+        assert shape == (B, KV, 1, D) and value.shape == shape, "key and value must be (B, KV, 1, D)"
+        assert key.dtype is dtype and value.dtype is dtype and device == key.get_device() == value.get_device(), \
+            "query, key and value must be alike"
         if rope is not None:
             r = _rope_arguments(rope, B, 1, D, dtype, device)
-        key, k_ptr, k_strides = _rows(key)
-        value, v_ptr, v_strides = _rows(value)
+        key, k_ptr, ka, kb, _ = _rows(key, 1)
+        value, v_ptr, va, vb, _ = _rows(value, 1)
     else:
         assert value is None, "key and value go together"
         assert rope is None, "rope is for the step with a new token"
@@ -228,29 +236,34 @@ def paged_decode(query: Tensor, key_pages: Tensor, value_pages: Tensor, page_tab
     sink_ptr = local_ptr = 0
     if sink_size is not None:
         for t in (sink_size, local_size):
-            _check_row_of_ints(t, KV, device, torch.int64, "sink_size and local_size must be contiguous int64 (KV,)")
+            assert t.dtype is torch.int64 and t.shape == (KV,) and t.is_contiguous(), \
+                "sink_size and local_size must be contiguous int64 (KV,)"
+            assert t.get_device() == device, "all tensors must be on the same device"
         sink_ptr, local_ptr = sink_size.data_ptr(), local_size.data_ptr()
-    _inference_only(query, key, value)
-    _cuda_only(device)
+    _refuse(device, query, key, value)
     if out is None:
-        assert out_dtype is None or out_dtype is dtype or out_dtype is torch.float32
-        out = torch.empty((B, 1, H, D), dtype=out_dtype or dtype, device=query.device)
+        if out_dtype is None or out_dtype is dtype:
+            out = query.new_empty((B, 1, H, D))
+        else:
+            assert out_dtype is torch.float32, "out_dtype must be the query's dtype or float32"
+            out = torch.empty((B, 1, H, D), dtype=torch.float32, device=query.device)
+        oa, ob = H * D, D
     else:
-        assert out.shape == (B, 1, H, D) and out.stride(3) == 1 and out.get_device() == device, "out must be (B, 1, H, D)"
+        assert out.shape == (B, 1, H, D) and out.get_device() == device, "out must be (B, 1, H, D)"
         assert out.dtype is dtype or out.dtype is torch.float32, "out must have the query's dtype or be float32"
         assert out_dtype is None or out_dtype is out.dtype
+        oa, _, ob, od = out.stride()
+        assert od == 1, "rows of out must be contiguous"
     if B == 0 or H == 0:
         return out
-    query, q_ptr, q_strides = _rows(query)
-    o_strides = out.stride()
+    query, q_ptr, qa, qb, _ = _rows(query, 1)
 
     def arguments(stream):
         ws = _workspace(device, stream)
         return _DECODE.pack(
             q_ptr, k_ptr, v_ptr, key_pages.data_ptr(), value_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(),
-            lengths.data_ptr(), sink_ptr, local_ptr, r[0], r[1], ws.data_ptr(), q_strides[0], q_strides[1],
-            k_strides[0], k_strides[1], v_strides[0], v_strides[1], o_strides[0], o_strides[2], *pool, *r[2:],
-            B, H, KV, D, _DTYPES[dtype], out.dtype is torch.float32, advance, ws.numel(), sm_scale)
+            lengths.data_ptr(), sink_ptr, local_ptr, r[0], r[1], ws.data_ptr(), qa, qb, ka, kb, va, vb, oa, ob,
+            *pool[:10], *r[2:], B, H, KV, D, _DTYPES[dtype], out.dtype is torch.float32, advance, ws.numel(), sm_scale)
 
     _launch("paged_decode", lib.moa_paged_decode, arguments, device)
     return out
