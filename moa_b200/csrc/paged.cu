@@ -80,40 +80,48 @@ struct AppendParams {
   const int32_t* counts;
   void *q_out, *k_out;
   int64_t k_sb, k_sh, k_sn, v_sb, v_sh, v_sn, q_sb, q_sh, q_sn;
-  int H, KV, jobs;   // jobs: rows of work per token, KV key/value heads and then, with q, H query heads
+  int H, KV, kv_jobs, jobs;   // jobs of a token: kHeads key/value heads each, then, with q, kHeads query heads each
   int64_t N;
 };
 
-// The two 8-wide pieces [8c, 8c+8) and [D/2 + 8c, ...) of a row, which the rotation mixes:
+// A row of a rope table for the two 8-wide pieces [8c, 8c+8) and [D/2 + 8c, ...) of a row, which the rotation mixes:
 //   x'[d] = x[d] cos[d] - x[d + D/2] sin[d],   x'[d + D/2] = x[d + D/2] cos[d + D/2] + x[d] sin[d + D/2]
 // in fp32, rounded once to T (that rounding is the cache's storage type).
 template <typename T, int D>
-__device__ __forceinline__ void rotate_pair(const Pool& p, int64_t row, int c, uint4& lo_u, uint4& hi_u) {
-  float lo[8], hi[8], cl[8], ch[8], sl[8], sh[8], a[8], b[8];
-  unpack8<T>(lo_u, lo);
-  unpack8<T>(hi_u, hi);
-  load_table8<T>(p, p.cos, row + c * 8, cl);
-  load_table8<T>(p, p.cos, row + D / 2 + c * 8, ch);
-  load_table8<T>(p, p.sin, row + c * 8, sl);
-  load_table8<T>(p, p.sin, row + D / 2 + c * 8, sh);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    a[j] = fmaf(lo[j], cl[j], -hi[j] * sl[j]);
-    b[j] = fmaf(hi[j], ch[j], lo[j] * sh[j]);
+struct Turn {
+  float cl[8], ch[8], sl[8], sh[8];
+  __device__ __forceinline__ void load(const Pool& p, int64_t row, int c) {
+    load_table8<T>(p, p.cos, row + c * 8, cl);
+    load_table8<T>(p, p.cos, row + D / 2 + c * 8, ch);
+    load_table8<T>(p, p.sin, row + c * 8, sl);
+    load_table8<T>(p, p.sin, row + D / 2 + c * 8, sh);
   }
-  lo_u = pack8<T>(a);
-  hi_u = pack8<T>(b);
-}
+  __device__ __forceinline__ void apply(uint4& lo_u, uint4& hi_u) const {
+    float lo[8], hi[8], a[8], b[8];
+    unpack8<T>(lo_u, lo);
+    unpack8<T>(hi_u, hi);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      a[j] = fmaf(lo[j], cl[j], -hi[j] * sl[j]);
+      b[j] = fmaf(hi[j], ch[j], lo[j] * sh[j]);
+    }
+    lo_u = pack8<T>(a);
+    hi_u = pack8<T>(b);
+  }
+};
 
-// D/16 threads per (token, head) row; each moves 16 bytes of either half of the key row and of the value
-// row (or of a query row).  Bound by memory: every row is read once and written once.
+// Bound by memory: every row is read once and written once (1.5 flops a byte).  D/16 threads take kHeads heads of a
+// token, of the keys and values or of the queries, and move 16 bytes of either half of each row: with all of a
+// thread's loads under way at once (128 bytes) and the token's table row used for all its heads.
+constexpr int kAppendThreads = 64, kHeads = 2;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int TPR = D / 16;
   const int64_t b = blockIdx.y;
-  const int64_t idx = ((int64_t)blockIdx.x * 256 + threadIdx.x) / TPR;
+  const uint32_t idx = (blockIdx.x * kAppendThreads + threadIdx.x) / TPR;        // (below 2^31: checked by the host)
   const int c = threadIdx.x % TPR;
-  const int64_t i = idx / p.jobs;
+  const uint32_t i = idx / p.jobs;
   const int job = (int)(idx - i * p.jobs);
   if (i >= p.N) return;
   const int64_t len = p.lengths[b];
@@ -128,46 +136,52 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
     if (!known && job == 0 && c == 0) report(kStatusRope, b, pos, 0);
   }
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  if (job >= p.KV) {                    // a query row
-    const int h = job - p.KV;
-    uint4 lo = zero, hi = zero;
-    if (known) {
-      const T* src = reinterpret_cast<const T*>(p.q) + b * p.q_sb + h * p.q_sh + i * p.q_sn + c * 8;
-      lo = *reinterpret_cast<const uint4*>(src);
-      hi = *reinterpret_cast<const uint4*>(src + D / 2);
-      rotate_pair<T, D>(p.pool, row, c, lo, hi);
+  const bool keys = job < p.kv_jobs;
+  const int h0 = (keys ? job : job - p.kv_jobs) * kHeads, heads = min((keys ? p.KV : p.H) - h0, kHeads);
+  uint4 lo[kHeads], hi[kHeads], vlo[kHeads], vhi[kHeads];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    lo[h] = hi[h] = vlo[h] = vhi[h] = zero;
+    if (!known || h >= heads) continue;
+    const T* src = keys ? reinterpret_cast<const T*>(p.k) + b * p.k_sb + (int64_t)(h0 + h) * p.k_sh + i * p.k_sn + c * 8
+                        : reinterpret_cast<const T*>(p.q) + b * p.q_sb + (int64_t)(h0 + h) * p.q_sh + i * p.q_sn + c * 8;
+    lo[h] = ld_stream16(src);
+    hi[h] = ld_stream16(src + D / 2);
+    if (keys) {
+      src = reinterpret_cast<const T*>(p.v) + b * p.v_sb + (int64_t)(h0 + h) * p.v_sh + i * p.v_sn + c * 8;
+      vlo[h] = ld_stream16(src);
+      vhi[h] = ld_stream16(src + D / 2);
     }
-    T* dst = reinterpret_cast<T*>(p.q_out) + ((b * p.H + h) * p.N + i) * D + c * 8;
-    *reinterpret_cast<uint4*>(dst) = lo;
-    *reinterpret_cast<uint4*>(dst + D / 2) = hi;
-    return;
   }
-  uint4 klo = zero, khi = zero, vlo = zero, vhi = zero;
-  if (known) {
-    const T* ks = reinterpret_cast<const T*>(p.k) + b * p.k_sb + job * p.k_sh + i * p.k_sn + c * 8;
-    const T* vs = reinterpret_cast<const T*>(p.v) + b * p.v_sb + job * p.v_sh + i * p.v_sn + c * 8;
-    klo = *reinterpret_cast<const uint4*>(ks);
-    khi = *reinterpret_cast<const uint4*>(ks + D / 2);
-    vlo = *reinterpret_cast<const uint4*>(vs);
-    vhi = *reinterpret_cast<const uint4*>(vs + D / 2);
-    if (p.pool.cos) rotate_pair<T, D>(p.pool, row, c, klo, khi);
-    const int32_t page = page_of(p.pool, p.pool.table + b * p.pool.table_stride, pos);
+  int32_t page = -1;
+  if (known && keys) {
+    page = page_of(p.pool, p.pool.table + b * p.pool.table_stride, pos);
+    if (page < 0 && job == 0 && c == 0) report(kStatusAppend, b, pos, 0);
+  }
+  if (known && p.pool.cos) {
+    Turn<T, D> turn;
+    turn.load(p.pool, row, c);
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) turn.apply(lo[h], hi[h]);
+  }
+  const int64_t slot = pos & ((1ll << p.pool.shift) - 1);
+  T* copy = reinterpret_cast<T*>(keys ? p.k_out : p.q_out);
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    if (h >= heads) break;
     if (page >= 0) {
-      const int64_t slot = pos & ((1ll << p.pool.shift) - 1);
-      T* kd = reinterpret_cast<T*>(p.pool.k) + page * p.pool.k_page + job * p.pool.k_head + slot * p.pool.k_slot + c * 8;
-      T* vd = reinterpret_cast<T*>(p.pool.v) + page * p.pool.v_page + job * p.pool.v_head + slot * p.pool.v_slot + c * 8;
-      *reinterpret_cast<uint4*>(kd) = klo;
-      *reinterpret_cast<uint4*>(kd + D / 2) = khi;
-      *reinterpret_cast<uint4*>(vd) = vlo;
-      *reinterpret_cast<uint4*>(vd + D / 2) = vhi;
-    } else if (job == 0 && c == 0) {
-      report(kStatusAppend, b, pos, 0);
+      T* kd = reinterpret_cast<T*>(p.pool.k) + page * p.pool.k_page + (int64_t)(h0 + h) * p.pool.k_head + slot * p.pool.k_slot + c * 8;
+      T* vd = reinterpret_cast<T*>(p.pool.v) + page * p.pool.v_page + (int64_t)(h0 + h) * p.pool.v_head + slot * p.pool.v_slot + c * 8;
+      *reinterpret_cast<uint4*>(kd) = lo[h];
+      *reinterpret_cast<uint4*>(kd + D / 2) = hi[h];
+      *reinterpret_cast<uint4*>(vd) = vlo[h];
+      *reinterpret_cast<uint4*>(vd + D / 2) = vhi[h];
     }
-  }
-  if (p.k_out) {
-    T* dst = reinterpret_cast<T*>(p.k_out) + ((b * p.KV + job) * p.N + i) * D + c * 8;
-    *reinterpret_cast<uint4*>(dst) = klo;
-    *reinterpret_cast<uint4*>(dst + D / 2) = khi;
+    if (copy) {
+      T* dst = copy + ((b * (keys ? p.KV : p.H) + h0 + h) * p.N + i) * D + c * 8;
+      *reinterpret_cast<uint4*>(dst) = lo[h];
+      *reinterpret_cast<uint4*>(dst + D / 2) = hi[h];
+    }
   }
 }
 
@@ -1257,17 +1271,17 @@ int moa_paged_append(const moa_paged_append_args* args, moa_stream_t stream) {
   p.k_sb = a.k_sb; p.k_sh = a.k_sh; p.k_sn = a.k_sn; p.v_sb = a.v_sb; p.v_sh = a.v_sh; p.v_sn = a.v_sn;
   p.q_sb = a.q_sb; p.q_sh = a.q_sh; p.q_sn = a.q_sn;
   p.H = (int)a.H; p.KV = (int)a.KV; p.N = a.N;
-  p.jobs = p.KV + (a.q ? p.H : 0);
-  const int64_t blocks = ceil_div64(a.N * p.jobs * (a.D / 16), 256);
-  MOA_REQUIRE(blocks <= 2147483647LL, "paged_append: too many rows");
-  dim3 grid((unsigned)blocks, (unsigned)a.B);
+  p.kv_jobs = (p.KV + kHeads - 1) / kHeads;
+  p.jobs = p.kv_jobs + (a.q ? (p.H + kHeads - 1) / kHeads : 0);
+  MOA_REQUIRE(a.N * p.jobs * (a.D / 16) < (1ll << 31) - kAppendThreads, "paged_append: too many rows");
+  dim3 grid((unsigned)ceil_div64(a.N * p.jobs * (a.D / 16), kAppendThreads), (unsigned)a.B);
   cudaStream_t st = (cudaStream_t)stream;
   if (a.dtype == MOA_F16) {
-    if (a.D == 128) paged_append_kernel<__half, 128><<<grid, 256, 0, st>>>(p);
-    else paged_append_kernel<__half, 64><<<grid, 256, 0, st>>>(p);
+    if (a.D == 128) paged_append_kernel<__half, 128><<<grid, kAppendThreads, 0, st>>>(p);
+    else paged_append_kernel<__half, 64><<<grid, kAppendThreads, 0, st>>>(p);
   } else {
-    if (a.D == 128) paged_append_kernel<__nv_bfloat16, 128><<<grid, 256, 0, st>>>(p);
-    else paged_append_kernel<__nv_bfloat16, 64><<<grid, 256, 0, st>>>(p);
+    if (a.D == 128) paged_append_kernel<__nv_bfloat16, 128><<<grid, kAppendThreads, 0, st>>>(p);
+    else paged_append_kernel<__nv_bfloat16, 64><<<grid, kAppendThreads, 0, st>>>(p);
   }
   MOA_CUDA_CHECK(cudaGetLastError());
   if (a.advance) {
