@@ -206,7 +206,9 @@ __global__ void paged_advance_kernel(int32_t* lengths, const int32_t* counts, in
 // ragged the lengths are, and the cut is computed on the device from `lengths` alone: nothing is planned on the
 // host, and a captured launch stays right when the lengths change.  An item that is cut leaves one partial
 // result (maximum, sum, sum of values) per block; the block that finishes last joins them, in the blocks'
-// order, so results do not depend on timing.  No block waits for another.
+// order, so results do not depend on timing.  No block waits for another.  When there are more items than blocks
+// and all are short, the line is cut into a part per warp, of whole items: nothing is shared between warps then
+// and an item costs no barriers (3840 items of up to 34 tokens: @@SOLO@@).
 //
 // Loads.  The warps of a block take the units of a segment in turn.  Each warp runs its own ring of kStages
 // units in shared memory, filled by a cursor that runs ahead of the arithmetic, over the ends of items too, so the
@@ -223,10 +225,10 @@ __global__ void paged_advance_kernel(int32_t* lengths, const int32_t* counts, in
 //
 // The fused step's new token is where one warp of the block that ends the item starts from (its score is the first
 // maximum, its value the first sum); it is stored into its page at the same time and read from no page.
-constexpr int kWarps = 4, kDecodeThreads = kWarps * 32;
 constexpr int kPerSm = 2;                   // resident blocks per SM
 constexpr int kUnit = 16;                   // positions of a unit (k of the second product)
-constexpr int kItemCost = 16;               // an item's epilogue, in units
+constexpr int kItemCost = 16, kSoloCost = 2;      // an item's epilogue, in units
+constexpr int kSoloTokens = 256;            // longest sequence for warps on their own
 constexpr int kMinUnits = 8;                // least share of a block: fewer blocks work when there is less
 constexpr int kJoin = 18;                   // partial results joined at once
 constexpr int kMaxParts = kJoin * kJoin;    // two levels of joining
@@ -312,16 +314,16 @@ struct Span {
   __device__ __forceinline__ bool sees_last() const { return n > 0 && (sink == n || from < n); }
 };
 
-// The line in equal parts, one per block.
+// The line in equal parts, one per team (a block, or a warp on its own).
 struct Cut {
   int64_t total, each;                      // units of the line; of a part, rounded down
   int parts, rest;                          // total = each * parts + rest
-  __device__ __forceinline__ Cut(int64_t t, int most) : total(t) {
-    parts = (int)min(max(t / kMinUnits, (int64_t)1), (int64_t)most);
+  __device__ __forceinline__ Cut(int64_t t, int most, int least) : total(t) {
+    parts = (int)min(max(t / least, (int64_t)1), (int64_t)most);
     each = t / parts;
     rest = (int)(t - each * parts);
   }
-  __device__ __forceinline__ int64_t begin(int c) const { return each * c + rest * c / parts; }
+  __device__ __forceinline__ int64_t begin(int c) const { return each * c + (int64_t)rest * c / parts; }
   // The last c with begin(c) <= x.
   __device__ __forceinline__ int part_of(int64_t x) const {
     int c = min((int)((float)x / (float)total * parts), parts - 1);
@@ -333,22 +335,32 @@ struct Cut {
   }
 };
 
-// A walk over the items of a block's part [lo, hi) of the line.
+// A walk over the items of a part [lo, hi) of the line: of those that begin in it when warps are on their own (`solo`),
+// of all that reach into it else.
+struct Part {
+  int64_t lo, hi;
+};
+template <bool SOLO>
 struct Cursor {
+  static constexpr int kCost = SOLO ? kSoloCost : kItemCost;
   int b, kh, tile;
   int n;                                    // tokens of sequence b
   Span span;
   int64_t at;                               // where the item begins on the line
   int u0, u1;                               // the units of the item that are in the part
-  __device__ __forceinline__ void enter(const Sizes& s, int64_t lo, int64_t hi) {
+  __device__ __forceinline__ void enter(const Sizes& s, const Part& part) {
     span = Span(s, n, kh);
-    u0 = (int)min(max(lo - at, (int64_t)0), (int64_t)span.units);
-    u1 = (int)min(hi - at, (int64_t)span.units);
+    u0 = 0;
+    u1 = span.units;
+    if (!SOLO) {
+      u0 = (int)min(max(part.lo - at, (int64_t)0), (int64_t)u1);
+      u1 = (int)min(part.hi - at, (int64_t)u1);
+    }
   }
   // To the next item; false when it is not in the part.
-  __device__ __forceinline__ bool next(const Sizes& s, int64_t lo, int64_t hi) {
-    at += span.units + kItemCost;
-    if (at >= hi) return false;
+  __device__ __forceinline__ bool next(const Sizes& s, const Part& part) {
+    at += span.units + kCost;
+    if (at >= part.hi) return false;
     if (++tile == s.p.tiles) {
       tile = 0;
       if (++kh == s.p.KV) {
@@ -357,7 +369,7 @@ struct Cursor {
         n = s.tokens(b);
       }
     }
-    enter(s, lo, hi);
+    enter(s, part);
     return true;
   }
 };
@@ -450,22 +462,41 @@ __device__ __forceinline__ float joined(float hi, float lo) { return isinf(hi) ?
 
 // A unit's keys (and values) are D/64 panels of 16 rows of 128 bytes, 16-byte chunk c of row r at c ^ (r % 8): TMA's
 // 128-byte swizzle, which ldmatrix reads without bank conflicts.
-template <int D, int MT>
+template <int D, int MT, bool SOLO>
 struct Layout {
+  static constexpr int kWarps = 4;
+  static constexpr int kThreads = kWarps * 32;
   static constexpr int kPanelBytes = kUnit * 128, kTileBytes = kUnit * D * 2, kStageBytes = 2 * kTileBytes;
-  static constexpr int kStages = D == 128 ? 2 : 4;
+  static constexpr int kStages = D == 64 ? 4 : 2;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kJoinBytes = kWarps * 8 * D * 4;                // a head's row: value d at d ^ 4 * head
   // what an item needs: queries (rows padded by 16 bytes), the new token's key, value, cos and sin, its page
   static constexpr int kQPitch = D * 2 + 16, kKey = 8 * MT * kQPitch, kValue = kKey + D * 2, kCos = kValue + D * 2,
                        kSin = kCos + D * 4, kPage = kSin + D * 4, kItemBytes = kPage + 16;
   static constexpr int kLowBytes = 8 * MT * kQPitch;                   // what rotated queries have beyond 16 bits
-  static constexpr int kBarBytes = kWarps * kStages * 8, kMaskBytes = kWarps * kStages * 4;
-  static constexpr int kBytes = 1024 + kRing + kJoinBytes + 2 * kItemBytes + kLowBytes + kBarBytes + kMaskBytes + 2 * kWarps * 8 * 4 + 128 +
-                                kCached * 12;
-  static_assert(kPerSm * (kBytes + 1024) <= 233472, "shared memory");
+  static constexpr int kTeamBytes = 2 * kItemBytes + kLowBytes;
+  // shared memory: the ring, its barriers and masks, maxima and sums of the warps, the scan, lengths and spans, the
+  // teams' (and behind a block's the join buffer)
+  static constexpr int kBar = kRing, kMask = kBar + kWarps * kStages * 8, kMax = kMask + kWarps * kStages * 4,
+                       kScan = kMax + 2 * kWarps * 8 * 4, kLen = kScan + 128 + (SOLO ? kThreads * 8 : 0),
+                       kTeams = kLen + kCached * 12;
+  static constexpr int kBytes = 1024 + kTeams + (SOLO ? kWarps * kTeamBytes : kTeamBytes + kJoinBytes);
+  static constexpr bool kFits = kPerSm * (kBytes + 1024) <= 233472;
+  static_assert((SOLO || kFits) && kTeams % 16 == 0, "shared memory");
   static __device__ __forceinline__ uint32_t at(int row, int chunk) {
     return (chunk >> 3) * kPanelBytes + row * 128 + (((chunk ^ row) & 7) << 4);
+  }
+};
+
+// A block, or a warp on its own.
+template <bool SOLO, int WARPS>
+struct Team {
+  static constexpr int warps = SOLO ? 1 : WARPS, size = warps * 32;
+  int rank, warp;                                  // thread of the team, warp of the team
+  __device__ __forceinline__ Team() : rank(SOLO ? threadIdx.x & 31 : threadIdx.x), warp(SOLO ? 0 : threadIdx.x >> 5) {}
+  __device__ __forceinline__ void sync() const {
+    if (SOLO) __syncwarp();
+    else __syncthreads();
   }
 };
 
@@ -481,35 +512,37 @@ __device__ __forceinline__ void store_out4(const DecodeParams& p, int b, int h, 
   else *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + off) = make_uint2(Cvt<T>::pack(O.x, O.y), Cvt<T>::pack(O.z, O.w));
 }
 
-// Fetches what an item needs into its buffer, with cp.async; called by the whole block.
-template <typename T, int D, int MT>
-__device__ __forceinline__ void fetch_item(const DecodeParams& p, const Cursor& c, bool fresh, uint32_t buf) {
-  using L = Layout<D, MT>;
+// Fetches what an item needs into its buffer, with cp.async; called by the whole team.
+template <typename T, int D, int MT, typename TEAM, typename CURSOR>
+__device__ __forceinline__ void fetch_item(const DecodeParams& p, const TEAM& team, const CURSOR& c, bool fresh, uint32_t buf) {
+  using L = Layout<D, MT, false>;            // (the same for both)
   constexpr int CPR = D / 8;                       // 16-byte chunks per row
-  const int tid = threadIdx.x;
   const int h0 = c.kh * p.G + c.tile * 8 * MT, heads = min(p.G - c.tile * 8 * MT, 8 * MT);
 #pragma unroll
-  for (int i = tid; i < 8 * MT * CPR; i += kDecodeThreads) {
+  for (int i = team.rank; i < 8 * MT * CPR; i += team.size) {
     const int row = i / CPR, chunk = i % CPR;
     const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)c.b * p.q_sb + (int64_t)(h0 + min(row, heads - 1)) * p.q_sh;
     cp_async16(buf + row * L::kQPitch + chunk * 16, src + chunk * 8, row < heads);
   }
   if (fresh) {
     const int64_t pos = c.n - 1;
-    if (tid < 2 * CPR) {
-      const int chunk = tid % CPR;
-      const T* src = tid < CPR ? reinterpret_cast<const T*>(p.k_new) + c.b * p.k_sb + c.kh * p.k_sh
-                               : reinterpret_cast<const T*>(p.v_new) + c.b * p.v_sb + c.kh * p.v_sh;
-      cp_async16(buf + (tid < CPR ? L::kKey : L::kValue) + chunk * 16, src + chunk * 8, true);
+    if (team.rank < 2 * CPR) {
+      const int chunk = team.rank % CPR;
+      const T* src = team.rank < CPR ? reinterpret_cast<const T*>(p.k_new) + c.b * p.k_sb + c.kh * p.k_sh
+                                     : reinterpret_cast<const T*>(p.v_new) + c.b * p.v_sb + c.kh * p.v_sh;
+      cp_async16(buf + (team.rank < CPR ? L::kKey : L::kValue) + chunk * 16, src + chunk * 8, true);
     }
     const int64_t row = p.pool.cos ? rope_row(p.pool, c.b, 0, pos) : -1;
     const int cells = p.pool.rope_f32 ? 4 : 2, chunks = D * cells / 16;      // bytes of a table's value
-    if (row >= 0 && tid >= kDecodeThreads - 2 * chunks) {
-      const int i = tid - (kDecodeThreads - 2 * chunks), chunk = i % chunks;
-      const char* src = reinterpret_cast<const char*>(i < chunks ? p.pool.cos : p.pool.sin) + row * cells;
-      cp_async16(buf + (i < chunks ? L::kCos : L::kSin) + chunk * 16, src + chunk * 16, true);
+    if (row >= 0) {
+#pragma unroll 1
+      for (int i = team.size - 1 - team.rank; i < 2 * chunks; i += team.size) {
+        const int chunk = i % chunks;
+        const char* src = reinterpret_cast<const char*>(i < chunks ? p.pool.cos : p.pool.sin) + row * cells;
+        cp_async16(buf + (i < chunks ? L::kCos : L::kSin) + chunk * 16, src + chunk * 16, true);
+      }
     }
-    if (tid == 0) cp_async4(buf + L::kPage, p.pool.table + (int64_t)c.b * p.pool.table_stride + (pos >> p.pool.shift));
+    if (team.rank == 0) cp_async4(buf + L::kPage, p.pool.table + (int64_t)c.b * p.pool.table_stride + (pos >> p.pool.shift));
   }
   cp_async_commit();
 }
@@ -521,13 +554,14 @@ __device__ __forceinline__ float2 table2(const unsigned char* row, int d, bool f
   return Cvt<T>::unpack(*reinterpret_cast<const uint32_t*>(row + d * 2));
 }
 
-// The item's queries are rotated in their buffer, by the whole block: what fits T stays there, the rest goes to `low`.
-template <typename T, int D, int MT>
-__device__ __forceinline__ void turn_queries(const DecodeParams& p, unsigned char* item, unsigned char* low, int heads) {
-  using L = Layout<D, MT>;
+// The item's queries are rotated in their buffer, by the whole team: what fits T stays there, the rest goes to `low`.
+template <typename T, int D, int MT, typename TEAM>
+__device__ __forceinline__ void turn_queries(const DecodeParams& p, const TEAM& team, unsigned char* item, unsigned char* low,
+                                             int heads) {
+  using L = Layout<D, MT, false>;            // (the same for both)
   const bool f32 = p.pool.rope_f32;
 #pragma unroll 1
-  for (int i = threadIdx.x; i < heads * (D / 4); i += kDecodeThreads) {
+  for (int i = team.rank; i < heads * (D / 4); i += team.size) {
     const int head = i / (D / 4), d = i % (D / 4) * 2;       // a pair of coordinates of either half
     uint32_t* q = reinterpret_cast<uint32_t*>(item + head * L::kQPitch);
     uint32_t* r = reinterpret_cast<uint32_t*>(low + head * L::kQPitch);
@@ -542,7 +576,7 @@ __device__ __forceinline__ void turn_queries(const DecodeParams& p, unsigned cha
 // The new token's key is rotated in its buffer (a warp's work).
 template <typename T, int D, int MT>
 __device__ __forceinline__ void turn_key(const DecodeParams& p, unsigned char* item) {
-  using L = Layout<D, MT>;
+  using L = Layout<D, MT, false>;            // (the same for both)
   const int d = (threadIdx.x & 31) * 2;            // a pair of coordinates of either half
   const bool f32 = p.pool.rope_f32;
   if (d < D / 2) {
@@ -559,7 +593,7 @@ __device__ __forceinline__ void turn_key(const DecodeParams& p, unsigned char* i
 // The new token's rows go into their page (a warp's work).
 template <typename T, int D, int MT>
 __device__ __forceinline__ void store_new(const DecodeParams& p, const unsigned char* item, int kh, int slot, int page) {
-  using L = Layout<D, MT>;
+  using L = Layout<D, MT, false>;            // (the same for both)
   const int lane = threadIdx.x & 31, chunk = lane % (D / 8);
   if (lane >= 2 * (D / 8)) return;
   if (lane < D / 8) {
@@ -577,7 +611,7 @@ __device__ __forceinline__ void store_new(const DecodeParams& p, const unsigned 
 template <typename T, int D, int MT>
 __device__ __noinline__ uint32_t load_rows(const DecodeParams& p, int b, int kh, int x, int32_t page, uint32_t present,
                                            uint32_t dst) {
-  using L = Layout<D, MT>;
+  using L = Layout<D, MT, false>;            // (the same for both)
   constexpr int LPR = D / 8, RPI = 32 / LPR;       // lanes per row, rows per load instruction
   const int lane = threadIdx.x & 31;
   const int pos = x * 16 + (lane & 15);
@@ -609,9 +643,10 @@ __device__ __noinline__ uint32_t load_rows(const DecodeParams& p, int b, int kh,
 // Joins the records that parts c0 .. c1 of the line left of one item (`heads` query heads from h0 of sequence b);
 // called by every block that left one.  kJoin neighbours are joined by the last of them, their results by the last
 // of those that joined, and so on; no block waits.
-template <typename T, int D>
+template <typename T, int D, int MT>
 __device__ __noinline__ void join_parts(const DecodeParams& p, int c0, int c1, int b, int h0, int heads, float* scratch,
                                         int* flag) {
+  constexpr int kThreads = Layout<D, MT, false>::kThreads;
   const int tid = threadIdx.x;
   float* weight = scratch;                         // (record, head); then by head
   float* top = scratch + kJoin * kRecHeads;
@@ -680,12 +715,12 @@ __device__ __noinline__ void join_parts(const DecodeParams& p, int c0, int c1, i
     }
     __syncthreads();
 #pragma unroll 1
-    for (int e = tid * 4; e < heads * D; e += kDecodeThreads * 4) {
+    for (int e = tid * 4; e < heads * D; e += kThreads * 4) {
       const int head = e / D;
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
       for (int i0 = 0; i0 < count; i0 += kAtOnce) {
-        if (e >= kDecodeThreads * 4 || i0 > 0) load(e, i0);
+        if (e >= kThreads * 4 || i0 > 0) load(e, i0);
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i)
           if (i0 + i < count) {
@@ -709,41 +744,42 @@ __device__ __noinline__ void join_parts(const DecodeParams& p, int c0, int c1, i
   }
 }
 
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k,
-                                                                              const __grid_constant__ CUtensorMap map_v,
-                                                                              const __grid_constant__ DecodeParams p) {
-  using L = Layout<D, MT>;
-  constexpr int kStages = L::kStages;
+// SOLO: a team is a warp, and items are not cut.
+template <typename T, int D, int MT, bool SOLO>
+__global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
+    paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                        const __grid_constant__ DecodeParams p) {
+  using L = Layout<D, MT, SOLO>;
+  constexpr int kStages = L::kStages, kWarps = L::kWarps, kThreads = L::kThreads, kCost = Cursor<SOLO>::kCost;
   constexpr int KS = D / 16;                       // k steps of the first product, pairs of n tiles of the second
   extern __shared__ unsigned char smem_raw[];      // the swizzle goes by the address: panels start at multiples of 1024
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  float* sm_o = reinterpret_cast<float*>(smem + L::kRing);
-  unsigned char* sm_item = smem + L::kRing + L::kJoinBytes;
-  unsigned char* sm_low = sm_item + 2 * L::kItemBytes;
-  unsigned char* sm_bar = sm_low + L::kLowBytes;
-  uint32_t* sm_mask = reinterpret_cast<uint32_t*>(sm_bar + L::kBarBytes);
-  float* sm_m = reinterpret_cast<float*>(sm_mask + kWarps * kStages);
+  float* sm_m = reinterpret_cast<float*>(smem + L::kMax);
   float* sm_l = sm_m + kWarps * 8;
-  int64_t* sm_scan = reinterpret_cast<int64_t*>(sm_l + kWarps * 8);   // warp sums, then {b, item of b, at} of the part
-  int* sm_flag = reinterpret_cast<int*>(sm_scan + 12);
-  int* sm_len = reinterpret_cast<int*>(sm_scan + 16);
+  int64_t* sm_sum = reinterpret_cast<int64_t*>(smem + L::kScan);      // by warp; then where the block's part begins
+  int64_t* sm_before = sm_sum + 16;                // (SOLO) by thread
+  int* sm_flag = reinterpret_cast<int*>(sm_sum + 12);
+  int* sm_len = reinterpret_cast<int*>(smem + L::kLen);
   int2* sm_span = reinterpret_cast<int2*>(sm_len + kCached);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Sizes sizes = {p, sm_len, sm_span};
+  const Team<SOLO, kWarps> team;
+  unsigned char* sm_item = smem + L::kTeams + (SOLO ? warp * L::kTeamBytes : 0);
+  unsigned char* sm_low = sm_item + 2 * L::kItemBytes;
+  float* sm_o = reinterpret_cast<float*>(smem + L::kTeams + L::kTeamBytes);
 
   if (tid == 0 && p.tma) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
   }
-  // ---- the line: its length, and where this block's part begins
+  // ---- the line: its length, and where this team's part begins
 #pragma unroll 1
-  for (int b = tid; b < min(p.B, kCached); b += kDecodeThreads) sm_len[b] = p.lengths[b];
+  for (int b = tid; b < min(p.B, kCached); b += kThreads) sm_len[b] = p.lengths[b];
   if (p.sink)
 #pragma unroll 1
-    for (int kh = tid; kh < min(p.KV, kCached); kh += kDecodeThreads) sm_span[kh] = Sizes::clamped(p.sink[kh], p.local[kh]);
-  const uint32_t bars = (uint32_t)__cvta_generic_to_shared(sm_bar) + warp * kStages * 8;
+    for (int kh = tid; kh < min(p.KV, kCached); kh += kThreads) sm_span[kh] = Sizes::clamped(p.sink[kh], p.local[kh]);
+  const uint32_t bars = (uint32_t)__cvta_generic_to_shared(smem + L::kBar) + warp * kStages * 8;
   if (lane < kStages) {
     bar_init(bars + lane * 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -751,10 +787,10 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
   __syncthreads();
   // in rows of items that cost the same: a sequence's, or with spans a (sequence, key head)'s
   const int per_seq = p.sink ? p.KV : 1, items = p.sink ? p.tiles : p.KV * p.tiles;
-  const uint32_t rows = (uint32_t)p.B * per_seq, per = (rows - 1) / kDecodeThreads + 1;      // (B, KV < 2^16)
+  const uint32_t rows = (uint32_t)p.B * per_seq, per = (rows - 1) / kThreads + 1;      // (B, KV < 2^16)
   const uint32_t row_lo = min(tid * per, rows), row_hi = row_lo + min(per, rows - row_lo);
   const int b_lo = (int)(row_lo / per_seq), kh_lo = (int)(row_lo - (uint32_t)b_lo * per_seq);
-  auto cost_of = [&](int b, int kh) { return Span(sizes, sizes.tokens(b), kh).units + kItemCost; };
+  auto cost_of = [&](int b, int kh) { return Span(sizes, sizes.tokens(b), kh).units + kCost; };
   int64_t mine = 0;
   int b_at = b_lo, kh_at = kh_lo;
 #pragma unroll 4
@@ -771,59 +807,81 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
     const int64_t other = __shfl_up_sync(0xffffffffu, before, off);
     if (lane >= off) before += other;
   }
-  if (lane == 31) sm_scan[warp] = before;
+  if (lane == 31) sm_sum[warp] = before;
   before -= mine;
   __syncthreads();
   int64_t total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += sm_scan[w];
-    total += sm_scan[w];
+    if (w < warp) before += sm_sum[w];
+    total += sm_sum[w];
   }
-  const Cut cut(total, gridDim.x);
-  const int block = blockIdx.x;
+  const Cut cut(total, SOLO ? gridDim.x * kWarps : gridDim.x, SOLO ? 1 : kMinUnits);
+  const int number = SOLO ? warp * gridDim.x + blockIdx.x : blockIdx.x;
+  if (SOLO) {                                      // (the warps of a block look for different parts)
+    sm_before[tid] = before;
+    __syncthreads();
+  }
 
-  if (block < cut.parts) {
-    const int64_t lo = cut.begin(block), hi = cut.begin(block + 1);
-    if (before <= lo && lo < before + mine) {      // one thread: the part begins in one of its rows
-      int64_t at = before;
-      int b = b_lo, kh = kh_lo, cost;
+  if (number < cut.parts) {
+    const Part part = {cut.begin(number), cut.begin(number + 1)};
+    Cursor<SOLO> cur;
+    // from the first of a thread's rows (b, kh, at) on to the row, and the item of it, in which the part begins
+    auto walk = [&](int b, int kh, int64_t at) {
+      int cost;
 #pragma unroll 1
       for (;;) {
         cost = cost_of(b, kh);
         const int64_t end = at + (int64_t)items * cost;
-        if (lo < end) break;
+        if (part.lo < end) break;
         at = end;
         if (++kh == per_seq) {
           kh = 0;
           ++b;
         }
       }
-      const int item = (int)((lo - at) / cost);
-      sm_scan[8] = b;
-      sm_scan[9] = (int64_t)(kh + item / p.tiles) << 32 | (item % p.tiles);
-      sm_scan[10] = at + (int64_t)item * cost;
+      const int item = (int)((part.lo - at) / cost);
+      cur.b = b;
+      cur.kh = kh + item / p.tiles;
+      cur.tile = item % p.tiles;
+      cur.at = at + (int64_t)item * cost;
+    };
+    if (SOLO) {
+      int j = 0;                                   // threads whose rows begin at or before the part
+#pragma unroll
+      for (int k = 0; k < kThreads; k += 32)
+        j += __popc(__ballot_sync(0xffffffffu, (k + lane) * per < rows && sm_before[k + lane] <= part.lo));
+      const uint32_t row = (j - 1) * per;
+      walk((int)(row / per_seq), (int)(row % per_seq), sm_before[j - 1]);
+    } else {
+      if (before <= part.lo && part.lo < before + mine) {      // one thread
+        walk(b_lo, kh_lo, before);
+        sm_sum[8] = cur.b;
+        sm_sum[9] = (int64_t)cur.kh << 32 | cur.tile;
+        sm_sum[10] = cur.at;
+      }
+      __syncthreads();
+      cur.b = (int)sm_sum[8];
+      cur.kh = (int)(sm_sum[9] >> 32);
+      cur.tile = (int)sm_sum[9];
+      cur.at = sm_sum[10];
     }
-    __syncthreads();
-    Cursor cur;
-    cur.b = (int)sm_scan[8];
-    cur.kh = (int)(sm_scan[9] >> 32);
-    cur.tile = (int)sm_scan[9];
-    cur.at = sm_scan[10];
     cur.n = sizes.tokens(cur.b);
-    cur.enter(sizes, lo, hi);
+    cur.enter(sizes, part);
+    bool any = true;
+    if (SOLO && cur.at < part.lo) any = cur.next(sizes, part);      // it begins in the part before
     const uint32_t item_at = (uint32_t)__cvta_generic_to_shared(sm_item);
-    fetch_item<T, D, MT>(p, cur, sizes.fresh(cur.b), item_at);
+    if (any) fetch_item<T, D, MT>(p, team, cur, sizes.fresh(cur.b), item_at);
 
     // ---- loads: a cursor of this warp's own
-    Cursor ld = cur;
-    bool ld_more = true;
-    int ld_u = ld.u0 + warp;
+    Cursor<SOLO> ld = cur;
+    bool ld_more = any;
+    int ld_u = ld.u0 + team.warp;
     int ld_x = 0;                                  // aligned unit that is loaded next, its attended positions and its page
     uint32_t ld_mask = 0;                          // (of position lane % 16 when pages are smaller than a unit)
     int32_t ld_page = -1;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * kStages * L::kStageBytes;
-    uint32_t* my_mask = sm_mask + warp * kStages;
+    uint32_t* my_mask = reinterpret_cast<uint32_t*>(smem + L::kMask) + warp * kStages;
 
     auto ld_look = [&]() {                         // look up the next unit's page
       ld_x = ld.span.unit(ld_u);
@@ -839,11 +897,11 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
     };
     auto ld_seek = [&]() {                         // to the next unit of this warp
       while (ld_u >= ld.u1) {
-        if (!ld.next(sizes, lo, hi)) {
+        if (!ld.next(sizes, part)) {
           ld_more = false;
           return;
         }
-        ld_u = ld.u0 + warp;
+        ld_u = ld.u0 + team.warp;
       }
       ld_look();
     };
@@ -867,13 +925,13 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
             bar_arrive(bar);
           }
         }
-        ld_u += kWarps;
+        ld_u += team.warps;
         ld_seek();
       }
       cp_async_commit();                           // a group per call, empty or not: they are counted
     };
 
-    ld_seek();
+    if (any) ld_seek();
 #pragma unroll 1
     for (int s = 0; s < kStages; ++s) ld_issue(s);
 
@@ -882,37 +940,37 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
     int stage = 0, buf = 0;
     uint32_t parity = 0;
     bool waiting = true;                           // until a wait runs out
-    for (bool more = true; more; buf ^= 1) {
-      Cursor next = cur;
-      more = next.next(sizes, lo, hi);
+    for (bool more = any; more; buf ^= 1) {
+      Cursor<SOLO> next = cur;
+      more = next.next(sizes, part);
       cp_async_wait_all();                         // the item's own data; its buffers were fetched an item ago
-      __syncthreads();                             // (and the item before is through with the join buffer)
-      if (more) fetch_item<T, D, MT>(p, next, sizes.fresh(next.b), item_at + (buf ^ 1) * L::kItemBytes);
+      team.sync();                                 // (and the item before is through with the join buffer)
+      if (more) fetch_item<T, D, MT>(p, team, next, sizes.fresh(next.b), item_at + (buf ^ 1) * L::kItemBytes);
 
       unsigned char* item = sm_item + buf * L::kItemBytes;
       const int h0 = cur.kh * p.G + cur.tile * 8 * MT;                   // first query head of the item
       const int heads = min(p.G - cur.tile * 8 * MT, 8 * MT);
       const int units = cur.span.units;
-      const bool owner = cur.at >= lo;             // the item begins in this part
+      const bool owner = cur.at >= part.lo;        // the item begins in this part
       const bool ends = units == 0 ? owner : cur.u0 < cur.u1 && cur.u1 == units;
       const bool fresh = sizes.fresh(cur.b);
       const bool turn = fresh && p.pool.cos && rope_row(p.pool, cur.b, 0, cur.n - 1) >= 0;
       if (turn) {
-        turn_queries<T, D, MT>(p, item, sm_low, heads);
-        if (warp == kWarps - 1 && ends) turn_key<T, D, MT>(p, item);
-        __syncthreads();
+        turn_queries<T, D, MT>(p, team, item, sm_low, heads);
+        if (team.warp == team.warps - 1 && ends) turn_key<T, D, MT>(p, item);
+        team.sync();
       }
       bool with_new = false;                       // this block attends the new token
       if (fresh && ends) {
         const int page = *reinterpret_cast<const int*>(item + L::kPage);
         const bool placed = (uint32_t)page < (uint32_t)p.pool.num_pages && (turn || !p.pool.cos);
         with_new = placed && cur.span.sees_last();
-        if (warp == kWarps - 1 && cur.tile == 0) {
+        if (team.warp == team.warps - 1 && cur.tile == 0) {
           if (placed) store_new<T, D, MT>(p, item, cur.kh, (cur.n - 1) & ((1 << p.pool.shift) - 1), page);
           else if (lane == 0) report(p.pool.cos && !turn ? kStatusRope : kStatusAppend, cur.b, cur.n - 1, cur.kh);
         }
       }
-      if (owner && cur.kh == 0 && cur.tile == 0 && tid == 0) {
+      if (owner && cur.kh == 0 && cur.tile == 0 && team.rank == 0) {
         const int64_t wanted = (int64_t)sizes.length(cur.b) + (p.k_new ? 1 : 0);
         if (wanted > p.capacity) report(kStatusLength, cur.b, wanted, 0);
       }
@@ -920,7 +978,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
       if (units == 0) {                            // nothing to attend (a part's first item may not be its own)
         if (owner)
 #pragma unroll 1
-          for (int i = tid * 4; i < heads * D; i += kDecodeThreads * 4)
+          for (int i = team.rank * 4; i < heads * D; i += team.size * 4)
             store_out4<T>(p, cur.b, h0 + i / D, i % D, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
       } else if (cur.u0 < cur.u1) {
         float m[MT], l[MT], acc[MT][D / 8][4];
@@ -933,7 +991,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[mt][j][e] = 0.f;
         }
-        if (cur.u0 + warp < cur.u1) {
+        if (cur.u0 + team.warp < cur.u1) {
           // query fragments: rows 0-7 the heads, rows 8-15 what a rotated query has beyond 16 bits
           uint32_t qa[MT][KS][4];
 #pragma unroll
@@ -954,7 +1012,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
               }
             }
           }
-          if (with_new && warp == 0) {             // start from the new token: column 0 of a tile of keys, weight 1
+          if (with_new && team.warp == 0) {             // start from the new token: column 0 of a tile of keys, weight 1
             const uint32_t* key = reinterpret_cast<const uint32_t*>(item + L::kKey);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
@@ -981,7 +1039,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
           const uint32_t k_at = ((mi >> 1) * 8 + r8) * 128 + (((mi & 1) ^ r8) << 4);
           const uint32_t v_at = L::kTileBytes + ((mi & 1) * 8 + r8) * 128 + (((mi >> 1) ^ r8) << 4);
 #pragma unroll 1
-          for (int u = cur.u0 + warp; u < cur.u1; u += kWarps) {
+          for (int u = cur.u0 + team.warp; u < cur.u1; u += team.warps) {
             if (opaque(waiting)) waiting = __all_sync(0xffffffffu, bar_wait(bars + stage * 8, parity));
             const uint32_t base = ring + stage * L::kStageBytes;
             const uint32_t present = my_mask[stage];
@@ -1062,10 +1120,32 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
           }
         }
 
+        if (SOLO) {                           // ---- a warp's own result
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            float sum = l[mt];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (mt * 8 + g >= heads) continue;
+            const float f = sum == 0.f ? 0.f : 1.f / sum;
+            const int64_t off = (int64_t)cur.b * p.o_sb + (int64_t)(h0 + mt * 8 + g) * p.o_sh + 2 * t;
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) {
+              float x = joined(acc[mt][j][0], acc[mt][j][2]), y = joined(acc[mt][j][1], acc[mt][j][3]);
+              x = sum == 0.f ? 0.f : x * f;
+              y = sum == 0.f ? 0.f : y * f;
+              if (p.out_f32) *reinterpret_cast<float2*>(reinterpret_cast<float*>(p.out) + off + j * 8) = make_float2(x, y);
+              else *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + off + j * 8) = Cvt<T>::pack(x, y);
+            }
+          }
+          if (more) cur = next;
+          continue;
+        }
+
         // ---- the warps' results joined
         const bool whole = cur.u0 == 0 && cur.u1 == units;
         const int nw = min(kWarps, cur.u1 - cur.u0);
-        float* rec = p.records + (int64_t)(2 * block + (owner ? 1 : 0)) * kRecFloats;
+        float* rec = p.records + (int64_t)(2 * blockIdx.x + (owner ? 1 : 0)) * kRecFloats;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           const int here = min(heads - mt * 8, 8);
@@ -1089,7 +1169,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
           }
           __syncthreads();
 #pragma unroll 1
-          for (int i = tid * 4; i < here * D; i += kDecodeThreads * 4) {
+          for (int i = tid * 4; i < here * D; i += kThreads * 4) {
             const int head = i / D, d = i % D;
             float M = -INFINITY, Ls = 0.f;
 #pragma unroll
@@ -1114,7 +1194,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
           }
         }
         if (!whole)
-          join_parts<T, D>(p, cut.part_of(cur.at), cut.part_of(cur.at + units - 1), cur.b, h0, heads, sm_o, sm_flag);
+          join_parts<T, D, MT>(p, cut.part_of(cur.at), cut.part_of(cur.at + units - 1), cur.b, h0, heads, sm_o, sm_flag);
       }
       if (more) cur = next;
     }
@@ -1130,7 +1210,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kPerSm) paged_decode_kernel(co
     __syncthreads();
     if (*sm_flag)
 #pragma unroll 1
-      for (int b = tid; b < p.B; b += kDecodeThreads) {
+      for (int b = tid; b < p.B; b += kThreads) {
         const int len = p.lengths[b];
         if (len >= 0 && len < 2147483647) p.lengths[b] = len + 1;
       }
@@ -1175,16 +1255,18 @@ bool make_map(CUtensorMap* map, const void* base, const DecodeParams& p, int64_t
   const cuuint32_t box[4] = {64, kUnit, 1, 1}, step[4] = {1, 1, 1, 1};
   return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
                 dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                // rows of 128 bytes apart from one another: a neighbour's would be fetched for nothing
+                D == 64 && slot != D ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D, int MT, bool SOLO>
 int launch_decode(DecodeParams& p, int grid, cudaStream_t stream) {
+  using L = Layout<D, MT, SOLO>;
   static bool ready[kMaxDevices];
   int dev = 0;
   MOA_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= kMaxDevices || !ready[dev]) {
-    MOA_CUDA_CHECK(cudaFuncSetAttribute(paged_decode_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D, MT>::kBytes));
+    MOA_CUDA_CHECK(cudaFuncSetAttribute(paged_decode_kernel<T, D, MT, SOLO>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
     if (dev >= 0 && dev < kMaxDevices) ready[dev] = true;
   }
   CUtensorMap map_k, map_v;
@@ -1192,9 +1274,17 @@ int launch_decode(DecodeParams& p, int grid, cudaStream_t stream) {
   p.tma = p.pool.shift >= 4 &&      // a unit lies in one page
           make_map(&map_k, p.pool.k, p, p.pool.k_page, p.pool.k_head, p.pool.k_slot, D, bf16) &&
           make_map(&map_v, p.pool.v, p, p.pool.v_page, p.pool.v_head, p.pool.v_slot, D, bf16);
-  paged_decode_kernel<T, D, MT><<<grid, kDecodeThreads, Layout<D, MT>::kBytes, stream>>>(map_k, map_v, p);
+  paged_decode_kernel<T, D, MT, SOLO><<<grid, L::kThreads, L::kBytes, stream>>>(map_k, map_v, p);
   MOA_CUDA_CHECK(cudaGetLastError());
   return MOA_OK;
+}
+template <typename T, int D, int MT>
+int launch_decode(DecodeParams& p, int grid, cudaStream_t stream) {
+  // Warps on their own where no sequence can be long (the page table reaches kSoloTokens at most) and blocks would have
+  // to take several items each: @@RULE@@
+  if constexpr (Layout<D, MT, true>::kFits)        // (16 heads of 128: no room)
+    if (p.capacity <= kSoloTokens && (int64_t)p.B * p.KV * p.tiles > grid) return launch_decode<T, D, MT, true>(p, grid, stream);
+  return launch_decode<T, D, MT, false>(p, grid, stream);
 }
 template <typename T>
 int launch_decode(DecodeParams& p, int D, int grid, cudaStream_t stream) {
