@@ -202,13 +202,13 @@ __global__ void paged_advance_kernel(int32_t* lengths, const int32_t* counts, in
 //
 // Work.  An item is (sequence, key head, tile of up to 8*MT query heads).  Its positions are counted in units of 16;
 // all items' units, and kItemCost more per item for its epilogue, are laid out on one line that is cut into
-// equal parts, one per block (two blocks per SM).  A block therefore moves the same number of bytes however
+// equal parts, one per block (two blocks of four warps per SM).  A block therefore moves the same number of bytes however
 // ragged the lengths are, and the cut is computed on the device from `lengths` alone: nothing is planned on the
 // host, and a captured launch stays right when the lengths change.  An item that is cut leaves one partial
 // result (maximum, sum, sum of values) per block; the block that finishes last joins them, in the blocks'
 // order, so results do not depend on timing.  No block waits for another.  When there are more items than blocks
-// and all are short, the line is cut into a part per warp, of whole items: nothing is shared between warps then
-// and an item costs no barriers (3840 items of up to 34 tokens: @@SOLO@@).
+// and the page table allows short ones only, the line is cut into a part per warp, of whole items: nothing is
+// shared between warps then and an item costs no barriers (3840 items of up to 34 tokens: 53 us by blocks, 20 by warps).
 //
 // Loads.  The warps of a block take the units of a segment in turn.  Each warp runs its own ring of kStages
 // units in shared memory, filled by a cursor that runs ahead of the arithmetic, over the ends of items too, so the
@@ -221,7 +221,8 @@ __global__ void paged_advance_kernel(int32_t* lengths, const int32_t* counts, in
 // Arithmetic.  m16n8k16 tensor instructions with the 8 query heads of a tile in rows 0-7 and, where an operand
 // does not fit 16 bits, its remainder in rows 8-15: the weights w are held to 16 + 16 bits that way (hi + lo),
 // and so is the rotated query of the fused step.  Rows 8-15 would idle otherwise (G is small), so the result has
-// fp32 weights at no cost.  MT = 2 serves 9..16 heads with one pass over the keys.
+// fp32 weights at no cost.  With 9..16 heads (MT = 2) all rows are heads, and the remainders are products of their
+// own into the same sums.  (An infinite value attended with MT = 2 therefore gives NaN, not infinity.)
 //
 // The fused step's new token is where one warp of the block that ends the item starts from (its score is the first
 // maximum, its value the first sum); it is stored into its page at the same time and read from no page.
@@ -481,6 +482,7 @@ struct Layout {
                        kScan = kMax + 2 * kWarps * 8 * 4, kLen = kScan + 128 + (SOLO ? kThreads * 8 : 0),
                        kTeams = kLen + kCached * 12;
   static constexpr int kBytes = 1024 + kTeams + (SOLO ? kWarps * kTeamBytes : kTeamBytes + kJoinBytes);
+  static_assert(kPanelBytes * (D / 64) == kTileBytes, "panels");
   static constexpr bool kFits = kPerSm * (kBytes + 1024) <= 233472;
   static_assert((SOLO || kFits) && kTeams % 16 == 0, "shared memory");
   static __device__ __forceinline__ uint32_t at(int row, int chunk) {
@@ -981,57 +983,62 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
           for (int i = team.rank * 4; i < heads * D; i += team.size * 4)
             store_out4<T>(p, cur.b, h0 + i / D, i % D, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
       } else if (cur.u0 < cur.u1) {
-        float m[MT], l[MT], acc[MT][D / 8][4];
+        float m[MT], l[MT], acc[D / 8][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           m[mt] = -INFINITY;
           l[mt] = 0.f;
-#pragma unroll
-          for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[mt][j][e] = 0.f;
         }
-        if (cur.u0 + team.warp < cur.u1) {
-          // query fragments: rows 0-7 the heads, rows 8-15 what a rotated query has beyond 16 bits
-          uint32_t qa[MT][KS][4];
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            const unsigned char* q = item + (mt * 8 + g) * L::kQPitch + 4 * t;
+        for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+        // coordinates 8j + 2t and the next of query head 8 mt + g
+        auto result = [&](int mt, int j) {
+          return MT == 1 ? make_float2(joined(acc[j][0], acc[j][2]), joined(acc[j][1], acc[j][3]))
+                         : make_float2(acc[j][2 * mt], acc[j][2 * mt + 1]);
+        };
+        if (cur.u0 + team.warp < cur.u1) {
+          // query fragments.  One tile: rows 0-7 the heads, rows 8-15 what a rotated query has beyond 16 bits (without
+          // tables those rows are whatever is there, and their scores are not looked at).  Two: 16 heads; what they
+          // have beyond 16 bits is a second product, its fragments read when it is made.
+          uint32_t qa[KS][4];
+          const uint32_t q_row = (lane & 7) * L::kQPitch + (lane >> 4) * 16, q_8 = 8 * L::kQPitch;
+          const uint32_t q_at = item_at + buf * L::kItemBytes + q_row, low_at = item_at + 2 * L::kItemBytes + q_row;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) ldmatrix4(qa[ks], ((lane & 8) ? (MT == 1 ? low_at : q_at + q_8) : q_at) + ks * 32);
+          auto low_query = [&](int ks, uint32_t(&q)[4]) { ldmatrix4(q, low_at + ((lane & 8) ? q_8 : 0) + ks * 32); };
+          if (with_new && team.warp == 0) {        // start from the new token: column 0 of a tile of keys, weight 1
+            const uint32_t* key = reinterpret_cast<const uint32_t*>(item + L::kKey);
+            float sc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-              qa[mt][ks][0] = *reinterpret_cast<const uint32_t*>(q + ks * 32);
-              qa[mt][ks][2] = *reinterpret_cast<const uint32_t*>(q + ks * 32 + 16);
-              qa[mt][ks][1] = qa[mt][ks][3] = 0u;
-            }
-            if (turn) {
-              const unsigned char* r = sm_low + (mt * 8 + g) * L::kQPitch + 4 * t;
-#pragma unroll
-              for (int ks = 0; ks < KS; ++ks) {
-                qa[mt][ks][1] = *reinterpret_cast<const uint32_t*>(r + ks * 32);
-                qa[mt][ks][3] = *reinterpret_cast<const uint32_t*>(r + ks * 32 + 16);
+              const uint32_t k0 = g == 0 ? key[ks * 8 + t] : 0u, k1 = g == 0 ? key[ks * 8 + 4 + t] : 0u;
+              mma16816<T>(sc, qa[ks], k0, k1);
+              if (MT > 1 && turn) {
+                uint32_t q[4];
+                low_query(ks, q);
+                mma16816<T>(sc, q, k0, k1);
               }
             }
-          }
-          if (with_new && team.warp == 0) {             // start from the new token: column 0 of a tile of keys, weight 1
-            const uint32_t* key = reinterpret_cast<const uint32_t*>(item + L::kKey);
+            float w[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              float sc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-              for (int ks = 0; ks < KS; ++ks)
-                mma16816<T>(sc, qa[mt][ks], g == 0 ? key[ks * 8 + t] : 0u, g == 0 ? key[ks * 8 + 4 + t] : 0u);
-              const float score = (turn ? joined(sc[0], sc[2]) : sc[0]) * p.scale_log2;
+              const float score = (MT == 1 && turn ? joined(sc[0], sc[2]) : sc[2 * mt]) * p.scale_log2;
               m[mt] = __shfl_sync(0xffffffffu, score, lane & ~3);
               // (weights of scores that are no numbers follow the formula: exp(inf - inf) and the like)
-              const float w = m[mt] == -INFINITY ? 0.f : exp2f(m[mt] - m[mt]);
-              l[mt] = t == 0 ? w : 0.f;
-#pragma unroll
-              for (int j = 0; j < D / 8; ++j) {
-                const float2 v = Cvt<T>::unpack(*reinterpret_cast<const uint32_t*>(item + L::kValue + (j * 8 + 2 * t) * 2));
-                acc[mt][j][0] = w * v.x;
-                acc[mt][j][1] = w * v.y;
-              }
+              w[mt] = m[mt] == -INFINITY ? 0.f : exp2f(m[mt] - m[mt]);
+              l[mt] = t == 0 ? w[mt] : 0.f;
               if (m[mt] != m[mt]) m[mt] = -INFINITY;           // (a maximum passes over NaN)
+            }
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) {
+              const float2 v = Cvt<T>::unpack(*reinterpret_cast<const uint32_t*>(item + L::kValue + (j * 8 + 2 * t) * 2));
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                acc[j][2 * mt] = w[mt] * v.x;
+                acc[j][2 * mt + 1] = w[mt] * v.y;
+              }
             }
           }
           // ldmatrix addresses within a tile: four chunk pairs of a panel, the other panel behind them
@@ -1047,30 +1054,33 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
               cp_async_wait<kStages - 1>();        // one group per unit that was asked for after this one may be open
               __syncwarp();
             }
-            float sc[MT][2][4];
+            float sc[2][4];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) sc[mt][0][e] = sc[mt][1][e] = 0.f;
+            for (int e = 0; e < 4; ++e) sc[0][e] = sc[1][e] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
               uint32_t kb[4];
               ldmatrix4(kb, ((base + k_at) ^ ((ks & 3) << 5)) + (ks >> 2) * L::kPanelBytes);
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                mma16816<T>(sc[mt][0], qa[mt][ks], kb[0], kb[1]);
-                mma16816<T>(sc[mt][1], qa[mt][ks], kb[2], kb[3]);
+              mma16816<T>(sc[0], qa[ks], kb[0], kb[1]);
+              mma16816<T>(sc[1], qa[ks], kb[2], kb[3]);
+              if (MT > 1 && opaque(turn)) {
+                uint32_t q[4];
+                low_query(ks, q);
+                mma16816<T>(sc[0], q, kb[0], kb[1]);
+                mma16816<T>(sc[1], q, kb[2], kb[3]);
               }
             }
+            // weights as two 16-bit parts.  One tile: rows 0-7 of a fragment the upper parts, rows 8-15 the lower ones;
+            // two: a fragment each, 16 heads.
             uint32_t pa[MT][4];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
               float s[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[e] = sc[mt][e >> 1][e & 1];
-              if (opaque(turn)) {
+              for (int e = 0; e < 4; ++e) s[e] = sc[e >> 1][(e & 1) + 2 * mt];
+              if (MT == 1 && opaque(turn)) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[e] = joined(s[e], sc[mt][e >> 1][(e & 1) + 2]);
+                for (int e = 0; e < 4; ++e) s[e] = joined(s[e], sc[e >> 1][(e & 1) + 2]);
               }
 #pragma unroll
               for (int e = 0; e < 4; ++e) s[e] *= p.scale_log2;
@@ -1091,23 +1101,29 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
 #pragma unroll
                 for (int j = 0; j < D / 8; ++j)
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) acc[mt][j][e] *= corr;
+                  for (int e = 0; e < 4; ++e)
+                    if (MT == 1 || e >> 1 == mt) acc[j][e] *= corr;
               }
               const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
 #pragma unroll
               for (int e = 0; e < 4; ++e) s[e] = exp2f(s[e] - ref);
               l[mt] += (s[0] + s[1]) + (s[2] + s[3]);
-              split2<T, false>(s[0], s[1], pa[mt][0], pa[mt][1]);
-              split2<T, false>(s[2], s[3], pa[mt][2], pa[mt][3]);
+              if (MT == 1) {
+                split2<T, false>(s[0], s[1], pa[0][0], pa[0][1]);
+                split2<T, false>(s[2], s[3], pa[0][2], pa[0][3]);
+              } else {
+                split2<T, false>(s[0], s[1], pa[0][mt], pa[MT - 1][mt]);
+                split2<T, false>(s[2], s[3], pa[0][mt + 2], pa[MT - 1][mt + 2]);
+              }
             }
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
               uint32_t vb[4];
               ldmatrix4_trans(vb, ((base + v_at) ^ ((j & 3) << 5)) + (j >> 2) * L::kPanelBytes);
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                mma16816<T>(acc[mt][2 * j], pa[mt], vb[0], vb[1]);
-                mma16816<T>(acc[mt][2 * j + 1], pa[mt], vb[2], vb[3]);
+              for (int part16 = 0; part16 < MT; ++part16) {
+                mma16816<T>(acc[2 * j], pa[part16], vb[0], vb[1]);
+                mma16816<T>(acc[2 * j + 1], pa[part16], vb[2], vb[3]);
               }
             }
             if (present & kByHand) proxy_fence();
@@ -1131,9 +1147,8 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
             const int64_t off = (int64_t)cur.b * p.o_sb + (int64_t)(h0 + mt * 8 + g) * p.o_sh + 2 * t;
 #pragma unroll
             for (int j = 0; j < D / 8; ++j) {
-              float x = joined(acc[mt][j][0], acc[mt][j][2]), y = joined(acc[mt][j][1], acc[mt][j][3]);
-              x = sum == 0.f ? 0.f : x * f;
-              y = sum == 0.f ? 0.f : y * f;
+              const float2 o = result(mt, j);
+              const float x = sum == 0.f ? 0.f : o.x * f, y = sum == 0.f ? 0.f : o.y * f;
               if (p.out_f32) *reinterpret_cast<float2*>(reinterpret_cast<float*>(p.out) + off + j * 8) = make_float2(x, y);
               else *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + off + j * 8) = Cvt<T>::pack(x, y);
             }
@@ -1163,8 +1178,7 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
               float* o = sm_o + (warp * 8 + g) * D;
 #pragma unroll
               for (int j = 0; j < D / 8; ++j)
-                *reinterpret_cast<float2*>(o + ((j * 8 + 2 * t) ^ (g << 2))) =
-                    make_float2(joined(acc[mt][j][0], acc[mt][j][2]), joined(acc[mt][j][1], acc[mt][j][3]));
+                *reinterpret_cast<float2*>(o + ((j * 8 + 2 * t) ^ (g << 2))) = result(mt, j);
             }
           }
           __syncthreads();
@@ -1281,7 +1295,8 @@ int launch_decode(DecodeParams& p, int grid, cudaStream_t stream) {
 template <typename T, int D, int MT>
 int launch_decode(DecodeParams& p, int grid, cudaStream_t stream) {
   // Warps on their own where no sequence can be long (the page table reaches kSoloTokens at most) and blocks would have
-  // to take several items each: @@RULE@@
+  // to take several items each.  By blocks and by warps: 120 sequences of 1..34 tokens, 32 heads of 128, 53 and 20 us;
+  // 51 of 128 tokens, 16 heads, 31 and 18.5; 20 of 156..318 tokens, 16 heads of 64, 18.0 and 21.1.
   if constexpr (Layout<D, MT, true>::kFits)        // (16 heads of 128: no room)
     if (p.capacity <= kSoloTokens && (int64_t)p.B * p.KV * p.tiles > grid) return launch_decode<T, D, MT, true>(p, grid, stream);
   return launch_decode<T, D, MT, false>(p, grid, stream);
