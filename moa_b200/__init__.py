@@ -12,7 +12,7 @@ from .attention import check_device_status, mixture_of_sparse_attention, sparse_
 from .cache import StaticCircularCache  # noqa: F401
 from .dist import HeadSharding, PeerGather  # noqa: F401
 from .module import DecodeGraph, MoAAttention, MoALlamaForCausalLM, MoALlamaModel, update_model_function  # noqa: F401
-from .paged import paged_append, paged_decode  # noqa: F401
+from .paged import PagedCache, paged_append, paged_decode  # noqa: F401
 from .plan import (  # noqa: F401
     decode_bytes,
     load_plan,
@@ -31,5 +31,5 @@ __all__ = [
     "permute_attention_projection", "permute_output_projection", "load_plan",
     "prefill_block_visits", "prefill_flops", "decode_bytes", "shard_heads", "MoaError", "LIB_PATH",
     "MoAAttention", "MoALlamaModel", "MoALlamaForCausalLM", "update_model_function", "HeadSharding", "PeerGather", "DecodeGraph",
-    "paged_append", "paged_decode",
+    "PagedCache", "paged_append", "paged_decode",
 ]

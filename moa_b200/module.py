@@ -23,13 +23,14 @@ plain torch ops (library kernels), the attention path is this package's kernels.
 from __future__ import annotations
 
 import copy
-from typing import Callable, Dict, List, Optional, Sequence, Tuple
+from typing import Callable, Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor, nn
 
 from .attention import check_device_status, mixture_of_sparse_attention
 from .cache import StaticCircularCache
+from .paged import PagedCache
 from .plan import (
     moa_config_to_cache_config,
     moa_config_to_permutation,
@@ -113,7 +114,7 @@ class MoAAttention(nn.Module):
         return w
 
     @torch.no_grad()
-    def attend(self, hidden_states: Tensor, past_key_value: StaticCircularCache,
+    def attend(self, hidden_states: Tensor, past_key_value: Union[StaticCircularCache, PagedCache],
                position_embeddings: Tuple[Tensor, Tensor], out: Optional[Tensor] = None) -> Tensor:
         """Projection, rotary embedding, cache update and attention of this module's heads:
         ``(B, q, hidden) -> (B, q, H_local, D)`` (everything of ``forward`` before the gather and ``o_proj``).
@@ -126,10 +127,14 @@ class MoAAttention(nn.Module):
         sm_scale = D ** -0.5
         if q_len == 1:
             # one launch: rotary embedding of q and k, ring append, flash-decoding, bookkeeping
+            if self.peer_gather is not None and isinstance(past_key_value, PagedCache):
+                raise NotImplementedError("the fused gather delivers the rows of ring caches only")
             if self.peer_gather is not None:    # ... and delivery of the rows to every rank: (B, 1, H, D) comes back
                 return self.peer_gather.decode_and_gather(past_key_value, q, k, v, self.layer_idx, sm_scale,
                                                           rope=(cos, sin))
             return past_key_value.decode_attention(q, k, v, self.layer_idx, sm_scale, out=out, rope=(cos, sin))
+        if isinstance(past_key_value, PagedCache):
+            return self._paged_prefill(q, k, v, past_key_value, (cos, sin), sm_scale)
         q, k = apply_rotary_pos_emb(q, k, cos, sin)
         past_key_value.update(k, v, self.layer_idx)
         return mixture_of_sparse_attention(
@@ -138,6 +143,20 @@ class MoAAttention(nn.Module):
             local_size=past_key_value.circular_cache_size[self.layer_idx],
             head_start_index=past_key_value.cache_head_start_index[self.layer_idx],
             head_valid_length=past_key_value.cache_valid_length[self.layer_idx])           # (B, q, H, D)
+
+    def _paged_prefill(self, q: Tensor, k: Tensor, v: Tensor, cache: PagedCache, rope: Tuple[Tensor, Tensor],
+                       sm_scale: float) -> Tensor:
+        """Prompts into empty slots of a paged cache: rotation and append in one launch, then the block-sparse
+        attention of the prompt (dense where the cache has no spans)."""
+        if cache.get_seq_length(self.layer_idx) > 0:
+            raise NotImplementedError("a prompt goes into empty slots (release or admit them first)")
+        H, N = q.shape[1], q.shape[2]
+        q, k = cache.update(k, v, self.layer_idx, rope=rope, query=q)
+        sink, local = cache.static_cache_size[self.layer_idx], cache.circular_cache_size[self.layer_idx]
+        if sink is None:
+            sink = torch.zeros(H, dtype=torch.int64, device=q.device)
+            local = torch.full((H,), N + 64, dtype=torch.int64, device=q.device)
+        return mixture_of_sparse_attention(q, k, v, sm_scale=sm_scale, sink_size=sink, local_size=local)
 
     @torch.no_grad()
     def forward(self, hidden_states: Tensor, attention_mask: Optional[Tensor] = None,
@@ -148,7 +167,8 @@ class MoAAttention(nn.Module):
         if output_attentions:
             raise NotImplementedError("output_attentions is not supported in mixture of attention")
         assert not self.training, "only support inference now"
-        assert isinstance(past_key_value, StaticCircularCache), "MoAAttention needs a StaticCircularCache"
+        assert isinstance(past_key_value, (StaticCircularCache, PagedCache)), \
+            "MoAAttention needs a StaticCircularCache or a PagedCache"
         bsz, q_len, _ = hidden_states.shape
         if position_embeddings is None:
             assert position_ids is not None, "position_ids or position_embeddings are required"
@@ -324,8 +344,28 @@ class MoALlamaModel(nn.Module):
         return StaticCircularCache(**cfg, batch_size=batch_size, head_dim=self.hidden_size // self.num_heads,
                                    device=self.device, dtype=self.dtype, update_cache_content=True)
 
+    def new_paged_cache(self, batch_size: int, seq_length: int, num_pages: Optional[int] = None, page_size: int = 64,
+                        max_length: Optional[int] = None) -> PagedCache:
+        """A paged cache for this model (of this rank's heads when they are sharded), to be passed as
+        ``past_key_values``: slots of up to ``max_length`` tokens (``seq_length`` and ``moa_max_new_token`` more, if not
+        given) that share ``num_pages`` pages (none: enough for all slots at that length).  With a plan installed its
+        spans at ``seq_length`` are the heads'; without one every head attends every token."""
+        heads = self.layers[0].self_attn.num_local_heads
+        static = circular = None
+        if self.use_moa:
+            plan = self.local_moa_config if self.local_moa_config is not None else self.moa_config
+            cfg = moa_config_to_cache_config(plan, seq_len=seq_length, max_new_token=self.moa_max_new_token, sink_size=64,
+                                             minimum_cache_size=128, split_size=64, verbose=self.moa_verbose)
+            static = cfg["static_size"]
+            circular = [[c - s for c, s in zip(cs, ss)] for cs, ss in zip(cfg["cache_size"], static)]
+        max_length = max_length if max_length is not None else seq_length + self.moa_max_new_token
+        num_pages = num_pages if num_pages is not None else batch_size * -(-max_length // page_size)
+        return PagedCache(len(self.layers), heads, num_pages, batch_size, max_length, self.hidden_size // self.num_heads,
+                          page_size, static, circular, self.device, self.dtype)
+
     @torch.no_grad()
-    def forward(self, input_ids: Optional[Tensor] = None, past_key_values: Optional[StaticCircularCache] = None,
+    def forward(self, input_ids: Optional[Tensor] = None,
+                past_key_values: Optional[Union[StaticCircularCache, PagedCache]] = None,
                 inputs_embeds: Optional[Tensor] = None, position_ids: Optional[Tensor] = None):
         """Returns ``(last_hidden_state, cache)``; ``last_hidden_state`` is ``(B, 1, hidden)`` when
         ``last_hidden_only`` (modeling_llama.py:195-199).  After a prefill (more than one token) the device
@@ -336,9 +376,11 @@ class MoALlamaModel(nn.Module):
         if inputs_embeds is None:
             inputs_embeds = self.embed_tokens(input_ids)
         batch_size, seq_length = inputs_embeds.shape[:2]
-        if not isinstance(past_key_values, StaticCircularCache):
+        if not isinstance(past_key_values, (StaticCircularCache, PagedCache)):
             past_key_values = self.new_cache(batch_size, seq_length)
-        if position_ids is None:
+        if position_ids is None and isinstance(past_key_values, PagedCache):
+            position_ids = past_key_values.positions(seq_length)
+        elif position_ids is None:
             past = past_key_values.get_seq_length()
             position_ids = torch.arange(past, past + seq_length, device=inputs_embeds.device).unsqueeze(0)
         head_dim = self.hidden_size // self.num_heads
@@ -401,7 +443,8 @@ class MoALlamaForCausalLM(nn.Module):
         self.model.set_mixture_of_attention(*args, **kwargs)
 
     @torch.no_grad()
-    def forward(self, input_ids: Optional[Tensor] = None, past_key_values: Optional[StaticCircularCache] = None,
+    def forward(self, input_ids: Optional[Tensor] = None,
+                past_key_values: Optional[Union[StaticCircularCache, PagedCache]] = None,
                 inputs_embeds: Optional[Tensor] = None, position_ids: Optional[Tensor] = None):
         """Returns ``(logits, cache)``; logits of the last position only when ``model.last_hidden_only``."""
         hidden, cache = self.model(input_ids, past_key_values, inputs_embeds, position_ids)
@@ -425,13 +468,20 @@ class DecodeGraph:
         out = graph.step(next_ids)                 # (B, 1, hidden) or (B, 1, vocab); overwritten by the next step
 
     With sharded heads every rank must capture and replay alike; a ``PeerGather`` needs an even number of
-    layers (its two buffers alternate by call)."""
+    layers (its two buffers alternate by call).
 
-    def __init__(self, model, cache: StaticCircularCache):
+    With a ``PagedCache`` positions and lengths are on the device too, slots may come and go between steps
+    (``release``, ``admit``, a prompt through ``slots``), and ``step`` hands out the pages that the next token needs."""
+
+    def __init__(self, model, cache: Union[StaticCircularCache, PagedCache]):
         self.model = model
         self.cache = cache
         base = model.model if isinstance(model, MoALlamaForCausalLM) else model
         device, B = base.device, cache.batch_size
+        self.paged = isinstance(cache, PagedCache)
+        if self.paged:
+            self._capture_paged(device, B)
+            return
         for layer in range(cache.num_layers):
             if cache.get_seq_length(layer) <= max(cache._static_host[layer]):
                 raise RuntimeError("DecodeGraph: capture once every ring has left its static part "
@@ -453,8 +503,30 @@ class DecodeGraph:
         # capturing ran the host side once without executing anything: take the host counters back
         cache._kv_len, cache.cache_position = kv_len, cache_position
 
+    def _capture_paged(self, device, B: int) -> None:
+        cache = self.cache
+        cache.reserve(1)
+        self.ids = torch.zeros(B, 1, dtype=torch.long, device=device)
+        counted = [list(row) for row in cache._tokens]
+        stream = torch.cuda.Stream(device)
+        stream.wait_stream(torch.cuda.current_stream(device))
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph, stream=stream):
+            self.out, _ = self.model(self.ids, past_key_values=cache)
+        torch.cuda.current_stream(device).wait_stream(stream)
+        # capturing ran the host side once without executing anything: take the host's counts back
+        for row, was in zip(cache._tokens, counted):
+            row[:] = was
+
     @torch.no_grad()
     def step(self, input_ids: Tensor) -> Tensor:
+        if self.paged:
+            self.cache.reserve(1)
+            self.ids.copy_(input_ids, non_blocking=True)
+            self.graph.replay()
+            for layer in range(self.cache.num_layers):
+                self.cache._count(layer, [1] * self.cache.batch_size)
+            return self.out
         self.ids.copy_(input_ids, non_blocking=True)
         self.graph.replay()
         self.cache._kv_len = [n + 1 for n in self.cache._kv_len]

@@ -7,8 +7,9 @@ The kernels are ``csrc/paged.cu``; there is no CPU path and no gradient, as in t
 """
 from __future__ import annotations
 
+import copy
 import struct
-from typing import Dict, Optional, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
@@ -289,3 +290,181 @@ def check_status(device=None) -> None:
         if code:
             name, text = _STATUS.get(code, ("moa_paged_decode", "status {0} {1} {2}"))
             raise _lib.MoaError(name, 1, lib.moa_strerror(1).decode(), text.format(*where))
+
+
+class PagedCache:
+    """Keys and values of a batch of sequences that grow, end and begin independently, in a pool of pages.
+
+    Beside ``StaticCircularCache``: a slot of the batch has its own length and takes pages as it grows; query
+    heads may share ``num_kv_heads`` key/value heads; ``update`` and ``decode_attention`` are called the same way, so
+    that ``MoAAttention`` and ``MoALlamaModel`` take either cache.  With ``static_size`` and ``circular_size``
+    (``[layer][head]``, in tokens) a head attends the first and the last of its sequence's tokens only, as a
+    ring of that size would; without them every token.
+
+    Host and device keep the lengths side by side: the kernels advance ``lengths`` ``(num_layers, batch_size)``,
+    the host counts along to hand out pages.  ``page_table`` ``(batch_size, max_length / page_size)`` and ``lengths``
+    stay where they are, so a captured decode step can be replayed while ``reserve`` hands out pages between
+    replays.  All calls of one cache belong on one stream."""
+
+    def __init__(self, num_layers: int, num_kv_heads: int, num_pages: int, batch_size: int = 1, max_length: int = 4096,
+                 head_dim: int = 128, page_size: int = 64, static_size: Optional[List[List[int]]] = None,
+                 circular_size: Optional[List[List[int]]] = None, device="cuda",
+                 dtype: torch.dtype = torch.float16) -> None:
+        assert dtype in _DTYPES, f"the paged cache supports float16 and bfloat16 only, got {dtype}"
+        assert head_dim in (64, 128), "head_dim must be 64 or 128"
+        assert page_size > 0 and page_size & (page_size - 1) == 0, "page_size must be a power of two"
+        assert num_layers > 0 and num_kv_heads > 0 and num_pages > 0 and batch_size > 0 and max_length > 0
+        assert (static_size is None) == (circular_size is None), "static_size and circular_size go together"
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.num_layers, self.num_kv_heads, self.head_dim, self.page_size = num_layers, num_kv_heads, head_dim, page_size
+        self.batch_size, self.device, self.dtype = batch_size, device, dtype
+        self.static_cache_size = self.circular_cache_size = [None] * num_layers
+        if static_size is not None:
+            for sizes in (static_size, circular_size):
+                assert len(sizes) == num_layers and all(len(row) == num_kv_heads for row in sizes), \
+                    "static_size and circular_size must be [layer][key/value head]"
+            self.static_cache_size = [torch.tensor(row, dtype=torch.int64, device=device) for row in static_size]
+            self.circular_cache_size = [torch.tensor(row, dtype=torch.int64, device=device) for row in circular_size]
+        shape = (num_pages, num_kv_heads, page_size, head_dim)
+        self.key_pages = [torch.empty(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.value_pages = [torch.empty(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        width = -(-max_length // page_size)
+        self.page_table = torch.full((batch_size, width), -1, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(num_layers, batch_size, dtype=torch.int32, device=device)
+        # shared by the views that slots() makes
+        self._first = 0
+        self._free: List[int] = list(range(num_pages - 1, -1, -1))
+        self._pages: List[List[int]] = [[] for _ in range(batch_size)]
+        self._tokens: List[List[int]] = [[0] * batch_size for _ in range(num_layers)]     # -1: no sequence
+
+    # ------------------------------------------------------------------ slots and pages
+    def slots(self, first: int, last: int) -> "PagedCache":
+        """This cache's slots ``first .. last - 1`` as a cache of their own, on the same pages: a prompt can be taken
+        in there while the other slots wait."""
+        if not 0 <= first < last <= self.batch_size:
+            raise IndexError(f"slots {first} .. {last - 1} of {self.batch_size}")
+        view = copy.copy(self)
+        view.batch_size, view._first = last - first, self._first + first
+        view.page_table, view.lengths = self.page_table[first:last], self.lengths[:, first:last]
+        return view
+
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def get_seq_length(self, layer_idx: Optional[int] = 0) -> int:
+        """Tokens of the longest sequence."""
+        return max(max(n, 0) for n in self.sequence_lengths(layer_idx))
+
+    def sequence_lengths(self, layer_idx: int = 0) -> List[int]:
+        """Tokens in every slot as the host counts them, -1 for a slot without a sequence."""
+        return self._tokens[layer_idx][self._first:self._first + self.batch_size]
+
+    def positions(self, q_len: int) -> Tensor:
+        """``(batch_size, q_len)`` positions of the next ``q_len`` tokens, from the lengths on the device."""
+        at = torch.arange(q_len, device=self.device)
+        return self.lengths[0].clamp(min=0).long()[:, None] + at
+
+    def release(self, slot: int) -> None:
+        """Ends the sequence in ``slot``: its pages go back to the pool, and the slot is idle until ``admit``."""
+        self._set(slot, -1)
+
+    def admit(self, slot: int) -> None:
+        """Begins a new, empty sequence in ``slot`` (whatever was there is released)."""
+        self._set(slot, 0)
+
+    def _set(self, slot: int, tokens: int) -> None:
+        if not 0 <= slot < self.batch_size:
+            raise IndexError(f"slot {slot} of {self.batch_size}")
+        self._free.extend(reversed(self._pages[self._first + slot]))
+        self._pages[self._first + slot] = []
+        for row in self._tokens:
+            row[self._first + slot] = tokens
+        self.page_table[slot].fill_(-1)
+        self.lengths[:, slot].fill_(tokens)
+
+    def reserve(self, tokens) -> None:
+        """Pages for ``tokens`` more tokens (a number, or one per slot) in every slot that has a sequence.  All or
+        nothing: raises without taking any page when the pool or a row of the page table is too small."""
+        tokens = [tokens] * self.batch_size if isinstance(tokens, int) else [int(n) for n in tokens]
+        assert len(tokens) == self.batch_size, "one number of tokens per slot"
+        wanted = []
+        for slot, more in enumerate(tokens):
+            at = self._first + slot
+            longest = max(row[at] for row in self._tokens)
+            missing = -(-(longest + more) // self.page_size) - len(self._pages[at]) if longest >= 0 and more > 0 else 0
+            if missing > 0:
+                if len(self._pages[at]) + missing > self.page_table.shape[1]:
+                    raise ValueError(f"slot {slot} would hold {longest + more} tokens: more than the cache's max_length")
+                wanted.append((slot, missing))
+        if not wanted:
+            return
+        if sum(missing for _, missing in wanted) > len(self._free):
+            raise RuntimeError(f"out of pages: {sum(m for _, m in wanted)} wanted, {len(self._free)} free")
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("pages cannot be handed out while a graph is captured: reserve() them before")
+        for slot, missing in wanted:
+            pages = self._pages[self._first + slot]
+            new = [self._free.pop() for _ in range(missing)]
+            self.page_table[slot, len(pages):len(pages) + missing] = torch.tensor(new, dtype=torch.int32).to(self.device)
+            pages.extend(new)
+
+    def _room(self, layer_idx: int, counts: List[int]) -> None:
+        """Pages for ``counts`` more tokens in the slots, if they are not there yet."""
+        row = self._tokens[layer_idx]
+        for slot, more in enumerate(counts):
+            at = self._first + slot
+            if row[at] >= 0 and row[at] + more > len(self._pages[at]) * self.page_size:
+                longest = [max(r[self._first + s] for r in self._tokens) for s in range(self.batch_size)]
+                self.reserve([max(row[self._first + s] + n - longest[s], 0) if row[self._first + s] >= 0 else 0
+                              for s, n in enumerate(counts)])
+                return
+
+    def _count(self, layer_idx: int, counts: List[int]) -> None:
+        row = self._tokens[layer_idx]
+        for slot, more in enumerate(counts):
+            if row[self._first + slot] >= 0:
+                row[self._first + slot] += more
+
+    # ------------------------------------------------------------------ the calls a layer makes
+    def update(self, key_states: Tensor, value_states: Tensor, layer_idx: int, attention_mask: Optional[Tensor] = None,
+               cache_kwargs: Optional[Dict] = None, counts: Optional[Sequence[int]] = None,
+               rope: Optional[Tuple[Tensor, Tensor]] = None, query: Optional[Tensor] = None):
+        """Appends ``(B, KV, q_len, D)`` states to the slots' sequences, of slot ``b`` the first ``counts[b]`` tokens (none:
+        all).  ``rope`` and ``query`` as in ``paged_append``.  Returns the rotated query and key when a query is given,
+        else the states it was given."""
+        if attention_mask is not None:
+            raise NotImplementedError("PagedCache.update: padding is told by counts, on the right")
+        assert layer_idx < self.num_layers
+        B, KV, N, D = key_states.shape
+        assert (B, KV, D) == (self.batch_size, self.num_kv_heads, self.head_dim), "states must be (B, KV, q_len, D)"
+        assert key_states.dtype == self.dtype and key_states.device == self.device, "states and cache must be alike"
+        each = [N] * B if counts is None else [min(max(int(n), 0), N) for n in counts]
+        assert len(each) == B, "one count per slot"
+        self._room(layer_idx, each)
+        on_device = None if counts is None else torch.tensor(each, dtype=torch.int32).to(self.device)
+        got = paged_append(key_states, value_states, self.key_pages[layer_idx], self.value_pages[layer_idx],
+                           self.page_table, self.lengths[layer_idx], counts=on_device, rope=rope, query=query, advance=True)
+        self._count(layer_idx, each)
+        return (key_states, value_states) if got is None else got
+
+    def decode_attention(self, query_states: Tensor, key_states: Tensor, value_states: Tensor, layer_idx: int,
+                         sm_scale: float, out: Optional[Tensor] = None, rope: Optional[Tuple[Tensor, Tensor]] = None,
+                         out_dtype: Optional[torch.dtype] = None) -> Tensor:
+        """One decode step of one layer in one launch, as ``StaticCircularCache.decode_attention``: rotate, append and
+        attend over every slot's sequence with its new token.  ``rope``: this step's tables, ``(B, 1, D)`` or
+        ``(B, D)``.  Rows of idle slots are zero.  A captured call replays on any lengths for which pages are
+        reserved; the host's count is then the replayer's to keep (``DecodeGraph`` does)."""
+        assert layer_idx < self.num_layers
+        B = self.batch_size
+        assert query_states.dtype == self.dtype and query_states.device == self.device, "states and cache must be alike"
+        self._room(layer_idx, [1] * B)
+        if rope is not None:
+            rope = tuple(t.reshape(B, 1, self.head_dim) for t in rope)
+        out = paged_decode(query_states, self.key_pages[layer_idx], self.value_pages[layer_idx], self.page_table,
+                           self.lengths[layer_idx], sm_scale, key=key_states, value=value_states, rope=rope,
+                           sink_size=self.static_cache_size[layer_idx], local_size=self.circular_cache_size[layer_idx],
+                           out=out, out_dtype=out_dtype, advance=True)
+        self._count(layer_idx, [1] * B)
+        return out

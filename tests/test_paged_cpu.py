@@ -186,3 +186,92 @@ def test_null_arguments_are_an_error_not_a_crash():
     assert _lib.lib.moa_paged_decode(None, 0) == 1
     assert _lib.lib.moa_paged_status(0) == 1
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+# ------------------------------------------------------------------------------------------- PagedCache, host side
+def _cache(**changes):
+    args = dict(num_layers=2, num_kv_heads=2, num_pages=6, batch_size=3, max_length=64, head_dim=64, page_size=16, device="cpu")
+    args.update(changes)
+    return moa_b200.PagedCache(**args)
+
+
+def _held(cache):
+    return [[p for p in row if p >= 0] for row in cache.page_table.tolist()]
+
+
+def test_cache_hands_out_pages_once_and_takes_them_back():
+    cache = _cache()
+    assert cache.free_pages() == 6 and cache.page_table.shape == (3, 4) and cache.get_seq_length() == 0
+    cache.reserve([16, 17, 0])
+    held = _held(cache)
+    assert [len(h) for h in held] == [1, 2, 0] and len(set(sum(held, []))) == 3 and cache.free_pages() == 3
+    cache.reserve(1)                                  # the third slot has none yet, the others have room
+    assert [len(h) for h in _held(cache)] == [1, 2, 1]
+    assert _held(cache)[:2] == held[:2]
+    cache.release(1)
+    assert _held(cache)[1] == [] and cache.free_pages() == 4 and cache.sequence_lengths() == [0, -1, 0]
+    assert cache.lengths[:, 1].tolist() == [-1, -1]
+    cache.reserve(10)                                 # nothing for the idle slot
+    assert _held(cache)[1] == []
+    cache.admit(1)
+    cache.reserve([0, 64, 0])
+    assert cache.free_pages() == 0 and len(set(sum(_held(cache), []))) == 6
+
+
+def test_cache_refuses_without_taking_anything():
+    cache = _cache()
+    with pytest.raises(RuntimeError, match="out of pages"):
+        cache.reserve([64, 33, 1])                    # 4 + 3 + 1 of 6
+    with pytest.raises(ValueError, match="max_length"):
+        cache.reserve([0, 65, 0])
+    assert cache.free_pages() == 6 and _held(cache) == [[], [], []]
+    with pytest.raises(IndexError):
+        cache.release(3)
+    with pytest.raises(IndexError):
+        cache.slots(1, 4)
+    with pytest.raises(AssertionError):
+        cache.reserve([1, 1])
+    for bad in (dict(page_size=48), dict(head_dim=96), dict(dtype=torch.float32), dict(static_size=[[1, 1], [1, 1]]),
+                dict(static_size=[[1, 1]], circular_size=[[1, 1]]), dict(num_pages=0)):
+        with pytest.raises(AssertionError):
+            _cache(**bad)
+
+
+def test_slots_are_a_view_with_shared_pages():
+    cache = _cache()
+    view = cache.slots(1, 3)
+    view.reserve([20, 0])
+    assert [len(h) for h in _held(cache)] == [0, 2, 0] and view.free_pages() == cache.free_pages() == 4
+    view._count(0, [20, 5])
+    assert cache.sequence_lengths(0) == [0, 20, 5] and view.get_seq_length() == 20 and view.slots(1, 2).sequence_lengths() == [5]
+    view.release(0)
+    assert cache.sequence_lengths(1) == [0, -1, 0] and cache.free_pages() == 6
+    assert view.page_table.data_ptr() == cache.page_table[1].data_ptr()
+
+
+def test_room_counts_layers_that_lag_behind():
+    cache = _cache()
+    cache._room(0, [16, 16, 16])
+    cache._count(0, [16, 16, 16])
+    cache._room(1, [16, 16, 16])                      # the second layer of the same step: no further pages
+    assert cache.free_pages() == 3
+    cache._count(1, [16, 16, 16])
+    cache._room(0, [1, 1, 1])
+    assert cache.free_pages() == 0
+
+
+def test_cache_calls_check_their_states():
+    cache = _cache()
+    k = torch.zeros(3, 2, 5, 64).half()
+    with pytest.raises(RuntimeError, match="CUDA"):
+        cache.update(k, k, 0)
+    with pytest.raises(NotImplementedError):
+        cache.update(k, k, 0, attention_mask=torch.ones(3, 5))
+    with pytest.raises(AssertionError):
+        cache.update(k[:2], k[:2], 0)
+    with pytest.raises(AssertionError):
+        cache.update(k.bfloat16(), k.bfloat16(), 0)
+    with pytest.raises(AssertionError):
+        cache.update(k, k, 0, counts=[1, 2])
+    with pytest.raises(AssertionError):
+        cache.update(k, k, 2)
