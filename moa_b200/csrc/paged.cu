@@ -1212,6 +1212,14 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
       }
       if (more) cur = next;
     }
+    if (!waiting)                                  // a load is late: it must not land in a block that has ended
+      for (int s = 0; s < kStages; ++s) {
+        bar_wait(bars + stage * 8, parity);
+        if (++stage == kStages) {
+          stage = 0;
+          parity ^= 1;
+        }
+      }
   }
 
   if (p.advance) {                                 // the last block to get here: every block has read the lengths

@@ -23,6 +23,9 @@ _DECODE = struct.Struct("=13Q30qd")
 _COUNTER_BYTES = 8192
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _NO_ROPE = (0, 0, 0, 0, 0, 0)
+# paged_decode takes (sequence, key head) pairs a warp each when there are more than blocks (two per SM) and the page
+# table reaches this many tokens at most
+_MANY, _SHORT = 296, 256
 
 # the stream's handle without a Stream object around it, as torch's own generated code asks for it
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or _lib.current_stream
@@ -462,7 +465,12 @@ class PagedCache:
         self._room(layer_idx, [1] * B)
         if rope is not None:
             rope = tuple(t.reshape(B, 1, self.head_dim) for t in rope)
-        out = paged_decode(query_states, self.key_pages[layer_idx], self.value_pages[layer_idx], self.page_table,
+        table = self.page_table
+        if B * self.num_kv_heads > _MANY and self.page_size <= _SHORT < table.shape[1] * self.page_size and \
+                max(self.sequence_lengths(layer_idx)) < _SHORT and not _capturing():
+            # the kernel for many short sequences goes by the table's width (a captured step keeps all of it)
+            table = table[:, :_SHORT // self.page_size]
+        out = paged_decode(query_states, self.key_pages[layer_idx], self.value_pages[layer_idx], table,
                            self.lengths[layer_idx], sm_scale, key=key_states, value=value_states, rope=rope,
                            sink_size=self.static_cache_size[layer_idx], local_size=self.circular_cache_size[layer_idx],
                            out=out, out_dtype=out_dtype, advance=True)

@@ -363,6 +363,71 @@ def test_non_finite_values_go_where_the_formula_puts_them():
     assert torch.isnan(out[0, 0, 1]).all() and torch.isfinite(out[1]).all()
 
 
+@pytest.mark.parametrize("dtype,D,H,KV,page", [(F16, 128, 4, 4, 16), (BF16, 128, 24, 3, 64), (F16, 64, 2, 2, 8), (BF16, 64, 36, 3, 16),
+                                              (F16, 64, 40, 2, 32), (BF16, 128, 24, 2, 16)])
+@pytest.mark.parametrize("step", ["attend", "plain step", "step"])
+@pytest.mark.parametrize("spanned", [False, True])
+def test_many_short_sequences(dtype, D, H, KV, page, step, spanned):
+    """More (sequence, key head) pairs than blocks, and page tables that reach 256 tokens at most."""
+    gen = torch.Generator().manual_seed(5)
+    lengths = [int(n) for n in torch.randint(0, 190, (210,), generator=gen)]
+    lengths[3], lengths[50], lengths[209], lengths[7] = 0, 1, 191, 190
+    if step != "attend":
+        lengths[11], lengths[208] = -1, -9
+    c = Case(lengths, H, KV, D, page, dtype, layout="tokens" if KV == 3 else "heads", room=1, width=256 // page)
+    assert c.table.shape[1] * page == 256 and c.B * KV > 296
+    c.table[:, -1] = -1
+    spans = ([0, 5, 16, 200][:KV], [33, 64, 0, 7][:KV]) if spanned else (None, None)
+    sink, local = (None, None) if not spanned else (torch.tensor(x, device="cuda") for x in spans)
+    q = c.normal(c.B, H, 1, D)
+    kb, vb = c.kp.clone(), c.vp.clone()
+    if step == "attend":
+        args, n, qr, rows = {}, c.lengths, q, []
+    else:
+        k, v = c.normal(c.B, KV, 1, D), c.normal(c.B, KV, 1, D)
+        args, qr = dict(key=k, value=v), q
+        n = torch.where(c.lengths < 0, c.lengths, c.lengths + 1)
+        live = (c.lengths >= 0).nonzero()[:, 0]
+        rows = [c.places(b, c.lengths[b:b + 1].long()) for b in live.tolist()]
+        if step == "step":
+            args["rope"] = tables(D, torch.arange(256), torch.float32)
+            cos, sin = (t[c.lengths.long().clamp(min=0)] for t in args["rope"])
+            qr = rotated64(q, cos[:, None, None], sin[:, None, None])[0]
+    out32 = moa_b200.paged_decode(q, *c.pool(), 0.11, sink_size=sink, local_size=local, out_dtype=torch.float32, **args)
+    out = moa_b200.paged_decode(q, *c.pool(), 0.11, sink_size=sink, local_size=local, **args)
+    moa_b200.check_device_status()
+    same_pool(c.kp, kb, rows)
+    same_pool(c.vp, vb, rows)
+    if rows:
+        for b, (pages, slots) in zip(live.tolist(), rows):
+            assert torch.equal(c.vp[pages, :, slots][0], v[b, :, 0])
+            if step == "step":
+                ref, parts = rotated64(k[b, :, 0], cos[b], sin[b])
+                close(c.kp[pages, :, slots][0], ref, 3 * U * parts)
+            else:
+                assert torch.equal(c.kp[pages, :, slots][0], k[b, :, 0])
+    ref, tol = attention64(c, qr, n, 0.11, *spans)
+    close(out32, ref, tol)
+    close(out, ref, tol)
+    assert torch.equal(out32.to(dtype), out)
+
+
+@pytest.mark.parametrize("B,H,KV,page,top", [(300, 2, 2, 64, 500), (2, 300, 300, 16, 40), (600, 1, 1, 16, 90), (270, 12, 1, 32, 700)])
+def test_more_sequences_or_heads_than_are_held_in_shared_memory(B, H, KV, page, top):
+    gen = torch.Generator().manual_seed(8)
+    lengths = [int(n) for n in torch.randint(0, top, (B,), generator=gen)]
+    c = Case(lengths, H, KV, 64, page, F16, room=1)
+    spans = ([int(x) for x in torch.randint(0, 20, (KV,), generator=gen)], [int(x) for x in torch.randint(0, 300, (KV,), generator=gen)])
+    _decode(c)
+    _decode(c, spans=spans)
+    q, k, v = c.normal(B, H, 1, 64), c.normal(B, KV, 1, 64), c.normal(B, KV, 1, 64)
+    out = moa_b200.paged_decode(q, *c.pool(), 0.2, key=k, value=v, advance=True)
+    assert c.lengths.tolist() == [n + 1 for n in lengths]
+    ref, tol = attention64(c, q, c.lengths, 0.2)
+    close(out, ref, tol)
+    moa_b200.check_device_status()
+
+
 def test_decode_into_a_wider_buffer_and_from_strided_queries():
     c = Case([70, 5, 200], 6, 3, 128, 32, F16, layout="inside", room=0)
     wide = torch.full((3, 1, 10, 128), 7.0, dtype=F16, device="cuda")

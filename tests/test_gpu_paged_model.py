@@ -160,3 +160,29 @@ def test_shared_key_heads_and_ragged_prompts_through_the_cache():
     ref, tol = attention64(c, qr, cache.lengths[0], 0.125, [4, 0], [50, 90])
     close(out, ref, tol)
     moa_b200.check_device_status()
+
+
+def test_many_short_sequences_through_the_cache():
+    """160 slots of two key heads each, grown over 256 tokens: the same as the pages hold, whichever kernel it takes."""
+    from test_gpu_paged import attention64, close
+
+    class Held:
+        pass
+
+    B, H, KV, D = 160, 4, 2, 64
+    cache = moa_b200.PagedCache(1, KV, B * 5, B, 320, D, 64, dtype=torch.float16)
+    gen = torch.Generator().manual_seed(2)
+    normal = lambda *s: torch.randn(*s, generator=gen).half().cuda()
+    counts = [int(n) for n in torch.randint(1, 254, (B,), generator=gen)]
+    counts[5] = 253
+    cache.update(normal(B, KV, 253, D), normal(B, KV, 253, D), 0, counts=counts)
+    c = Held()
+    c.B, c.H, c.KV, c.D, c.kp, c.vp = B, H, KV, D, cache.key_pages[0], cache.value_pages[0]
+    c.places = lambda b, pos: (cache.page_table[b, pos // 64].long(), pos % 64)
+    for step in range(6):                     # the longest sequence: 254 .. 259 tokens
+        q, k, v = normal(B, H, 1, D), normal(B, KV, 1, D), normal(B, KV, 1, D)
+        out = cache.decode_attention(q, k, v, 0, 0.125, out_dtype=torch.float32)
+        ref, tol = attention64(c, q, cache.lengths[0], 0.125)
+        close(out, ref, tol)
+    assert cache.sequence_lengths() == [n + 6 for n in counts]
+    moa_b200.check_device_status()
