@@ -315,19 +315,24 @@ struct Span {
   __device__ __forceinline__ bool sees_last() const { return n > 0 && (sink == n || from < n); }
 };
 
+// a / b for b > 0 and 0 <= a: 64-bit division takes some hundred instructions, and nearly always 32 bits do.
+__device__ __forceinline__ int64_t divided(int64_t a, int b) {
+  return a >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
 // The line in equal parts, one per team (a block, or a warp on its own).
 struct Cut {
   int64_t total, each;                      // units of the line; of a part, rounded down
   int parts, rest;                          // total = each * parts + rest
   __device__ __forceinline__ Cut(int64_t t, int most, int least) : total(t) {
     parts = (int)min(max(t / least, (int64_t)1), (int64_t)most);
-    each = t / parts;
+    each = divided(t, parts);
     rest = (int)(t - each * parts);
   }
-  __device__ __forceinline__ int64_t begin(int c) const { return each * c + (int64_t)rest * c / parts; }
+  __device__ __forceinline__ int64_t begin(int c) const { return each * c + (uint32_t)(rest * c) / (uint32_t)parts; }      // (parts < 2^15)
   // The last c with begin(c) <= x.
   __device__ __forceinline__ int part_of(int64_t x) const {
-    int c = min((int)((float)x / (float)total * parts), parts - 1);
+    int c = min((int)__fdividef((float)x * parts, (float)total), parts - 1);
 #pragma unroll 1
     while (begin(c) > x) --c;
 #pragma unroll 1
@@ -842,7 +847,7 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
           ++b;
         }
       }
-      const int item = (int)((part.lo - at) / cost);
+      const int item = (int)divided(part.lo - at, cost);
       cur.b = b;
       cur.kh = kh + item / p.tiles;
       cur.tile = item % p.tiles;
