@@ -655,3 +655,82 @@ def test_the_ring_cache_and_pages_with_spans_agree():
             close(b, ref, tol)
             close(a, ref, tol)
     moa_b200.check_device_status()
+
+
+@pytest.mark.parametrize("page,lengths", [(2048, [5000, 1, 2048]), (65536, [70000, 3]), (512, [511, 512, 513])])
+def test_large_pages(page, lengths):
+    c = Case(lengths, 4, 2, 64, page, BF16, room=1)
+    _decode(c)
+    k, v = c.normal(c.B, 2, 1, 64), c.normal(c.B, 2, 1, 64)
+    moa_b200.paged_append(k, v, *c.pool(), advance=True)
+    _decode(c)
+    moa_b200.check_device_status()
+
+
+def test_pools_whose_heads_are_one_head_repeated():
+    """An expanded dimension (stride zero) for reading: every key head is the same memory."""
+    c = Case([100, 333], 6, 1, 128, 64, F16, room=0)
+    q = c.normal(2, 6, 1, 128)
+    one = moa_b200.paged_decode(q, *c.pool(), 0.09)
+    three = moa_b200.paged_decode(q, c.kp.expand(-1, 3, -1, -1), c.vp.expand(-1, 3, -1, -1), c.table, c.lengths, 0.09)
+    ref, tol = attention64(c, q, c.lengths, 0.09)
+    close(one, ref, tol)
+    close(three, ref, tol)
+
+
+@pytest.mark.parametrize("G", [2, 12])
+def test_a_rotated_query_beyond_the_range_of_fp16(G):
+    """Coordinates of 60000 become up to 84852 when they are turned; the query is not rounded to fp16 on the way."""
+    c = Case([50, 7], 2 * G, 2, 64, 16, F16, room=1)
+    q = torch.where(c.normal(2, 2 * G, 1, 64) > 0, 60000.0, -60000.0).half()
+    k, v = c.normal(2, 2, 1, 64), c.normal(2, 2, 1, 64)
+    cos, sin = tables(64, torch.arange(64), torch.float32)
+    out = moa_b200.paged_decode(q, *c.pool(), 1e-6, key=k, value=v, rope=(cos, sin), out_dtype=torch.float32)
+    at = c.lengths.long()
+    qr = rotated64(q, cos[at][:, None, None], sin[at][:, None, None])[0]
+    assert qr.abs().max() > 70000
+    ref, tol = attention64(c, qr, c.lengths + 1, 1e-6)
+    close(out, ref, tol)
+
+
+def test_the_output_may_replace_the_query():
+    c = Case([3000, 40, 0], 8, 2, 64, 64, BF16, room=0)
+    q = c.normal(3, 1, 8, 64)
+    ref = moa_b200.paged_decode(q.transpose(1, 2), *c.pool(), 0.125)
+    got = moa_b200.paged_decode(q.transpose(1, 2), *c.pool(), 0.125, out=q)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(got, ref)
+
+
+CHILD = """
+import torch, moa_b200
+kp, vp = torch.randn(9, 2, 16, 64, device="cuda").half(), torch.randn(9, 2, 16, 64, device="cuda").half()
+table, lengths = torch.arange(9, device="cuda", dtype=torch.int32)[None], torch.full((1,), 100, device="cuda", dtype=torch.int32)
+q, k = torch.randn(1, 4, 1, 64, device="cuda").half(), torch.randn(1, 2, 1, 64, device="cuda").half()
+if CAPTURE:
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        moa_b200.paged_append(k, k, kp, vp, table, lengths)
+        out = moa_b200.paged_decode(q, kp, vp, table, lengths, 0.125, key=k, value=k, advance=True)
+    graph.replay(); graph.replay()
+else:
+    moa_b200.paged_append(k, k, kp, vp, table, lengths, advance=True)
+    moa_b200.paged_decode(q, kp, vp, table, lengths, 0.125, key=k, value=k, advance=True)
+    out = None
+moa_b200.check_device_status()
+assert lengths.tolist() == [102], lengths
+if out is not None:
+    assert torch.equal(out, moa_b200.paged_decode(q, kp, vp, table, lengths - 1, 0.125, key=k, value=k))
+print("child ok")
+"""
+
+
+@pytest.mark.parametrize("capture,env", [(True, {}), (False, {"MOA_B200_NVTX": "1"})])
+def test_a_process_whose_first_call_is_captured_and_one_with_ranges(capture, env):
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", "CAPTURE = %r\n%s" % (capture, CHILD)], cwd=root, text=True,
+                          capture_output=True, timeout=300, env={**os.environ, **env, "PYTHONPATH": root})
+    assert done.returncode == 0 and "child ok" in done.stdout, done.stderr[-2000:]
