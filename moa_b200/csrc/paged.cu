@@ -780,17 +780,21 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
   }
+  const uint32_t bars = (uint32_t)__cvta_generic_to_shared(smem + L::kBar) + warp * kStages * 8;
+  if (lane < kStages) {
+    bar_init(bars + lane * 8);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // So far nothing was read that a kernel before this one may have written: a launch may begin while the one before
+  // it ends (1.8 us less from launch to launch), and waits here until all of that one's writes are there.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   // ---- the line: its length, and where this team's part begins
 #pragma unroll 1
   for (int b = tid; b < min(p.B, kCached); b += kThreads) sm_len[b] = p.lengths[b];
   if (p.sink)
 #pragma unroll 1
     for (int kh = tid; kh < min(p.KV, kCached); kh += kThreads) sm_span[kh] = Sizes::clamped(p.sink[kh], p.local[kh]);
-  const uint32_t bars = (uint32_t)__cvta_generic_to_shared(smem + L::kBar) + warp * kStages * 8;
-  if (lane < kStages) {
-    bar_init(bars + lane * 8);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
   __syncthreads();
   // in rows of items that cost the same: a sequence's, or with spans a (sequence, key head)'s
   const int per_seq = p.sink ? p.KV : 1, items = p.sink ? p.tiles : p.KV * p.tiles;
@@ -1301,8 +1305,17 @@ int launch_decode(DecodeParams& p, int grid, cudaStream_t stream) {
   p.tma = p.pool.shift >= 4 &&      // a unit lies in one page
           make_map(&map_k, p.pool.k, p, p.pool.k_page, p.pool.k_head, p.pool.k_slot, D, bf16) &&
           make_map(&map_v, p.pool.v, p, p.pool.v_page, p.pool.v_head, p.pool.v_slot, D, bf16);
-  paged_decode_kernel<T, D, MT, SOLO><<<grid, L::kThreads, L::kBytes, stream>>>(map_k, map_v, p);
-  MOA_CUDA_CHECK(cudaGetLastError());
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)grid);
+  config.blockDim = dim3(L::kThreads);
+  config.dynamicSmemBytes = L::kBytes;
+  config.stream = stream;
+  cudaLaunchAttribute early = {};                  // see griddepcontrol.wait in the kernel
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  MOA_CUDA_CHECK(cudaLaunchKernelEx(&config, paged_decode_kernel<T, D, MT, SOLO>, map_k, map_v, p));
   return MOA_OK;
 }
 template <typename T, int D, int MT>
