@@ -1,4 +1,4 @@
-"""Builds libmoa_b200.so (the C-ABI library) in-tree with nvcc for sm_100a.
+"""Builds libmoa_b200.so (the C-ABI library) in-tree with nvcc for sm_100a, and _paged_host.so beside it.
 
     python moa_b200/build.py [--force] [--verbose]
 
@@ -18,6 +18,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmoa_b200.so")
 SOURCES = ["errors.cu", "decode.cu", "cache.cu", "prefill.cu", "peer.cu", "paged.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
+#: the host's share of the paged calls, compiled against the installed torch (moa_b200/paged.py does without it, slower)
+HOST = os.path.join(HERE, "_paged_host.so")
+HOST_SOURCE = os.path.join(CSRC, "paged_host.cpp")
 
 
 def _nvcc() -> str:
@@ -28,9 +31,9 @@ def _nvcc() -> str:
 
 
 def _stale() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(HOST):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(HOST))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(HERE, "..", "include", "moa_b200.h")]
     return any(os.path.getmtime(d) > t for d in deps)
 
@@ -54,7 +57,26 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
+    build_host(verbose)
     return LIB
+
+
+def build_host(verbose: bool = False) -> str:
+    """Compile csrc/paged_host.cpp with the host compiler against the installed torch."""
+    import sysconfig
+
+    import torch
+
+    base = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           *("-I" + d for d in (os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
+                                os.path.join(cuda, "include"), sysconfig.get_paths()["include"])),
+           HOST_SOURCE, "-o", HOST, "-L" + os.path.join(base, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    return HOST
 
 
 if __name__ == "__main__":

@@ -8,6 +8,7 @@ The kernels are ``csrc/paged.cu``; there is no CPU path and no gradient, as in t
 from __future__ import annotations
 
 import copy
+import ctypes
 import struct
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -31,6 +32,16 @@ _MANY, _SHORT = 296, 256
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or _lib.current_stream
 _capturing = torch.cuda.is_current_stream_capturing
 
+try:
+    from . import _paged_host as _host       # the common case of both calls, compiled (csrc/paged_host.cpp)
+except ImportError:                          # not built against this torch: the same calls, from Python alone
+    _host = None
+if _host is not None:
+    _host.init(ctypes.cast(lib.moa_paged_append, ctypes.c_void_p).value,
+               ctypes.cast(lib.moa_paged_decode, ctypes.c_void_p).value)
+if _lib.NVTX:
+    _host = None                             # ranges are marked from Python
+
 _workspaces: Dict = {}
 _touched = set()      # devices that a paged call has run on
 
@@ -46,6 +57,8 @@ def _workspace(index: int, stream: int) -> Tensor:
     if ws is None:
         ws = _workspaces[index, stream] = torch.zeros(lib.moa_paged_decode_workspace_bytes(), dtype=torch.uint8,
                                                       device=index)
+        if _host is not None:
+            _host.seen(index, stream, ws.data_ptr(), ws.numel())
     return ws
 
 
@@ -127,7 +140,10 @@ def _launch(name: str, entry, arguments, device: int) -> None:
         status = entry(arguments(stream), stream)
     if status:
         _lib.check("moa_" + name, status)
-    _touched.add(device)
+    if device not in _touched:
+        _touched.add(device)
+        if _host is not None:
+            _host.seen(device, 0, 0, 0)
 
 
 def paged_append(key: Tensor, value: Tensor, key_pages: Tensor, value_pages: Tensor, page_table: Tensor,
@@ -153,6 +169,14 @@ def paged_append(key: Tensor, value: Tensor, key_pages: Tensor, value_pages: Ten
 
     A token whose page (or row of a table by position) does not exist is not stored, and
     ``check_device_status()`` raises for it.  Two tokens of one call must not have the same place."""
+    if _host is not None:
+        got = _host.append(key, value, key_pages, value_pages, page_table, lengths, counts, rope, query, advance)
+        if got is not None:
+            if got is True:
+                return None
+            if got.__class__ is int:
+                _lib.check("moa_paged_append", got)
+            return got
     shape = key.shape
     assert len(shape) == 4 and value.shape == shape, "key and value must be (B, KV, N, D)"
     B, KV, N, D = shape
@@ -213,6 +237,13 @@ def paged_decode(query: Tensor, key_pages: Tensor, value_pages: Tensor, page_tab
     of every sequence; ``lengths[b] < 0`` marks a row without a sequence: nothing is stored and its output is zero.
 
     Tokens whose page does not exist are left out, and ``check_device_status()`` raises for them."""
+    if _host is not None:
+        got = _host.decode(query, key_pages, value_pages, page_table, lengths, sm_scale, key, value, rope, sink_size,
+                           local_size, out, out_dtype, advance)
+        if got is not None:
+            if got.__class__ is int:
+                _lib.check("moa_paged_decode", got)
+            return got
     shape = query.shape
     assert len(shape) == 4 and shape[2] == 1, "query must be (B, H, 1, D)"
     B, H, _, D = shape

@@ -734,3 +734,90 @@ def test_a_process_whose_first_call_is_captured_and_one_with_ranges(capture, env
     done = subprocess.run([sys.executable, "-c", "CAPTURE = %r\n%s" % (capture, CHILD)], cwd=root, text=True,
                           capture_output=True, timeout=300, env={**os.environ, **env, "PYTHONPATH": root})
     assert done.returncode == 0 and "child ok" in done.stdout, done.stderr[-2000:]
+
+
+def test_compiled_and_python_checks_make_the_same_calls(monkeypatch):
+    """The compiled common case against the calls from Python alone, and what it leaves to Python."""
+    from moa_b200 import paged
+
+    assert paged._host is not None, "moa_b200/_paged_host.so is not built"
+    c = Case([100, 333, -1, 0], 12, 3, 128, 32, BF16, room=9)
+    qkv = c.normal(4, 9, 18, 128)
+    q, k, v = (t.transpose(1, 2) for t in qkv.split([12, 3, 3], 2))
+    counts = torch.tensor([9, 4, 1, 0], dtype=torch.int32, device="cuda")
+    sink, local = torch.tensor([4, 0, 64], device="cuda"), torch.tensor([99, 10, 0], device="cuda")
+    where, token = tables(128, torch.arange(400), torch.float32), tables(128, torch.arange(9)[None] + 5, BF16)
+    one = [t[:, :, :1] for t in (q, k, v)]
+    shared = tables(128, torch.arange(1)[None] + 7, torch.float32)
+    calls = [lambda: moa_b200.paged_append(k, v, *c.pool()),
+             lambda: moa_b200.paged_append(k, v, *c.pool(), counts=counts, rope=where, query=q),
+             lambda: moa_b200.paged_append(k, v, *c.pool(), counts=counts, rope=token, query=q[:, :5]),
+             lambda: moa_b200.paged_append(k, v, *c.pool(), counts=counts, advance=True),
+             lambda: moa_b200.paged_decode(one[0], *c.pool(), 0.1),
+             lambda: moa_b200.paged_decode(one[0], *c.pool(), 0.1, sink_size=sink, local_size=local),
+             lambda: moa_b200.paged_decode(one[0], *c.pool(), 0.1, key=one[1], value=one[2]),
+             lambda: moa_b200.paged_decode(one[0], *c.pool(), 0.1, key=one[1], value=one[2], rope=where, advance=True),
+             lambda: moa_b200.paged_decode(one[0], *c.pool(), 0.1, key=one[1], value=one[2], rope=shared, sink_size=sink,
+                                           local_size=local)]
+    moa_b200.paged_decode(one[0], *c.pool(), 0.1)          # this stream's scratch
+    start = [t.clone() for t in (c.kp, c.vp, c.lengths)]
+
+    def results():
+        got = []
+        for call in calls:
+            for t, was in zip((c.kp, c.vp, c.lengths), start):
+                t.copy_(was)
+            out = call()
+            got.append([t.clone() for t in (out if isinstance(out, tuple) else () if out is None else (out,))] +
+                       [t.clone() for t in (c.kp, c.vp, c.lengths)])
+        return got
+
+    counted = {"decode": 0, "append": 0}
+
+    class Counting:
+        def __getattr__(self, name):
+            inner = getattr(host, name)
+
+            def call(*args):
+                got = inner(*args)
+                counted[name] = counted.get(name, 0) + (got is not None)
+                return got
+            return call
+
+    host = paged._host
+    monkeypatch.setattr(paged, "_host", Counting())
+    compiled = results()
+    assert counted["append"] == 4 and counted["decode"] == 5     # none of them was left to Python
+    # what it leaves: copies, an output of the caller's, fp32, gradients, refusals, captures
+    before = dict(counted)
+    moa_b200.paged_decode(c.normal(4, 12, 1, 131)[..., 3:], *c.pool(), 0.1)
+    moa_b200.paged_decode(one[0], *c.pool(), 0.1, out_dtype=torch.float32)
+    moa_b200.paged_append(k[..., 1:65].contiguous()[:, :, :0], v[..., :64][:, :, :0], c.kp[..., :64], c.vp[..., :64], c.table, c.lengths)
+    with pytest.raises(NotImplementedError):
+        moa_b200.paged_decode(one[0].detach().requires_grad_(), *c.pool(), 0.1)
+    for bad in (dict(lengths=c.lengths.long()), dict(page_table=c.table[:2]), dict(key=one[1]), dict(sink_size=sink),
+                dict(advance=True), dict(rope=where), dict(query=q), dict(query=one[0].half())):
+        args = dict(query=one[0], key_pages=c.kp, value_pages=c.vp, page_table=c.table, lengths=c.lengths, sm_scale=0.1)
+        args.update(bad)
+        with pytest.raises(AssertionError):
+            moa_b200.paged_decode(**args)
+    for bad in (dict(value=v[:, :2]), dict(counts=counts.long()), dict(query=q), dict(rope=(where[0], where[1][:7]), query=q),
+                dict(rope=tuple(t[:, :3] for t in token))):
+        args = dict(key=k, value=v, key_pages=c.kp, value_pages=c.vp, page_table=c.table, lengths=c.lengths)
+        args.update(bad)
+        with pytest.raises(AssertionError):
+            moa_b200.paged_append(**args)
+    with pytest.raises(moa_b200.MoaError, match="power of two"):     # an error of the C entry point comes through it
+        moa_b200.paged_append(k, v, c.kp[:, :, :24], c.vp[:, :, :24], c.table, c.lengths)
+    before["append"] += 1
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        moa_b200.paged_decode(one[0], *c.pool(), 0.1)
+    assert counted["decode"] == before["decode"] and counted["append"] == before["append"]
+    with torch.no_grad():
+        moa_b200.paged_decode(one[0].detach().requires_grad_(), *c.pool(), 0.1)
+    assert counted["decode"] == before["decode"] + 1
+    monkeypatch.setattr(paged, "_host", None)
+    for a, b in zip(compiled, results()):
+        assert len(a) == len(b) and all(x.shape == y.shape and x.stride() == y.stride() and torch.equal(
+            x.view(torch.int16) if x.dtype == BF16 else x, y.view(torch.int16) if y.dtype == BF16 else y) for x, y in zip(a, b))

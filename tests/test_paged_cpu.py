@@ -275,3 +275,14 @@ def test_cache_calls_check_their_states():
         cache.update(k, k, 0, counts=[1, 2])
     with pytest.raises(AssertionError):
         cache.update(k, k, 2)
+
+
+def test_compiled_checks_leave_everything_else_to_python():
+    """On tensors without a device, on things that are no tensors, and with too few arguments they answer None."""
+    assert paged._host is not None, "moa_b200/_paged_host.so is not built"
+    t = _inputs()
+    pools = (t["key_pages"], t["value_pages"], t["page_table"], t["lengths"])
+    assert paged._host.decode(t["query"], *pools, 0.1, None, None, None, None, None, None, None, False) is None
+    assert paged._host.append(t["key"], t["value"], *pools, None, None, None, False) is None
+    assert paged._host.decode(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14) is None
+    assert paged._host.decode() is None and paged._host.append(None) is None
