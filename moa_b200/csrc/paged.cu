@@ -668,15 +668,17 @@ __device__ __noinline__ void join_parts(const DecodeParams& p, int c0, int c1, i
     // counters of a part: of the item that begins in it 0 and 1 by level, of the one that began before 2
     int* counter = p.counters + kCounters * (c0 + first) + (group == 0 ? level : 2);
     const bool final = there <= kJoin;
-    __threadfence();
+    // One thread's acquire and release stand for the block's: the barriers around it order the others' records, which
+    // are read past L1.
     __syncthreads();
     if (tid == 0) {
-      *flag = atomicAdd(counter, 1) == count - 1;
-      if (*flag) *counter = 0;
+      int before;
+      asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+      *flag = before == count - 1;
+      if (before == count - 1) *counter = 0;
     }
     __syncthreads();
     if (!*flag) return;
-    __threadfence();
     // record i of the group; a part's second record is of the item that begins in it
     float* const records = p.records + (int64_t)(2 * (c0 + first)) * kRecFloats;
     const uint32_t stride = 2 * step * (uint32_t)kRecFloats, shift0 = first == 0 ? (uint32_t)kRecFloats : 0;
