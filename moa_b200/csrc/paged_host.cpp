@@ -155,9 +155,12 @@ PyObject* decode(PyObject*, PyObject* const* x, Py_ssize_t n) {
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
     const auto at_stream = scratch.find({device, stream});
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-    if (at_stream == scratch.end() || cudaStreamIsCapturing(stream, &capturing) != cudaSuccess ||
-        capturing != cudaStreamCaptureStatusNone)
+    if (at_stream == scratch.end()) Py_RETURN_NONE;
+    if (cudaStreamIsCapturing(stream, &capturing) != cudaSuccess) {
+      (void)cudaGetLastError();
       Py_RETURN_NONE;
+    }
+    if (capturing != cudaStreamCaptureStatusNone) Py_RETURN_NONE;
     at::Tensor out = at::empty({B, 1, H, D}, q->options().requires_grad(false));
     a.out = out.data_ptr();
     a.o_sb = H * D;
