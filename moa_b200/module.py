@@ -146,10 +146,14 @@ class MoAAttention(nn.Module):
 
     def _paged_prefill(self, q: Tensor, k: Tensor, v: Tensor, cache: PagedCache, rope: Tuple[Tensor, Tensor],
                        sm_scale: float) -> Tensor:
-        """Prompts into empty slots of a paged cache: rotation and append in one launch, then the block-sparse
-        attention of the prompt (dense where the cache has no spans)."""
-        if cache.get_seq_length(self.layer_idx) > 0:
-            raise NotImplementedError("a prompt goes into empty slots (release or admit them first)")
+        """Prompts into empty slots of a paged cache, each with a sequence to take them: rotation and append in one
+        launch, then the block-sparse attention of the prompt (dense where the cache has no spans)."""
+        lengths = cache.sequence_lengths(self.layer_idx)
+        if max(lengths) > 0:
+            raise NotImplementedError("a prompt goes into empty slots (admit them anew first)")
+        if min(lengths) < 0:        # nothing would be stored for it, and its rows would come back as if it had been
+            raise RuntimeError(f"slot {lengths.index(-1)} has no sequence: admit it before its prompt, or pass the other "
+                               "slots as a cache of their own")
         H, N = q.shape[1], q.shape[2]
         q, k = cache.update(k, v, self.layer_idx, rope=rope, query=q)
         sink, local = cache.static_cache_size[self.layer_idx], cache.circular_cache_size[self.layer_idx]

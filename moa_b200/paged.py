@@ -466,8 +466,9 @@ class PagedCache:
                cache_kwargs: Optional[Dict] = None, counts: Optional[Sequence[int]] = None,
                rope: Optional[Tuple[Tensor, Tensor]] = None, query: Optional[Tensor] = None):
         """Appends ``(B, KV, q_len, D)`` states to the slots' sequences, of slot ``b`` the first ``counts[b]`` tokens (none:
-        all).  ``rope`` and ``query`` as in ``paged_append``.  Returns the rotated query and key when a query is given,
-        else the states it was given."""
+        all); rows of idle slots are left alone, and it is an error when no slot can take what it is given.  ``rope`` and
+        ``query`` as in ``paged_append``.  Returns the rotated query and key when a query is given, else the states it
+        was given."""
         if attention_mask is not None:
             raise NotImplementedError("PagedCache.update: padding is told by counts, on the right")
         assert layer_idx < self.num_layers
@@ -476,6 +477,9 @@ class PagedCache:
         assert key_states.dtype == self.dtype and key_states.device == self.device, "states and cache must be alike"
         each = [N] * B if counts is None else [min(max(int(n), 0), N) for n in counts]
         assert len(each) == B, "one count per slot"
+        given = [held for more, held in zip(each, self.sequence_lengths(layer_idx)) if more > 0]
+        if given and max(given) < 0:
+            raise RuntimeError("no slot that tokens are given for has a sequence: admit one first")
         self._room(layer_idx, each)
         on_device = None if counts is None else torch.tensor(each, dtype=torch.int32).to(self.device)
         got = paged_append(key_states, value_states, self.key_pages[layer_idx], self.value_pages[layer_idx],

@@ -1,0 +1,64 @@
+"""Calls with a paged cache that must be refused before anything is written or handed out.  No GPU."""
+import pytest
+import torch
+
+import moa_b200
+
+
+def _attention(**changes):
+    torch.manual_seed(0)
+    attention = moa_b200.MoAAttention(128, 2, 0, dtype=torch.float16).eval()
+    for name, value in changes.items():
+        setattr(attention, name, value)
+    return attention
+
+
+def _cache(batch_size=2):
+    return moa_b200.PagedCache(num_layers=1, num_kv_heads=2, num_pages=8, batch_size=batch_size, max_length=64, head_dim=64,
+                               page_size=16, device="cpu")
+
+
+def _attend(attention, cache, tokens):
+    hidden = torch.zeros(cache.batch_size, tokens, 128, dtype=torch.float16)
+    tables = tuple(torch.zeros(cache.batch_size, tokens, 64, dtype=torch.float16) for _ in range(2))
+    return attention.attend(hidden, cache, tables)
+
+
+def _state(cache):
+    return cache.free_pages(), cache.sequence_lengths(), cache.lengths.tolist(), cache.page_table.tolist()
+
+
+@pytest.mark.parametrize("idle", [[0], [1], [0, 1]])
+def test_a_prompt_into_a_slot_without_a_sequence_is_refused(idle):
+    cache = _cache()
+    for slot in idle:
+        cache.release(slot)
+    before = _state(cache)
+    with pytest.raises(RuntimeError, match="admit"):
+        _attend(_attention(), cache, 5)
+    assert _state(cache) == before
+    one = cache.slots(idle[0], idle[0] + 1)
+    with pytest.raises(RuntimeError, match="admit"):
+        _attend(_attention(), one, 5)
+    assert _state(cache) == before
+    for slot in idle:
+        cache.admit(slot)
+    with pytest.raises(RuntimeError, match="CUDA"):       # and nothing else is wrong with the call
+        _attend(_attention(), cache, 5)
+
+
+def test_update_refuses_tokens_that_no_slot_can_take():
+    cache = _cache()
+    k = torch.zeros(2, 2, 5, 64).half()
+    cache.release(0), cache.release(1)
+    before = _state(cache)
+    for counts in (None, [5, 0], [0, 3]):
+        with pytest.raises(RuntimeError, match="admit"):
+            cache.update(k, k, 0, counts=counts)
+    assert _state(cache) == before
+    cache.admit(1)
+    with pytest.raises(RuntimeError, match="admit"):
+        cache.update(k, k, 0, counts=[5, 0])
+    # one of them can: rows of idle slots are left alone
+    with pytest.raises(RuntimeError, match="CUDA"):
+        cache.update(k, k, 0)
