@@ -221,9 +221,13 @@ __global__ void paged_advance_kernel(int32_t* lengths, const int32_t* counts, in
 // needs (queries, the new token's rows) is fetched while the item before it is worked on.
 //
 // Arithmetic.  m16n8k16 tensor instructions with the 8 query heads of a tile in rows 0-7 and, where an operand
-// does not fit 16 bits, its remainder in rows 8-15: the weights w are held to 16 + 16 bits that way (hi + lo),
-// and so is the rotated query of the fused step.  Rows 8-15 would idle otherwise (G is small), so the result has
-// fp32 weights at no cost.  With 9..16 heads (MT = 2) all rows are heads, and the remainders are products of their
+// does not fit 16 bits, its remainder in rows 8-15: the weights w are held in two 16-bit parts that way (hi + lo),
+// and so is the rotated query of the fused step.  Rows 8-15 would idle otherwise (G is small), so the second part costs
+// nothing.  A weight is off by 2^-23 of itself in fp16 and by 2^-17 in bf16, whose third part would cost products of its
+// own (64 sequences of up to 8192 tokens 174 -> 180 us) and change little: the result is as far from 64 bits with it (1.5e-6
+// against 1.6e-6, of sums in the tensor cores).  fp16 has those bits from 2^-14 on only, so its weights are 2^15 times what
+// they are, sums and records with them, and the factor falls out at the division: steps of 2^-40 of the largest.
+// With 9..16 heads (MT = 2) all rows are heads, and the remainders are products of their
 // own into the same sums.  (An infinite value attended with MT = 2 therefore gives NaN, not infinity.)
 //
 // The fused step's new token is where one warp of the block that ends the item starts from (its score is the first
@@ -256,6 +260,14 @@ struct DecodeParams {
   int* counters;                            // kCounters per part, zero between launches, and one behind them
   float* records;                           // 2 per part
 };
+
+// Weights are exp2(score - m) with m the running maximum less 15 in fp16, so that the largest is 2^15.  m is rounded
+// before it is used, and the same m is in the records, so that this adds no error; it is rounded up, so that no weight
+// is more than 2^15 however large the scores are.
+template <typename T>
+__device__ __forceinline__ float lifted(float top) {
+  return std::is_same<T, __half>::value ? __fsub_ru(top, 15.f) : top;
+}
 
 // A flag that the compiler takes to change: loops are not made in two versions for it (the kernel has to be
 // fetched through the caches that the keys run through, its size counts).
@@ -455,7 +467,7 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uin
 }
 
 // x = hi + lo with both in T, for two values; hi of an fp16 that does not fit is its largest, lo takes the rest.
-// (A weight fits: it is 1 at most.)
+// (A weight fits: it is 2^15 at most.)
 template <typename T, bool LARGE>
 __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
   if (LARGE && std::is_same<T, __half>::value) {
@@ -1042,10 +1054,11 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
             float w[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              const float score = (MT == 1 && turn ? joined(sc[0], sc[2]) : sc[2 * mt]) * p.scale_log2;
-              m[mt] = __shfl_sync(0xffffffffu, score, lane & ~3);
+              float score = (MT == 1 && turn ? joined(sc[0], sc[2]) : sc[2 * mt]) * p.scale_log2;
+              score = __shfl_sync(0xffffffffu, score, lane & ~3);
+              m[mt] = lifted<T>(score);
               // (weights of scores that are no numbers follow the formula: exp(inf - inf) and the like)
-              w[mt] = m[mt] == -INFINITY ? 0.f : exp2f(m[mt] - m[mt]);
+              w[mt] = score == -INFINITY ? 0.f : exp2f(score - m[mt]);
               l[mt] = t == 0 ? w[mt] : 0.f;
               if (m[mt] != m[mt]) m[mt] = -INFINITY;           // (a maximum passes over NaN)
             }
@@ -1110,7 +1123,7 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
               }
               float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+              top = lifted<T>(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)));
               if (__any_sync(0xffffffffu, top > m[mt])) {      // a new maximum: what there is so far is scaled down
                 const float m_new = fmaxf(m[mt], top);
                 const float corr = m_new == m[mt] ? 1.f : exp2f(m[mt] - m_new);
