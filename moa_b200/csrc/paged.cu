@@ -226,9 +226,13 @@ __global__ void paged_advance_kernel(int32_t* lengths, const int32_t* counts, in
 // nothing.  A weight is off by 2^-23 of itself in fp16 and by 2^-17 in bf16, whose third part would cost products of its
 // own (64 sequences of up to 8192 tokens 174 -> 180 us) and change little: the result is as far from 64 bits with it (1.5e-6
 // against 1.6e-6, of sums in the tensor cores).  fp16 has those bits from 2^-14 on only, so its weights are 2^15 times what
-// they are, sums and records with them, and the factor falls out at the division: steps of 2^-40 of the largest.
-// With 9..16 heads (MT = 2) all rows are heads, and the remainders are products of their
-// own into the same sums.  (An infinite value attended with MT = 2 therefore gives NaN, not infinity.)
+// they are, sums and records with them, and the factor falls out at the division: steps of 2^-39 of the largest.
+// With 9..16 heads (MT = 2) all rows are heads, and the other parts are products of their own.
+//
+// An infinite value with a weight is infinite in the result, so a weight's upper part is never 0 (fp16: 2^-39 of the
+// largest at least), and what a lower part makes of an infinity (0 * inf, or the other sign) must not get into it: it is in
+// a row of its own (MT = 1) or in sums of its own (scores), and where values are summed with MT = 2 all parts are positive,
+// cut off and not rounded, so that bf16 needs three (60 query heads on 5, 69 sequences of 482 tokens: 23.1 -> 24.0 us).
 //
 // The fused step's new token is where one warp of the block that ends the item starts from (its score is the first
 // maximum, its value the first sum); it is stored into its page at the same time and read from no page.
@@ -477,6 +481,26 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_
   }
   const float2 h = Cvt<T>::unpack(hi);
   lo = Cvt<T>::pack(x0 - h.x, x1 - h.y);
+}
+// x as a sum of positive numbers in T, for two values from 0 on.  (Of 0 itself the parts are 0, in bf16 the second and
+// third the least normal number.)
+template <typename T>
+constexpr int kPositiveParts = std::is_same<T, __half>::value ? 2 : 3;
+template <typename T>
+__device__ __forceinline__ void split_positive2(float x0, float x1, uint32_t (&part)[kPositiveParts<T>]) {
+  if constexpr (std::is_same<T, __half>::value) {
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(part[0]) : "f"(x1), "f"(x0));
+    const float2 h = Cvt<T>::unpack(part[0]);
+    part[1] = Cvt<T>::pack(fmaxf(x0 - h.x, fminf(x0, 0x1p-24f)), fmaxf(x1 - h.y, fminf(x1, 0x1p-24f)));
+  } else {                                         // eight bits a part: the upper halves of what is left
+#pragma unroll
+    for (int i = 0; i < kPositiveParts<T>; ++i) {
+      part[i] = __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
+      const float2 h = Cvt<T>::unpack(part[i]);
+      x0 = fmaxf(x0 - h.x, 0x1p-126f);
+      x1 = fmaxf(x1 - h.y, 0x1p-126f);
+    }
+  }
 }
 // hi + lo of a sum that was split; an infinity of hi is the result (its lo is inf - inf or 0 * inf).
 __device__ __forceinline__ float joined(float hi, float lo) { return isinf(hi) ? hi : hi + lo; }
@@ -1040,7 +1064,7 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
           auto low_query = [&](int ks, uint32_t(&q)[4]) { ldmatrix4(q, low_at + ((lane & 8) ? q_8 : 0) + ks * 32); };
           if (with_new && team.warp == 0) {        // start from the new token: column 0 of a tile of keys, weight 1
             const uint32_t* key = reinterpret_cast<const uint32_t*>(item + L::kKey);
-            float sc[4] = {0.f, 0.f, 0.f, 0.f};
+            float sc[4] = {0.f, 0.f, 0.f, 0.f}, low[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
               const uint32_t k0 = g == 0 ? key[ks * 8 + t] : 0u, k1 = g == 0 ? key[ks * 8 + 4 + t] : 0u;
@@ -1048,13 +1072,13 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
               if (MT > 1 && turn) {
                 uint32_t q[4];
                 low_query(ks, q);
-                mma16816<T>(sc, q, k0, k1);
+                mma16816<T>(low, q, k0, k1);
               }
             }
             float w[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              float score = (MT == 1 && turn ? joined(sc[0], sc[2]) : sc[2 * mt]) * p.scale_log2;
+              float score = (turn ? joined(sc[2 * mt], MT == 1 ? sc[2] : low[2 * mt]) : sc[2 * mt]) * p.scale_log2;
               score = __shfl_sync(0xffffffffu, score, lane & ~3);
               m[mt] = lifted<T>(score);
               // (weights of scores that are no numbers follow the formula: exp(inf - inf) and the like)
@@ -1085,9 +1109,9 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
               cp_async_wait<kStages - 1>();        // one group per unit that was asked for after this one may be open
               __syncwarp();
             }
-            float sc[2][4];
+            float sc[2][4], low[2][4];               // (low: of the queries' lower parts, MT = 2)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[0][e] = sc[1][e] = 0.f;
+            for (int e = 0; e < 4; ++e) sc[0][e] = sc[1][e] = low[0][e] = low[1][e] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
               uint32_t kb[4];
@@ -1097,21 +1121,23 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
               if (MT > 1 && opaque(turn)) {
                 uint32_t q[4];
                 low_query(ks, q);
-                mma16816<T>(sc[0], q, kb[0], kb[1]);
-                mma16816<T>(sc[1], q, kb[2], kb[3]);
+                mma16816<T>(low[0], q, kb[0], kb[1]);
+                mma16816<T>(low[1], q, kb[2], kb[3]);
               }
             }
-            // weights as two 16-bit parts.  One tile: rows 0-7 of a fragment the upper parts, rows 8-15 the lower ones;
+            // weights as 16-bit parts.  One tile: rows 0-7 of a fragment the upper parts, rows 8-15 the lower ones;
             // two: a fragment each, 16 heads.
-            uint32_t pa[MT][4];
+            constexpr int kFragments = MT == 1 ? 1 : kPositiveParts<T>;
+            uint32_t pa[kFragments][4];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
               float s[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) s[e] = sc[e >> 1][(e & 1) + 2 * mt];
-              if (MT == 1 && opaque(turn)) {
+              if (opaque(turn)) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[e] = joined(s[e], sc[e >> 1][(e & 1) + 2]);
+                for (int e = 0; e < 4; ++e)
+                  s[e] = joined(s[e], MT == 1 ? sc[e >> 1][(e & 1) + 2] : low[e >> 1][(e & 1) + 2 * mt]);
               }
 #pragma unroll
               for (int e = 0; e < 4; ++e) s[e] *= p.scale_log2;
@@ -1137,14 +1163,23 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
               }
               const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[e] = exp2f(s[e] - ref);
+              for (int e = 0; e < 4; ++e) {
+                s[e] = exp2f(s[e] - ref);
+                if (std::is_same<T, __half>::value && s[e] > 0.f) s[e] = fmaxf(s[e], 0x1p-24f);
+              }
               l[mt] += (s[0] + s[1]) + (s[2] + s[3]);
               if (MT == 1) {
                 split2<T, false>(s[0], s[1], pa[0][0], pa[0][1]);
                 split2<T, false>(s[2], s[3], pa[0][2], pa[0][3]);
               } else {
-                split2<T, false>(s[0], s[1], pa[0][mt], pa[MT - 1][mt]);
-                split2<T, false>(s[2], s[3], pa[0][mt + 2], pa[MT - 1][mt + 2]);
+                uint32_t w01[kPositiveParts<T>], w23[kPositiveParts<T>];
+                split_positive2<T>(s[0], s[1], w01);
+                split_positive2<T>(s[2], s[3], w23);
+#pragma unroll
+                for (int i = 0; i < kFragments; ++i) {
+                  pa[i][mt] = w01[i];
+                  pa[i][mt + 2] = w23[i];
+                }
               }
             }
 #pragma unroll
@@ -1152,7 +1187,7 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
               uint32_t vb[4];
               ldmatrix4_trans(vb, ((base + v_at) ^ ((j & 3) << 5)) + (j >> 2) * L::kPanelBytes);
 #pragma unroll
-              for (int part16 = 0; part16 < MT; ++part16) {
+              for (int part16 = 0; part16 < kFragments; ++part16) {
                 mma16816<T>(acc[2 * j], pa[part16], vb[0], vb[1]);
                 mma16816<T>(acc[2 * j + 1], pa[part16], vb[2], vb[3]);
               }
