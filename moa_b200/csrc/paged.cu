@@ -11,6 +11,7 @@
 #include <cuda.h>
 
 #include "common.cuh"
+#include "ring.h"
 
 namespace moa {
 namespace {
@@ -232,7 +233,7 @@ __global__ void paged_advance_kernel(int32_t* lengths, const int32_t* counts, in
 // An infinite value with a weight is infinite in the result, so a weight's upper part is never 0 (fp16: 2^-39 of the
 // largest at least), and what a lower part makes of an infinity (0 * inf, or the other sign) must not get into it: it is in
 // a row of its own (MT = 1) or in sums of its own (scores), and where values are summed with MT = 2 all parts are positive,
-// cut off and not rounded, so that bf16 needs three (60 query heads on 5, 69 sequences of 482 tokens: 23.1 -> 24.0 us).
+// cut off and not rounded, so that bf16 needs three (48 query heads on 4, 8 sequences of 16384 tokens: 57.4 -> 61.1 us).
 //
 // The fused step's new token is where one warp of the block that ends the item starts from (its score is the first
 // maximum, its value the first sum); it is stored into its page at the same time and read from no page.
@@ -961,6 +962,7 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
       }
       ld_look();
     };
+    Ring<kStages> loads;
     auto ld_issue = [&](int stage) {
       if (ld_more) {
         const uint32_t dst = ring + stage * L::kStageBytes, bar = bars + stage * 8;
@@ -993,9 +995,7 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
 
     // ---- items
     const int g = lane >> 2, t = lane & 3;         // row (query head of a tile) and column pair of a fragment
-    int stage = 0, buf = 0;
-    uint32_t parity = 0;
-    bool waiting = true;                           // until a wait runs out
+    int buf = 0;
     for (bool more = any; more; buf ^= 1) {
       Cursor<SOLO> next = cur;
       more = next.next(sizes, part);
@@ -1102,9 +1102,11 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
           const uint32_t v_at = L::kTileBytes + ((mi & 1) * 8 + r8) * 128 + (((mi >> 1) ^ r8) << 4);
 #pragma unroll 1
           for (int u = cur.u0 + team.warp; u < cur.u1; u += team.warps) {
-            if (opaque(waiting)) waiting = __all_sync(0xffffffffu, bar_wait(bars + stage * 8, parity));
-            const uint32_t base = ring + stage * L::kStageBytes;
-            const uint32_t present = my_mask[stage];
+            if (opaque(!loads.late))
+              loads.take([&](int at, uint32_t parity) { return __all_sync(0xffffffffu, bar_wait(bars + at * 8, parity)) != 0; });
+            ld_more = ld_more && !loads.late;      // (a late load is reported; the block goes on to its end without others)
+            const uint32_t base = ring + loads.stage() * L::kStageBytes;
+            const uint32_t present = my_mask[loads.stage()];
             if (present & kByHand) {
               cp_async_wait<kStages - 1>();        // one group per unit that was asked for after this one may be open
               __syncwarp();
@@ -1194,11 +1196,8 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
             }
             if (present & kByHand) proxy_fence();
             __syncwarp();
-            ld_issue(stage);
-            if (++stage == kStages) {
-              stage = 0;
-              parity ^= 1;
-            }
+            ld_issue(loads.stage());
+            loads.next();
           }
         }
 
@@ -1278,14 +1277,13 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
       }
       if (more) cur = next;
     }
-    if (!waiting)                                  // a load is late: it must not land in a block that has ended
-      for (int s = 0; s < kStages; ++s) {
-        bar_wait(bars + stage * 8, parity);
-        if (++stage == kStages) {
-          stage = 0;
-          parity ^= 1;
-        }
-      }
+    if (loads.late) {                              // one limit for all stages
+      const long long start = clock64();
+      loads.drain([&](int at, uint32_t parity) {
+        while (!bar_try(bars + at * 8, parity))
+          if (clock64() - start > kWaitCycles) break;
+      });
+    }
   }
 
   if (p.advance) {                                 // the last block to get here: every block has read the lengths
