@@ -224,16 +224,19 @@ __global__ void paged_advance_kernel(int32_t* lengths, const int32_t* counts, in
 // Arithmetic.  m16n8k16 tensor instructions with the 8 query heads of a tile in rows 0-7 and, where an operand
 // does not fit 16 bits, its remainder in rows 8-15: the weights w are held in two 16-bit parts that way (hi + lo),
 // and so is the rotated query of the fused step.  Rows 8-15 would idle otherwise (G is small), so the second part costs
-// nothing.  A weight is off by 2^-23 of itself in fp16 and by 2^-17 in bf16, whose third part would cost products of its
+// nothing.  A weight is off by 2^-22 of itself in fp16 and by 2^-17 in bf16, whose third part would cost products of its
 // own (64 sequences of up to 8192 tokens 174 -> 180 us) and change little: the result is as far from 64 bits with it (1.5e-6
 // against 1.6e-6, of sums in the tensor cores).  fp16 has those bits from 2^-14 on only, so its weights are 2^15 times what
 // they are, sums and records with them, and the factor falls out at the division: steps of 2^-39 of the largest.
-// With 9..16 heads (MT = 2) all rows are heads, and the other parts are products of their own.
+// With 9..16 heads (MT = 2) all rows are heads, and the lower parts are products of their own into the same sums.
 //
-// An infinite value with a weight is infinite in the result, so a weight's upper part is never 0 (fp16: 2^-39 of the
-// largest at least), and what a lower part makes of an infinity (0 * inf, or the other sign) must not get into it: it is in
-// a row of its own (MT = 1) or in sums of its own (scores), and where values are summed with MT = 2 all parts are positive,
-// cut off and not rounded, so that bf16 needs three (48 query heads on 4, 8 sequences of 16384 tokens: 57.4 -> 61.1 us).
+// An infinite value with a weight is infinite in the result, and a token with a score of -infinity has none.  So a weight's
+// upper part is never 0 (fp16: 2^-39 of the largest at least), and what a lower part makes of an infinity (0 * inf, or the
+// other sign) must not get into the sum: with MT = 1 it is in a row of its own.  With MT = 2 the lower part has the sign of
+// the upper one, which is cut off and not rounded, and is not 0: that costs rotated queries in bf16 a bit (2^-16).  Only the
+// weights in bf16 stay rounded, and their lower part meets the largest finite number in place of an infinity.  (38 sequences
+// of up to 35129 tokens, 64 heads of 64 on 4: bf16 162 -> 165 us, with a third part instead 184; fp16 166 -> 167, with finite
+// numbers instead 172; finite numbers for keys too: 10 % more in the step.)
 //
 // The fused step's new token is where one warp of the block that ends the item starts from (its score is the first
 // maximum, its value the first sum); it is stored into its page at the same time and read from no page.
@@ -483,25 +486,43 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_
   const float2 h = Cvt<T>::unpack(hi);
   lo = Cvt<T>::pack(x0 - h.x, x1 - h.y);
 }
-// x as a sum of positive numbers in T, for two values from 0 on.  (Of 0 itself the parts are 0, in bf16 the second and
-// third the least normal number.)
+// The same with hi cut off, so that lo has its sign, and lo not 0 (unless x is): hi is one step less where x fits it.
 template <typename T>
-constexpr int kPositiveParts = std::is_same<T, __half>::value ? 2 : 3;
-template <typename T>
-__device__ __forceinline__ void split_positive2(float x0, float x1, uint32_t (&part)[kPositiveParts<T>]) {
+__device__ __forceinline__ void split_one_sign(float x, uint16_t& hi, uint16_t& lo) {
   if constexpr (std::is_same<T, __half>::value) {
-    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(part[0]) : "f"(x1), "f"(x0));
-    const float2 h = Cvt<T>::unpack(part[0]);
-    part[1] = Cvt<T>::pack(fmaxf(x0 - h.x, fminf(x0, 0x1p-24f)), fmaxf(x1 - h.y, fminf(x1, 0x1p-24f)));
-  } else {                                         // eight bits a part: the upper halves of what is left
-#pragma unroll
-    for (int i = 0; i < kPositiveParts<T>; ++i) {
-      part[i] = __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
-      const float2 h = Cvt<T>::unpack(part[i]);
-      x0 = fmaxf(x0 - h.x, 0x1p-126f);
-      x1 = fmaxf(x1 - h.y, 0x1p-126f);
-    }
+    hi = __half_as_ushort(__float2half_rz(x));
+    lo = __half_as_ushort(__float2half_rn(x - __half2float(__ushort_as_half(hi))));
+    if ((lo & 0x7fff) == 0 && (hi & 0x7fff) > 1) lo = __half_as_ushort(__float2half_rn(x - __half2float(__ushort_as_half(--hi))));
+  } else {
+    hi = (uint16_t)(__float_as_uint(x) >> 16);
+    lo = __bfloat16_as_ushort(__float2bfloat16_rn(x - __uint_as_float((uint32_t)hi << 16)));
+    if ((lo & 0x7fff) == 0 && (hi & 0x7fff) > 1) lo = __bfloat16_as_ushort(__float2bfloat16_rn(x - __uint_as_float((uint32_t)--hi << 16)));
   }
+}
+template <typename T>
+__device__ __forceinline__ void split_one_sign2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  uint16_t h0, l0, h1, l1;
+  split_one_sign<T>(x0, h0, l0);
+  split_one_sign<T>(x1, h1, l1);
+  hi = h0 | (uint32_t)h1 << 16;
+  lo = l0 | (uint32_t)l1 << 16;
+}
+// Two weights as hi + lo for sums that hold both.  fp16: positive, and only of 0 itself 0 (from 2^-24 on a weight is one
+// step at least); bf16 is rounded, its lo to be multiplied with finite2(value).
+template <typename T>
+__device__ __forceinline__ void split_weights2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  if constexpr (std::is_same<T, __half>::value) {
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(x1), "f"(x0));
+    const float2 h = Cvt<T>::unpack(hi);
+    lo = Cvt<T>::pack(fmaxf(x0 - h.x, fminf(x0, 0x1p-24f)), fmaxf(x1 - h.y, fminf(x1, 0x1p-24f)));
+  } else {
+    split2<T, false>(x0, x1, hi, lo);
+  }
+}
+// Two bf16 whose infinities have given way to the largest number.
+__device__ __forceinline__ uint32_t finite2(uint32_t v) {
+  asm("min.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(0x7f7f7f7fu));
+  return v;
 }
 // hi + lo of a sum that was split; an infinity of hi is the result (its lo is inf - inf or 0 * inf).
 __device__ __forceinline__ float joined(float hi, float lo) { return isinf(hi) ? hi : hi + lo; }
@@ -615,8 +636,15 @@ __device__ __forceinline__ void turn_queries(const DecodeParams& p, const TEAM& 
     const float2 a = Cvt<T>::unpack(q[d / 2]), b = Cvt<T>::unpack(q[(d + D / 2) / 2]);
     const float2 cl = table2<T>(item + L::kCos, d, f32), ch = table2<T>(item + L::kCos, d + D / 2, f32);
     const float2 sl = table2<T>(item + L::kSin, d, f32), sh = table2<T>(item + L::kSin, d + D / 2, f32);
-    split2<T, true>(fmaf(a.x, cl.x, -b.x * sl.x), fmaf(a.y, cl.y, -b.y * sl.y), q[d / 2], r[d / 2]);
-    split2<T, true>(fmaf(b.x, ch.x, a.x * sh.x), fmaf(b.y, ch.y, a.y * sh.y), q[(d + D / 2) / 2], r[(d + D / 2) / 2]);
+    const float2 lo = make_float2(fmaf(a.x, cl.x, -b.x * sl.x), fmaf(a.y, cl.y, -b.y * sl.y));
+    const float2 hi = make_float2(fmaf(b.x, ch.x, a.x * sh.x), fmaf(b.y, ch.y, a.y * sh.y));
+    if (MT == 1) {
+      split2<T, true>(lo.x, lo.y, q[d / 2], r[d / 2]);
+      split2<T, true>(hi.x, hi.y, q[(d + D / 2) / 2], r[(d + D / 2) / 2]);
+    } else {
+      split_one_sign2<T>(lo.x, lo.y, q[d / 2], r[d / 2]);
+      split_one_sign2<T>(hi.x, hi.y, q[(d + D / 2) / 2], r[(d + D / 2) / 2]);
+    }
   }
 }
 
@@ -1064,7 +1092,7 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
           auto low_query = [&](int ks, uint32_t(&q)[4]) { ldmatrix4(q, low_at + ((lane & 8) ? q_8 : 0) + ks * 32); };
           if (with_new && team.warp == 0) {        // start from the new token: column 0 of a tile of keys, weight 1
             const uint32_t* key = reinterpret_cast<const uint32_t*>(item + L::kKey);
-            float sc[4] = {0.f, 0.f, 0.f, 0.f}, low[4] = {0.f, 0.f, 0.f, 0.f};
+            float sc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
               const uint32_t k0 = g == 0 ? key[ks * 8 + t] : 0u, k1 = g == 0 ? key[ks * 8 + 4 + t] : 0u;
@@ -1072,13 +1100,13 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
               if (MT > 1 && turn) {
                 uint32_t q[4];
                 low_query(ks, q);
-                mma16816<T>(low, q, k0, k1);
+                mma16816<T>(sc, q, k0, k1);
               }
             }
             float w[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              float score = (turn ? joined(sc[2 * mt], MT == 1 ? sc[2] : low[2 * mt]) : sc[2 * mt]) * p.scale_log2;
+              float score = (MT == 1 && turn ? joined(sc[0], sc[2]) : sc[2 * mt]) * p.scale_log2;
               score = __shfl_sync(0xffffffffu, score, lane & ~3);
               m[mt] = lifted<T>(score);
               // (weights of scores that are no numbers follow the formula: exp(inf - inf) and the like)
@@ -1105,15 +1133,15 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
             if (opaque(!loads.late))
               loads.take([&](int at, uint32_t parity) { return __all_sync(0xffffffffu, bar_wait(bars + at * 8, parity)) != 0; });
             ld_more = ld_more && !loads.late;      // (a late load is reported; the block goes on to its end without others)
-            const uint32_t base = ring + loads.stage() * L::kStageBytes;
-            const uint32_t present = my_mask[loads.stage()];
+            const uint32_t base = ring + loads.stage * L::kStageBytes;
+            const uint32_t present = my_mask[loads.stage];
             if (present & kByHand) {
               cp_async_wait<kStages - 1>();        // one group per unit that was asked for after this one may be open
               __syncwarp();
             }
-            float sc[2][4], low[2][4];               // (low: of the queries' lower parts, MT = 2)
+            float sc[2][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[0][e] = sc[1][e] = low[0][e] = low[1][e] = 0.f;
+            for (int e = 0; e < 4; ++e) sc[0][e] = sc[1][e] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
               uint32_t kb[4];
@@ -1123,23 +1151,21 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
               if (MT > 1 && opaque(turn)) {
                 uint32_t q[4];
                 low_query(ks, q);
-                mma16816<T>(low[0], q, kb[0], kb[1]);
-                mma16816<T>(low[1], q, kb[2], kb[3]);
+                mma16816<T>(sc[0], q, kb[0], kb[1]);
+                mma16816<T>(sc[1], q, kb[2], kb[3]);
               }
             }
-            // weights as 16-bit parts.  One tile: rows 0-7 of a fragment the upper parts, rows 8-15 the lower ones;
+            // weights as two 16-bit parts.  One tile: rows 0-7 of a fragment the upper parts, rows 8-15 the lower ones;
             // two: a fragment each, 16 heads.
-            constexpr int kFragments = MT == 1 ? 1 : kPositiveParts<T>;
-            uint32_t pa[kFragments][4];
+            uint32_t pa[MT][4];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
               float s[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) s[e] = sc[e >> 1][(e & 1) + 2 * mt];
-              if (opaque(turn)) {
+              if (MT == 1 && opaque(turn)) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  s[e] = joined(s[e], MT == 1 ? sc[e >> 1][(e & 1) + 2] : low[e >> 1][(e & 1) + 2 * mt]);
+                for (int e = 0; e < 4; ++e) s[e] = joined(s[e], sc[e >> 1][(e & 1) + 2]);
               }
 #pragma unroll
               for (int e = 0; e < 4; ++e) s[e] *= p.scale_log2;
@@ -1174,14 +1200,8 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
                 split2<T, false>(s[0], s[1], pa[0][0], pa[0][1]);
                 split2<T, false>(s[2], s[3], pa[0][2], pa[0][3]);
               } else {
-                uint32_t w01[kPositiveParts<T>], w23[kPositiveParts<T>];
-                split_positive2<T>(s[0], s[1], w01);
-                split_positive2<T>(s[2], s[3], w23);
-#pragma unroll
-                for (int i = 0; i < kFragments; ++i) {
-                  pa[i][mt] = w01[i];
-                  pa[i][mt + 2] = w23[i];
-                }
+                split_weights2<T>(s[0], s[1], pa[0][mt], pa[MT - 1][mt]);
+                split_weights2<T>(s[2], s[3], pa[0][mt + 2], pa[MT - 1][mt + 2]);
               }
             }
 #pragma unroll
@@ -1189,14 +1209,17 @@ __global__ void __launch_bounds__(Layout<D, MT, SOLO>::kThreads, kPerSm)
               uint32_t vb[4];
               ldmatrix4_trans(vb, ((base + v_at) ^ ((j & 3) << 5)) + (j >> 2) * L::kPanelBytes);
 #pragma unroll
-              for (int part16 = 0; part16 < kFragments; ++part16) {
+              for (int part16 = 0; part16 < MT; ++part16) {
+                if (part16 == 1 && std::is_same<T, __nv_bfloat16>::value)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) vb[i] = finite2(vb[i]);
                 mma16816<T>(acc[2 * j], pa[part16], vb[0], vb[1]);
                 mma16816<T>(acc[2 * j + 1], pa[part16], vb[2], vb[3]);
               }
             }
             if (present & kByHand) proxy_fence();
             __syncwarp();
-            ld_issue(loads.stage());
+            ld_issue(loads.stage);
             loads.next();
           }
         }

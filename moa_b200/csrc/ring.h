@@ -17,22 +17,19 @@ namespace moa {
 // `wait(stage, parity)` waits for the phase of that parity, with a limit, and is false when it ran out.  From then on the
 // ring is late and stays where it is: nothing may be taken or armed any more, for a barrier whose phase is open cannot
 // take another load's, nor its buffer another load.
-// (One counter and a number, no branches: a stage, a parity and a flag take registers that the kernel's loop has not got,
-// 64 instead of 60 us for 8 sequences of 16384 tokens, 48 query heads on 4.)
 template <int kStages>
 struct Ring {
-  static_assert((kStages & (kStages - 1)) == 0, "stages are counted modulo a power of two");
-  uint32_t count = 0;       // stages taken
-  int late = 0;             // 1: a wait ran out
-
-  MOA_RING_FN int stage() const { return (int)(count % kStages); }            // taken next
-  MOA_RING_FN uint32_t parity() const { return count / kStages & 1; }         // of its barrier's phase
+  int stage = 0;            // taken next
+  uint32_t parity = 0;      // of its barrier's phase
+  bool late = false;
 
   template <typename Wait>
   MOA_RING_FN void take(Wait wait) {
-    late = wait(stage(), parity()) ? 0 : 1;
+    late = !wait(stage, parity);
   }
-  MOA_RING_FN void next() { count += 1 - late; }
+  MOA_RING_FN void next() {
+    if (!late) advance();
+  }
   // At the end: a late ring's loads under way, from the one that was waited for in vain on, are waited for once more, so
   // that none of them lands in a block that has ended.  (Which stages were armed is not noted: for those that were not,
   // the wait runs out.)
@@ -40,8 +37,16 @@ struct Ring {
   MOA_RING_FN void drain(Wait wait) {
 #pragma unroll 1
     for (int s = 0; s < kStages; ++s) {
-      wait(stage(), parity());
-      ++count;
+      wait(stage, parity);
+      advance();
+    }
+  }
+
+ private:
+  MOA_RING_FN void advance() {
+    if (++stage == kStages) {
+      stage = 0;
+      parity ^= 1;
     }
   }
 };

@@ -226,7 +226,8 @@ def paged_decode(query: Tensor, key_pages: Tensor, value_pages: Tensor, page_tab
     ``h // (H // KV)``.  Pool, ``page_table`` and ``lengths`` as in ``paged_append``.  Returns ``(B, 1, H, D)`` (into
     ``out`` if given, whose rows must be 16-byte aligned) in the query's dtype, or float32 with ``out_dtype=torch.float32`` (the
     result before that rounding).  Scores, maxima and sums are fp32; a weight is held to 2^-22 of itself in fp16 (and 2^-39
-    of the largest) and to 2^-17 of itself in bf16.
+    of the largest) and to 2^-17 of itself in bf16, the coordinates of a rotated query to 2^-22 (and 2^-25) and to 2^-16.
+    Infinite values and keys give what the formula gives.
 
     ``sink_size, local_size``: int64 ``(KV,)`` in tokens, both or none; a head then attends only the first
     ``sink_size`` and last ``local_size`` tokens of a sequence (what a ring cache of that size holds), and only

@@ -53,13 +53,13 @@ int run(int units, int late, int needs) {
   for (int s = 0; s < kStages; ++s) issue(s);
   for (int u = 0; u < units; ++u) {            // the warp goes through all its units, late or not
     if (!ring.late) {
-      const int stage = ring.stage();
+      const int stage = ring.stage;
       if (bars[stage].unit != u) fail("another unit's stage");
       ring.take(wait);
       if (ring.late) more = false;
       else ++taken;
     }
-    issue(ring.stage());
+    issue(ring.stage);
     ring.next();
   }
   const bool was_late = ring.late;
@@ -98,10 +98,10 @@ def test_ring_arms_takes_and_drains(tmp_path):
 
 
 @pytest.mark.parametrize("right,wrong,what", [
-    ("late = wait(stage(), parity()) ? 0 : 1;", "wait(stage(), parity());", "armed while|without a wait"),   # on as if nothing were
-    ("count += 1 - late;", "++count;", "phase that is over|without a wait"),
+    ("late = !wait(stage, parity);", "wait(stage, parity);", "armed while|without a wait"),     # on as if nothing had happened
+    ("if (!late) advance();", "advance();", "phase that is over|without a wait"),
     ("for (int s = 0; s < kStages; ++s) {", "for (int s = 1; s < kStages; ++s) {", "without a wait|waits"),
-    ("count / kStages & 1", "count / kStages + 1 & 1", "phase that is over"),
+    ("parity ^= 1;", "", "phase that is over"),
 ])
 def test_the_model_sees_mistakes(tmp_path, right, wrong, what):
     text = open(os.path.join(CSRC, "ring.h")).read()
