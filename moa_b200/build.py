@@ -1,4 +1,4 @@
-"""Builds libmoa_b200.so (the C-ABI library) in-tree with nvcc for sm_100a, and _paged_host.so beside it.
+"""Builds libmoa_b200.so (the C-ABI library) in-tree with nvcc for sm_100a, and _paged_host.*.so beside it.
 
     python moa_b200/build.py [--force] [--verbose]
 
@@ -8,19 +8,37 @@ package loads it with ctypes.  nvcc cross-compiles, so no GPU is needed to build
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
+import sysconfig
+import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmoa_b200.so")
 SOURCES = ["errors.cu", "decode.cu", "cache.cu", "prefill.cu", "peer.cu", "paged.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-#: the host's share of the paged calls, compiled against the installed torch (moa_b200/paged.py does without it, slower)
-HOST = os.path.join(HERE, "_paged_host.so")
 HOST_SOURCE = os.path.join(CSRC, "paged_host.cpp")
+HEADER = os.path.join(HERE, "..", "include", "moa_b200.h")
+
+
+def _torch_version() -> str:
+    """Of the installed torch, without importing it; empty where there is none."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return ""
+    with open(os.path.join(os.path.dirname(spec.origin), "version.py")) as f:
+        found = re.search(r"^__version__ = '(.*)'", f.read(), flags=re.M)
+    return found.group(1) if found else ""
+
+
+#: the host's share of the paged calls, compiled against the installed torch (moa_b200/paged.py does without it, slower); it
+#: reads torch's objects in place, so its name says which Python and torch it is for and no other ones load it
+HOST = os.path.join(HERE, f"_paged_host.{sys.implementation.cache_tag}-torch{_torch_version()}.so")
 
 
 def _nvcc() -> str:
@@ -30,18 +48,29 @@ def _nvcc() -> str:
     raise RuntimeError("nvcc not found; set NVCC or put it on PATH")
 
 
-def _stale() -> bool:
-    if not os.path.exists(LIB) or not os.path.exists(HOST):
-        return True
-    t = min(os.path.getmtime(LIB), os.path.getmtime(HOST))
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(HERE, "..", "include", "moa_b200.h")]
-    return any(os.path.getmtime(d) > t for d in deps)
+def _stale(made: str, sources) -> bool:
+    return not os.path.exists(made) or any(os.path.getmtime(d) > os.path.getmtime(made) for d in sources)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile every .cu under csrc/ into libmoa_b200.so; returns the library path."""
-    if not force and not _stale():
-        return LIB
+    """Compile every .cu under csrc/ into libmoa_b200.so, and the host part where that is possible; returns the library's
+    path."""
+    kernels = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if os.path.join(CSRC, f) != HOST_SOURCE]
+    if force or _stale(LIB, kernels + [HEADER]):
+        _build_library(verbose)
+    if force or _stale(HOST, [HOST_SOURCE, HEADER]):
+        if os.path.exists(HOST):
+            os.remove(HOST)                       # should the new one fail, the old one's arguments may no longer fit
+        try:
+            build_host(verbose)
+        except (OSError, subprocess.CalledProcessError) as e:
+            why = f"exit status {e.returncode}" if isinstance(e, subprocess.CalledProcessError) else e
+            warnings.warn(f"the host part of the paged calls was not built ({why}): each takes some ten microseconds more "
+                          "from Python", RuntimeWarning, stacklevel=2)
+    return LIB
+
+
+def _build_library(verbose: bool) -> None:
     objs = []
     os.makedirs(os.path.join(HERE, "build"), exist_ok=True)
     for src in SOURCES:
@@ -57,17 +86,14 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
-    build_host(verbose)
-    return LIB
 
 
 def build_host(verbose: bool = False) -> str:
     """Compile csrc/paged_host.cpp with the host compiler against the installed torch."""
-    import sysconfig
-
-    import torch
-
-    base = os.path.dirname(torch.__file__)
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise FileNotFoundError("torch is not installed")
+    base = os.path.dirname(spec.origin)
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
            *("-I" + d for d in (os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),

@@ -263,4 +263,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_paged_host", nullptr, -1, methods
 
 }  // namespace
 
-extern "C" PyObject* PyInit__paged_host() { return PyModule_Create(&module); }
+// `abi`: of the library whose argument structs are compiled in.
+extern "C" PyObject* PyInit__paged_host() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddIntConstant(m, "abi", MOA_ABI_VERSION) != 0) Py_CLEAR(m);
+  return m;
+}

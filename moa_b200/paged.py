@@ -9,7 +9,10 @@ from __future__ import annotations
 
 import copy
 import ctypes
+import importlib.util
+import os
 import struct
+import sys
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -32,15 +35,29 @@ _MANY, _SHORT = 296, 256
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or _lib.current_stream
 _capturing = torch.cuda.is_current_stream_capturing
 
-try:
-    from . import _paged_host as _host       # the common case of both calls, compiled (csrc/paged_host.cpp)
-except ImportError:                          # not built against this torch: the same calls, from Python alone
-    _host = None
-if _host is not None:
-    _host.init(ctypes.cast(lib.moa_paged_append, ctypes.c_void_p).value,
-               ctypes.cast(lib.moa_paged_decode, ctypes.c_void_p).value)
-if _lib.NVTX:
-    _host = None                             # ranges are marked from Python
+#: the common case of both calls, compiled (csrc/paged_host.cpp) for one Python and one torch, as its name says
+HOST_PATH = os.path.join(_lib.HERE, f"_paged_host.{sys.implementation.cache_tag}-torch{torch.__version__}.so")
+
+
+def _load_host():
+    """The compiled part, or None where there is none for this Python, torch and library: the same calls are then made
+    from Python alone."""
+    if not os.path.exists(HOST_PATH):
+        return None
+    spec = importlib.util.spec_from_file_location("moa_b200._paged_host", HOST_PATH)
+    try:
+        host = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(host)
+    except ImportError:
+        return None
+    if getattr(host, "abi", None) != _lib.ABI_VERSION:
+        return None
+    host.init(ctypes.cast(lib.moa_paged_append, ctypes.c_void_p).value,
+              ctypes.cast(lib.moa_paged_decode, ctypes.c_void_p).value)
+    return host
+
+
+_host = None if _lib.NVTX else _load_host()      # (ranges are marked from Python)
 
 _workspaces: Dict = {}
 _touched = set()      # devices that a paged call has run on

@@ -13,7 +13,7 @@ INF = float("inf")
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("D,G", [(64, 1), (64, 9), (64, 16), (128, 8), (128, 12)])
 @pytest.mark.parametrize("form", ["blocks", "warps"])
-@pytest.mark.parametrize("call", ["attend", "step", "turned step"])
+@pytest.mark.parametrize("call", ["attend", "step", "turned step", "step turned by nothing"])
 def test_infinite_values_and_keys(dtype, D, G, form, call):
     B, KV, page = (150, 2, 16) if form == "warps" else (7, 2, 16)
     n, width = (200, 16) if form == "warps" else (611, 48)
@@ -35,8 +35,8 @@ def test_infinite_values_and_keys(dtype, D, G, form, call):
         k, v = c.normal(B, KV, 1, D) * 0.1, c.normal(B, KV, 1, D)
         v[:, 0, :, 12] = -INF
         args, length = dict(key=k, value=v), c.lengths + 1
-        if call == "turned step":
-            args["rope"] = tables(D, torch.arange(n + 1), torch.float32)
+        if call not in ("attend", "step"):                # (turned by nothing: queries have no part beyond 16 bits)
+            args["rope"] = tables(D, torch.arange(n + 1) * (call == "turned step"), torch.float32)
             cos, sin = (t[n] for t in args["rope"])
             qr = rotated64(q, cos, sin)[0]
             assert qr[..., slow].min() > 0.5
