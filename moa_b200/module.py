@@ -67,6 +67,9 @@ def apply_rotary_pos_emb(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor) -> Tupl
     return q, k
 
 
+_NO_GATHER = "the fused gather delivers the rows of ring caches only"
+
+
 class MoAAttention(nn.Module):
     """Multi-head attention with per-head sink + sliding-window spans.
 
@@ -119,6 +122,8 @@ class MoAAttention(nn.Module):
         """Projection, rotary embedding, cache update and attention of this module's heads:
         ``(B, q, hidden) -> (B, q, H_local, D)`` (everything of ``forward`` before the gather and ``o_proj``).
         ``out`` (decode only) may be a ``(B, 1, H_local, D)`` slice of a gather buffer."""
+        if self.peer_gather is not None and isinstance(past_key_value, PagedCache):     # (its decode steps would be refused)
+            raise NotImplementedError(_NO_GATHER)
         bsz, q_len, _ = hidden_states.shape
         H, D = self.num_local_heads, self.head_dim
         qkv = torch.nn.functional.linear(hidden_states, self.fused_qkv_weight()).view(bsz, q_len, 3, H, D)
@@ -127,8 +132,6 @@ class MoAAttention(nn.Module):
         sm_scale = D ** -0.5
         if q_len == 1:
             # one launch: rotary embedding of q and k, ring append, flash-decoding, bookkeeping
-            if self.peer_gather is not None and isinstance(past_key_value, PagedCache):
-                raise NotImplementedError("the fused gather delivers the rows of ring caches only")
             if self.peer_gather is not None:    # ... and delivery of the rows to every rank: (B, 1, H, D) comes back
                 return self.peer_gather.decode_and_gather(past_key_value, q, k, v, self.layer_idx, sm_scale,
                                                           rope=(cos, sin))
@@ -484,6 +487,8 @@ class DecodeGraph:
         device, B = base.device, cache.batch_size
         self.paged = isinstance(cache, PagedCache)
         if self.paged:
+            if any(l.self_attn.peer_gather is not None for l in base.layers):
+                raise NotImplementedError(_NO_GATHER)
             self._capture_paged(device, B)
             return
         for layer in range(cache.num_layers):

@@ -62,3 +62,22 @@ def test_update_refuses_tokens_that_no_slot_can_take():
     # one of them can: rows of idle slots are left alone
     with pytest.raises(RuntimeError, match="CUDA"):
         cache.update(k, k, 0)
+
+
+@pytest.mark.parametrize("tokens", [1, 5])
+def test_the_fused_gather_refuses_pages_before_anything_is_stored(tokens):
+    cache = _cache()
+    before = _state(cache)
+    with pytest.raises(NotImplementedError, match="ring caches"):
+        _attend(_attention(peer_gather=object()), cache, tokens)
+    assert _state(cache) == before
+
+
+def test_a_graph_over_pages_is_refused_with_the_fused_gather_before_pages_are_taken():
+    model = moa_b200.MoALlamaModel(num_layers=2, hidden_size=128, num_heads=2, intermediate_size=64, vocab_size=11, device="cpu")
+    model.layers[1].self_attn.peer_gather = object()
+    cache = _cache()
+    before = _state(cache)
+    with pytest.raises(NotImplementedError, match="ring caches"):
+        moa_b200.DecodeGraph(model, cache)
+    assert _state(cache) == before
