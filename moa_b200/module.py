@@ -520,12 +520,14 @@ class DecodeGraph:
         stream = torch.cuda.Stream(device)
         stream.wait_stream(torch.cuda.current_stream(device))
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph, stream=stream):
-            self.out, _ = self.model(self.ids, past_key_values=cache)
+        try:
+            with torch.cuda.graph(self.graph, stream=stream):
+                self.out, _ = self.model(self.ids, past_key_values=cache)
+        finally:
+            # capturing runs the host side without executing anything, up to where it raises: take the host's counts back
+            for row, was in zip(cache._tokens, counted):
+                row[:] = was
         torch.cuda.current_stream(device).wait_stream(stream)
-        # capturing ran the host side once without executing anything: take the host's counts back
-        for row, was in zip(cache._tokens, counted):
-            row[:] = was
 
     @torch.no_grad()
     def step(self, input_ids: Tensor) -> Tensor:

@@ -81,3 +81,42 @@ def test_a_graph_over_pages_is_refused_with_the_fused_gather_before_pages_are_ta
     with pytest.raises(NotImplementedError, match="ring caches"):
         moa_b200.DecodeGraph(model, cache)
     assert _state(cache) == before
+
+
+def test_a_capture_that_fails_leaves_the_lengths_as_they_were(monkeypatch):
+    """The host counts a captured step's tokens and takes them back; also when the step raises half way."""
+    import contextlib
+
+    class Stream:
+        def __init__(self, device=None):
+            pass
+
+        def wait_stream(self, other):
+            pass
+
+    monkeypatch.setattr(torch.cuda, "Stream", Stream)
+    monkeypatch.setattr(torch.cuda, "current_stream", Stream)
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", object)
+    monkeypatch.setattr(torch.cuda, "graph", lambda graph, stream=None: contextlib.nullcontext())
+    cache = moa_b200.PagedCache(2, 2, 8, 2, 64, 64, 16, device="cpu")
+    cache.reserve([3, 16])
+    for layer in range(2):
+        cache._count(layer, [3, 16])
+
+    class Model:
+        device, layers, fails = torch.device("cpu"), [], True
+
+        def __call__(self, ids, past_key_values):
+            past_key_values._count(0, [1, 1])
+            if self.fails:
+                raise ValueError("layer 1")
+            past_key_values._count(1, [1, 1])
+            return ids, past_key_values
+
+    model = Model()
+    with pytest.raises(ValueError, match="layer 1"):
+        moa_b200.DecodeGraph(model, cache)
+    assert [cache.sequence_lengths(layer) for layer in range(2)] == [[3, 16]] * 2
+    model.fails = False
+    moa_b200.DecodeGraph(model, cache)
+    assert [cache.sequence_lengths(layer) for layer in range(2)] == [[3, 16]] * 2
