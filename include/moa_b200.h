@@ -251,7 +251,7 @@ int moa_rope_qk(void* q, void* k, int64_t sb, int64_t sh, int64_t sn, const void
  *   k_pages, v_pages  element (page, head, slot, d) at page*xp_page + head*xp_head + slot*xp_slot + d: both
  *                     (pages, heads, slots, D) and (pages, slots, heads, D) memory orders, and pools that
  *                     interleave keys and values, are strides.  16-byte aligned, strides multiples of 8
- *   page_table        int32, row b at page_table + b*table_stride, max_pages entries.  Entries that hold no
+ *   page_table        int32 (this and the other index arrays aligned to their type), row b at page_table + b*table_stride, max_pages entries.  Entries that hold no
  *                     token are never read through (they may be anything, -1 for instance)
  *   lengths           (B) int32, tokens in the pages before the call.  Advanced by the call when `advance` is
  *                     set, else left as they are
@@ -283,7 +283,7 @@ int moa_rope_qk(void* q, void* k, int64_t sb, int64_t sh, int64_t sn, const void
  *   k_new, v_new NULL: n = lengths[b].  Given, (B, KV, D) through their strides: the new token is stored at
  *   position lengths[b] and attended, n = lengths[b] + 1 (lengths[b] < 0: no sequence, nothing is stored and the
  *   output row is zero); with tables q and k_new are rotated, and the key is attended as it is stored.
- *   workspace: moa_paged_decode_workspace_bytes() bytes on the current device, the first
+ *   workspace: moa_paged_decode_workspace_bytes() bytes on the current device, 16-byte aligned, the first
  *   MOA_PAGED_COUNTER_BYTES of them zeroed once; the kernel leaves them zero.  Calls that can overlap in time
  *   need one each.
  * Both take their arguments as a struct of 8-byte fields and read it before they return.

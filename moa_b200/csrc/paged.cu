@@ -1411,7 +1411,8 @@ int launch_decode(DecodeParams& p, int D, int grid, cudaStream_t stream) {
   return p.G > 8 ? launch_decode<T, 64, 2>(p, grid, stream) : launch_decode<T, 64, 1>(p, grid, stream);
 }
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned(const void* p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+inline bool aligned16(const void* p) { return aligned(p, 16); }
 inline bool multiples_of_8(std::initializer_list<int64_t> strides) {
   for (int64_t s : strides)
     if (s % 8 != 0 || s < 0) return false;
@@ -1431,6 +1432,7 @@ int make_pool(const A& a, Pool& p) {
   MOA_REQUIRE(aligned16(a.k_pages) && aligned16(a.v_pages) &&
                   multiples_of_8({a.kp_page, a.kp_head, a.kp_slot, a.vp_page, a.vp_head, a.vp_slot}),
               "paged: pages must be 16-byte aligned with strides that are multiples of 8 elements");
+  MOA_REQUIRE(aligned(a.page_table, 4) && aligned(a.lengths, 4), "paged: page_table and lengths must be 4-byte aligned");
   MOA_REQUIRE((a.rope_cos == nullptr) == (a.rope_sin == nullptr), "paged: rope_cos and rope_sin go together");
   if (a.rope_cos) {
     MOA_REQUIRE(aligned16(a.rope_cos) && aligned16(a.rope_sin) && multiples_of_8({a.rope_sb, a.rope_sn}) && a.rope_rows >= 0,
@@ -1476,6 +1478,7 @@ int moa_paged_append(const moa_paged_append_args* args, moa_stream_t stream) {
   MOA_REQUIRE(aligned16(a.k) && aligned16(a.v) && aligned16(a.q) && aligned16(a.q_out) && aligned16(a.k_out) &&
                   multiples_of_8({a.k_sb, a.k_sh, a.k_sn, a.v_sb, a.v_sh, a.v_sn, a.q_sb, a.q_sh, a.q_sn}),
               "paged_append: rows must be 16-byte aligned with strides that are multiples of 8 elements");
+  MOA_REQUIRE(aligned(a.counts, 4), "paged_append: counts must be 4-byte aligned");
   p.k = a.k; p.v = a.v; p.q = a.q; p.lengths = a.lengths; p.counts = a.counts; p.q_out = a.q_out; p.k_out = a.k_out;
   p.k_sb = a.k_sb; p.k_sh = a.k_sh; p.k_sn = a.k_sn; p.v_sb = a.v_sb; p.v_sh = a.v_sh; p.v_sn = a.v_sn;
   p.q_sb = a.q_sb; p.q_sh = a.q_sh; p.q_sn = a.q_sn;
@@ -1524,6 +1527,8 @@ int moa_paged_decode(const moa_paged_decode_args* args, moa_stream_t stream) {
               "paged_decode: rows must be 16-byte aligned with strides that are multiples of 8 elements");
   MOA_REQUIRE(aligned16(a.out) && multiples_of_8({a.o_sb, a.o_sh}),
               "paged_decode: rows of out must be 16-byte aligned with strides that are multiples of 8 elements");
+  MOA_REQUIRE(aligned(a.sink_size, 8) && aligned(a.local_size, 8), "paged_decode: sink_size and local_size must be 8-byte aligned");
+  MOA_REQUIRE(aligned16(a.workspace), "paged_decode: workspace must be 16-byte aligned");
   if (!a.workspace || a.workspace_bytes < moa_paged_decode_workspace_bytes()) {
     set_error_text("paged_decode: workspace missing or smaller than moa_paged_decode_workspace_bytes()");
     return MOA_ERR_WORKSPACE;

@@ -120,3 +120,18 @@ def test_a_capture_that_fails_leaves_the_lengths_as_they_were(monkeypatch):
     model.fails = False
     moa_b200.DecodeGraph(model, cache)
     assert [cache.sequence_lengths(layer) for layer in range(2)] == [[3, 16]] * 2
+
+
+@pytest.mark.parametrize("entry,changes", [
+    ("append", dict(page_table=2)), ("append", dict(lengths=2)), ("append", dict(counts=2)),
+    ("decode", dict(page_table=2)), ("decode", dict(lengths=1)), ("decode", dict(sink_size=4, local_size=0)),
+    ("decode", dict(sink_size=0, local_size=4)), ("decode", dict(workspace=8)),
+])
+def test_the_c_entries_refuse_addresses_that_a_kernel_cannot_read_at(entry, changes):
+    from moa_b200 import _lib, paged
+    from test_paged_cpu import A, APPEND_OK, DECODE_OK, _call_c
+
+    good, packer = (APPEND_OK, paged._APPEND) if entry == "append" else (DECODE_OK, paged._DECODE)
+    at = {name: A + off for name, off in changes.items()}
+    assert _call_c("paged_" + entry, packer, good, **at) == 1
+    assert b"aligned" in _lib.lib.moa_last_error_detail()
