@@ -512,11 +512,15 @@ class PagedCache:
                          out_dtype: Optional[torch.dtype] = None) -> Tensor:
         """One decode step of one layer in one launch, as ``StaticCircularCache.decode_attention``: rotate, append and
         attend over every slot's sequence with its new token.  ``rope``: this step's tables, ``(B, 1, D)`` or
-        ``(B, D)``.  Rows of idle slots are zero.  A captured call replays on any lengths for which pages are
+        ``(B, D)``.  Rows of idle slots are zero; it is an error when every slot is idle.  A captured call replays on any lengths for which pages are
         reserved; the host's count is then the replayer's to keep (``DecodeGraph`` does)."""
         assert layer_idx < self.num_layers
         B = self.batch_size
         assert query_states.dtype == self.dtype and query_states.device == self.device, "states and cache must be alike"
+        # (the first slot is looked at alone; a captured step is for the lengths that its replays find)
+        if self._tokens[layer_idx][self._first] < 0 and max(self.sequence_lengths(layer_idx)) < 0 and \
+                not (self.device.type == "cuda" and _capturing()):
+            raise RuntimeError("no slot has a sequence to append to: admit one first")
         self._room(layer_idx, [1] * B)
         if rope is not None:
             rope = tuple(t.reshape(B, 1, self.head_dim) for t in rope)

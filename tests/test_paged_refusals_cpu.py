@@ -135,3 +135,18 @@ def test_the_c_entries_refuse_addresses_that_a_kernel_cannot_read_at(entry, chan
     at = {name: A + off for name, off in changes.items()}
     assert _call_c("paged_" + entry, packer, good, **at) == 1
     assert b"aligned" in _lib.lib.moa_last_error_detail()
+
+
+def test_a_token_for_a_cache_without_any_sequence_is_refused():
+    """A prompt of one token takes the decode step's way."""
+    cache = _cache()
+    cache.release(1)
+    before = _state(cache)
+    with pytest.raises(RuntimeError, match="admit"):
+        _attend(_attention(), cache.slots(1, 2), 1)
+    assert _state(cache) == before
+    with pytest.raises(RuntimeError, match="CUDA"):       # an idle slot beside another one: its row is zero
+        _attend(_attention(), cache, 1)
+    cache.release(0)
+    with pytest.raises(RuntimeError, match="admit"):
+        _attend(_attention(), cache, 1)
